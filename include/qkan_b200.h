@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define QK_ABI_VERSION 4
+#define QK_ABI_VERSION 5
 
 enum QkDtype { QK_F32 = 0, QK_BF16 = 1 };
 
@@ -218,6 +218,76 @@ int qk_pz_forward_noalloc(const QkDesc* desc, const void* x, const float* theta,
                           const float* preacts_weight, const float* preacts_bias,
                           const void* postact_weights, const void* postact_bias,
                           const void* base_weight, const void* mask, void* y, void* cuda_stream);
+
+/*
+ * Dense operators of the hybrid block (Linear -> QKAN -> Linear, src/qkan/solver/cute/cute_ops.py:449-490) and of the
+ * Linear-SiLU-Linear head (src/qkan/qkan.py:1170-1211): the linear map with bias, activation and residual in its
+ * epilogue, and layer norm, each with its backward pass. All tensors are contiguous and row-major; pointers need the
+ * alignment of their element only (16-byte aligned rows take faster paths). Gradients are OVERWRITTEN, summed in a
+ * fixed order (run-to-run bitwise reproducible), and written in the type of the tensor that they belong to.
+ */
+enum QkActivation {
+    QK_ACT_NONE = 0,
+    QK_ACT_SILU = 1,
+    QK_ACT_GELU = 2,      /* x/2 (1 + erf(x/sqrt 2)) */
+    QK_ACT_GELU_TANH = 3, /* x/2 (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) */
+    QK_ACT_RELU = 4,
+    QK_ACT_TANH = 5,
+    QK_ACT_SIGMOID = 6
+};
+
+typedef struct QkLinearDesc {
+    int32_t rows;         /* M */
+    int32_t in_features;  /* K */
+    int32_t out_features; /* N */
+    int32_t io_dtype;     /* QkDtype of every tensor but the tape */
+    int32_t activation;   /* QkActivation */
+    uint32_t flags;       /* 0 */
+} QkLinearDesc;
+
+/*
+ * y (M,N) = act(x (M,K) weight (N,K)^T + bias (N)) + residual (M,N); bias and residual may be NULL.
+ * tape (M,N), NULL when no backward follows or the activation is QK_ACT_NONE: the argument of the activation, for
+ * qk_linear_backward. It is float32 for QK_F32 and IEEE half for QK_BF16: three more bits than bfloat16 where the
+ * activations bend. A finite value beyond half's range is held at its largest, and one below its smallest at plus or
+ * minus that, so that no sign is lost. Products and sums: float32, for QK_F32 to float32 accuracy.
+ * y may not overlap an input. in_features == 0 gives act(bias) + residual.
+ */
+size_t qk_linear_forward_workspace_bytes(const QkLinearDesc* desc);
+int qk_linear_forward(const QkLinearDesc* desc, const void* x, const void* weight, const void* bias,
+                      const void* residual, void* y, void* tape, void* workspace, size_t workspace_bytes,
+                      void* cuda_stream);
+
+/*
+ * With gz = grad_y * act'(tape): grad_x (M,K) = gz weight, grad_weight (N,K) = gz^T x, grad_bias (N) = column sums of
+ * gz. Any of the three may be NULL; x and weight are read only by the gradient that needs them. The gradient of the
+ * residual is grad_y itself.
+ */
+size_t qk_linear_backward_workspace_bytes(const QkLinearDesc* desc);
+int qk_linear_backward(const QkLinearDesc* desc, const void* x, const void* weight, const void* tape,
+                       const void* grad_y, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                       size_t workspace_bytes, void* cuda_stream);
+
+typedef struct QkNormDesc {
+    int32_t rows;        /* M */
+    int32_t dim;         /* D >= 1, the normalised axis */
+    int32_t io_dtype;    /* QkDtype of x, y, grad_y, grad_x */
+    int32_t param_dtype; /* QkDtype of weight, bias and their gradients */
+    float eps;           /* added to the variance; >= 0 */
+    uint32_t flags;      /* 0 */
+} QkNormDesc;
+
+/*
+ * y = (x - mean) * rstd * weight + bias over rows of `dim` elements, mean and rstd = 1/sqrt(var + eps) in float32 with
+ * the biased variance taken about the mean. weight and bias may be NULL (ones, zeros). stats (M,2) float32 receives
+ * (mean, rstd) for the backward; NULL when none follows.
+ */
+int qk_layer_norm_forward(const QkNormDesc* desc, const void* x, const void* weight, const void* bias, void* y,
+                          float* stats, void* cuda_stream);
+size_t qk_layer_norm_backward_workspace_bytes(const QkNormDesc* desc);
+int qk_layer_norm_backward(const QkNormDesc* desc, const void* x, const void* weight, const float* stats,
+                           const void* grad_y, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                           size_t workspace_bytes, void* cuda_stream);
 
 /*
  * Developer overrides of the tile choice, process-wide; no counterpart in the reference (its batch-tile

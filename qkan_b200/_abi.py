@@ -7,9 +7,9 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import Structure, c_char_p, c_int, c_int32, c_size_t, c_uint32, c_void_p
+from ctypes import Structure, c_char_p, c_float, c_int, c_int32, c_size_t, c_uint32, c_void_p
 
-QK_ABI_VERSION = 4
+QK_ABI_VERSION = 5
 
 QK_F32 = 0
 QK_BF16 = 1
@@ -19,6 +19,12 @@ QK_ANSATZ_RPZ = 1
 QK_ANSATZ_REAL = 2
 ANSATZ_CODES = {"pz_encoding": QK_ANSATZ_PZ, "pz": QK_ANSATZ_PZ, "rpz_encoding": QK_ANSATZ_RPZ,
                 "rpz": QK_ANSATZ_RPZ, "real": QK_ANSATZ_REAL}
+
+(QK_ACT_NONE, QK_ACT_SILU, QK_ACT_GELU, QK_ACT_GELU_TANH, QK_ACT_RELU, QK_ACT_TANH, QK_ACT_SIGMOID) = range(7)
+# the names of layer.make_base_activation, and "none"
+ACTIVATION_CODES = {"none": QK_ACT_NONE, "silu": QK_ACT_SILU, "swish": QK_ACT_SILU, "gelu": QK_ACT_GELU,
+                    "gelu_exact": QK_ACT_GELU, "gelu_tanh": QK_ACT_GELU_TANH, "relu": QK_ACT_RELU,
+                    "tanh": QK_ACT_TANH, "sigmoid": QK_ACT_SIGMOID}
 
 QK_PREACT_TRAINABLE = 1
 QK_FAST_MEASURE = 2
@@ -55,6 +61,13 @@ SYMBOLS = {
     "qk_pz_backward_prepared": (c_int, [_P, _P, _P, c_size_t, _P, _P, _P, c_int] + [_P] * 8 + [_P, c_size_t, _P]),
     "qk_edge_stats_scratch_bytes": (c_size_t, [_P]),
     "qk_pz_edge_stats": (c_int, [_P, _P, _P, c_size_t, c_int, _P, _P, c_size_t, _P]),
+    "qk_linear_forward_workspace_bytes": (c_size_t, [_P]),
+    "qk_linear_forward": (c_int, [_P] * 7 + [_P, c_size_t, _P]),
+    "qk_linear_backward_workspace_bytes": (c_size_t, [_P]),
+    "qk_linear_backward": (c_int, [_P] * 8 + [_P, c_size_t, _P]),
+    "qk_layer_norm_forward": (c_int, [_P] * 7),
+    "qk_layer_norm_backward_workspace_bytes": (c_size_t, [_P]),
+    "qk_layer_norm_backward": (c_int, [_P] * 8 + [_P, c_size_t, _P]),
     "qk_debug_set": (None, [c_int, c_int]),
     "qk_noalloc_max_scratch_bytes": (c_size_t, []),
     "qk_noalloc_last_error": (c_char_p, []),
@@ -73,6 +86,28 @@ class QkDesc(Structure):
         ("flags", c_uint32),
         ("ansatz", c_int32),
         ("group", c_int32),
+    ]
+
+
+class QkLinearDesc(Structure):
+    _fields_ = [
+        ("rows", c_int32),
+        ("in_features", c_int32),
+        ("out_features", c_int32),
+        ("io_dtype", c_int32),
+        ("activation", c_int32),
+        ("flags", c_uint32),
+    ]
+
+
+class QkNormDesc(Structure):
+    _fields_ = [
+        ("rows", c_int32),
+        ("dim", c_int32),
+        ("io_dtype", c_int32),
+        ("param_dtype", c_int32),
+        ("eps", c_float),
+        ("flags", c_uint32),
     ]
 
 
@@ -122,9 +157,9 @@ def check(rc: int, what: str) -> None:
     raise QkanLibraryError(msg)
 
 
-def desc_pointer(desc: QkDesc):
+def desc_pointer(desc: Structure):
     return ctypes.cast(ctypes.pointer(desc), c_void_p)
 
 
 __all__ = [name for name in dir() if name.startswith("QK") or name in (
-    "QkDesc", "QkanLibraryError", "ANSATZ_CODES", "load", "last_error", "check", "desc_pointer", "SYMBOLS", "LIB_PATH")]
+    "QkDesc", "QkLinearDesc", "QkNormDesc", "QkanLibraryError", "ANSATZ_CODES", "ACTIVATION_CODES", "load", "last_error", "check", "desc_pointer", "SYMBOLS", "LIB_PATH")]

@@ -9,9 +9,10 @@
 #include "qk_kernels.cuh"
 
 namespace {
-
 thread_local char g_err[512] = "";
+}
 
+namespace qk {
 int fail(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
@@ -19,6 +20,22 @@ int fail(int code, const char* fmt, ...) {
     va_end(ap);
     return code;
 }
+int cuda_fail(cudaError_t e, const char* what) {
+    return fail(QK_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
+}
+int check_buffer(const void* p, size_t have, size_t need, const char* what) {
+    if (!p || have < need)
+        return fail(QK_ERR_WORKSPACE, "%s too small: need %zu bytes, got %zu", what, need, p ? have : (size_t)0);
+    if ((uintptr_t)p % 256) return fail(QK_ERR_WORKSPACE, "%s must be 256-byte aligned", what);
+    return QK_OK;
+}
+}  // namespace qk
+
+namespace {
+
+using qk::check_buffer;
+using qk::cuda_fail;
+using qk::fail;
 
 int check_desc(const QkDesc* d) {
     if (!d) return fail(QK_ERR_BAD_ARGUMENT, "desc is NULL");
@@ -122,17 +139,6 @@ Scratch scratch_layout(const QkDesc& d) {
 bool empty(const QkDesc& d) { return d.batch == 0 || d.in_dim == 0 || d.out_dim == 0; }
 // the prepared state has no batch axis: only a layer without edges has nothing to prepare
 bool no_edges(const QkDesc& d) { return d.in_dim == 0 || d.out_dim == 0; }
-
-int cuda_fail(cudaError_t e, const char* what) {
-    return fail(QK_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
-}
-
-int check_buffer(const void* p, size_t have, size_t need, const char* what) {
-    if (!p || have < need)
-        return fail(QK_ERR_WORKSPACE, "%s too small: need %zu bytes, got %zu", what, need, p ? have : (size_t)0);
-    if ((uintptr_t)p % 256) return fail(QK_ERR_WORKSPACE, "%s must be 256-byte aligned", what);
-    return QK_OK;
-}
 
 // `edges`: solver-contract mode (no epilogue: weight 1, no bias, no base term, no mask)
 int run_prepare(const QkDesc* desc, const float* theta, const float* pw, const float* pb, const void* postw,

@@ -1,0 +1,131 @@
+// Shared pieces of the dense operators (layer norm, linear map with epilogue): typed loads, activations, argument
+// blocks and launchers.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "qk_kernels.cuh"
+
+namespace qk {
+
+constexpr int kSms = 148;
+
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// one element of a tensor whose QkDtype is known at run time only
+__device__ __forceinline__ float load_dt(const void* p, size_t i, int dtype) {
+    return dtype == QK_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i])
+                            : static_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ void store_dt(void* p, size_t i, int dtype, float v) {
+    if (dtype == QK_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+    else static_cast<float*>(p)[i] = v;
+}
+inline size_t dtype_bytes(int dtype) { return dtype == QK_BF16 ? 2 : 4; }
+
+struct NormArgs {
+    int rows, dim, io_dtype, param_dtype;
+    float eps;
+    const void* x;
+    const void* w;  // nullptr: ones
+    const void* b;  // nullptr: zeros
+    void* y;
+    float2* stats_out;     // (mean, rstd) of each row; nullptr: not wanted
+    const float2* stats;
+    const void* gy;
+    void* gx;              // nullptr: not wanted
+    void* gw;
+    void* gb;
+    float* part;           // [2][slices][dim] partial sums of gw, gb
+};
+// slices of the backward's partial sums for this problem
+int norm_slices(int rows, int dim);
+cudaError_t launch_norm_forward(const NormArgs& a, cudaStream_t st);
+cudaError_t launch_norm_backward(const NormArgs& a, cudaStream_t st);
+
+// ---- linear map --------------------------------------------------------------
+// act(z) and its derivative, float32, by CUDA's own functions
+__device__ __forceinline__ float sigmoid_of(float z) { return 1.f / (1.f + expf(-z)); }
+__device__ __forceinline__ float activate(float z, int act) {
+    switch (act) {
+        case QK_ACT_SILU: return z / (1.f + expf(-z));
+        case QK_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+        case QK_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(0.79788456080286536f * fmaf(0.044715f * z * z, z, z)));
+        case QK_ACT_RELU: return z < 0.f ? 0.f : z;  // a NaN stays one
+        case QK_ACT_TANH: return tanhf(z);
+        case QK_ACT_SIGMOID: return sigmoid_of(z);
+        default: return z;
+    }
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+    switch (act) {
+        case QK_ACT_SILU: {
+            const float s = sigmoid_of(z);
+            return s * fmaf(z, 1.f - s, 1.f);
+        }
+        case QK_ACT_GELU:
+            return fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
+        case QK_ACT_GELU_TANH: {
+            const float t = tanhf(0.79788456080286536f * fmaf(0.044715f * z * z, z, z));
+            return 0.5f * (1.f + t) +
+                   0.5f * z * (1.f - t * t) * 0.79788456080286536f * fmaf(3.f * 0.044715f * z, z, 1.f);
+        }
+        case QK_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+        case QK_ACT_TANH: {
+            const float t = tanhf(z);
+            return 1.f - t * t;
+        }
+        case QK_ACT_SIGMOID: {
+            const float s = sigmoid_of(z);
+            return s * (1.f - s);
+        }
+        default: return 1.f;
+    }
+}
+
+// The tape: float32, or half for bfloat16 activations. Rounding an argument of the activation to half moves it by at
+// most 2^-12 of itself (2^-9 in bfloat16). What half cannot hold keeps its sign: beyond +-65504 every derivative here
+// has reached its limit, and below half's smallest number the value is stored as that (relu asks for z > 0 only).
+__device__ __forceinline__ __half tape_half(float z) {
+    if (fabsf(z) <= 65504.f || z != z) {
+        const __half h = __float2half_rn(z);
+        if (z != 0.f && __half2float(h) == 0.f) return __ushort_as_half(z < 0.f ? 0x8001 : 0x0001);
+        return h;
+    }
+    if (isinf(z)) return __float2half_rn(z);
+    return __float2half_rn(copysignf(65504.f, z));
+}
+__device__ __forceinline__ void store_tape(void* tape, size_t i, int io_dtype, float z) {
+    if (io_dtype == QK_BF16) static_cast<__half*>(tape)[i] = tape_half(z);
+    else static_cast<float*>(tape)[i] = z;
+}
+__device__ __forceinline__ float load_tape(const void* tape, size_t i, int io_dtype) {
+    return io_dtype == QK_BF16 ? __half2float(static_cast<const __half*>(tape)[i]) : static_cast<const float*>(tape)[i];
+}
+
+// What becomes of the sums acc[r,c]: z = acc + bias[c]; tape = z; out = act(z) + residual[r,c]
+struct Epilogue {
+    const void* bias;      // nullptr: none
+    const void* residual;  // nullptr: none; row-major, `cols` wide, like out and tape
+    void* out;
+    void* tape;            // nullptr: not wanted
+    int act, io_dtype;
+};
+__device__ __forceinline__ void finish_element(const Epilogue& e, size_t at, int c, float acc) {
+    float z = acc;
+    if (e.bias) z += load_dt(e.bias, c, e.io_dtype);
+    if (e.tape) store_tape(e.tape, at, e.io_dtype, z);
+    float y = activate(z, e.act);
+    if (e.residual) y += load_dt(e.residual, at, e.io_dtype);
+    store_dt(e.out, at, e.io_dtype, y);
+}
+
+}  // namespace qk

@@ -1,0 +1,147 @@
+// C ABI of the dense operators (see include/qkan_b200.h): argument validation and scratch carving.
+#include "qk_linear.cuh"
+
+namespace {
+
+using qk::check_buffer;
+using qk::cuda_fail;
+using qk::fail;
+
+bool is_dtype(int t) { return t == QK_F32 || t == QK_BF16; }
+
+int check_linear(const QkLinearDesc* d) {
+    if (!d) return fail(QK_ERR_BAD_ARGUMENT, "desc is NULL");
+    if (d->rows < 0 || d->in_features < 0 || d->out_features < 0)
+        return fail(QK_ERR_BAD_ARGUMENT, "negative dimension (rows=%d in=%d out=%d)", d->rows, d->in_features,
+                    d->out_features);
+    if (!is_dtype(d->io_dtype)) return fail(QK_ERR_BAD_ARGUMENT, "io_dtype %d is neither QK_F32 nor QK_BF16", d->io_dtype);
+    if (d->activation < QK_ACT_NONE || d->activation > QK_ACT_SIGMOID)
+        return fail(QK_ERR_BAD_ARGUMENT, "activation %d is not a QkActivation value", d->activation);
+    if (d->flags) return fail(QK_ERR_BAD_ARGUMENT, "unknown flag bits 0x%x", d->flags);
+    return QK_OK;
+}
+
+int check_norm(const QkNormDesc* d) {
+    if (!d) return fail(QK_ERR_BAD_ARGUMENT, "desc is NULL");
+    if (d->rows < 0 || d->dim < 1) return fail(QK_ERR_BAD_ARGUMENT, "rows=%d dim=%d: rows >= 0 and dim >= 1 are wanted", d->rows, d->dim);
+    if (!is_dtype(d->io_dtype) || !is_dtype(d->param_dtype))
+        return fail(QK_ERR_BAD_ARGUMENT, "io_dtype %d / param_dtype %d is neither QK_F32 nor QK_BF16", d->io_dtype, d->param_dtype);
+    if (!(d->eps >= 0.f)) return fail(QK_ERR_BAD_ARGUMENT, "eps must be >= 0");
+    if (d->flags) return fail(QK_ERR_BAD_ARGUMENT, "unknown flag bits 0x%x", d->flags);
+    return QK_OK;
+}
+
+size_t norm_scratch(const QkNormDesc& d) {
+    return qk::align256((size_t)2 * qk::norm_slices(d.rows, d.dim) * d.dim * sizeof(float));
+}
+
+// zeros for a gradient that sums over nothing
+cudaError_t zero(void* p, size_t n, int dtype, cudaStream_t st) {
+    return p && n ? cudaMemsetAsync(p, 0, n * qk::dtype_bytes(dtype), st) : cudaSuccess;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t qk_linear_forward_workspace_bytes(const QkLinearDesc* desc) {
+    return check_linear(desc) ? 0 : qk::linear_forward_scratch(*desc);
+}
+
+int qk_linear_forward(const QkLinearDesc* desc, const void* x, const void* weight, const void* bias,
+                      const void* residual, void* y, void* tape, void* ws, size_t ws_bytes, void* stream) {
+    int rc = check_linear(desc);
+    if (rc) return rc;
+    const QkLinearDesc& d = *desc;
+    if (d.rows == 0 || d.out_features == 0) return QK_OK;
+    if (!y) return fail(QK_ERR_BAD_ARGUMENT, "y is NULL");
+    if (d.in_features && (!x || !weight)) return fail(QK_ERR_BAD_ARGUMENT, "x or weight is NULL");
+    rc = check_buffer(ws, ws_bytes, qk::linear_forward_scratch(d), "workspace");
+    if (rc) return rc;
+    qk::LinearArgs a{};
+    a.rows = d.rows, a.in = d.in_features, a.out = d.out_features, a.act = d.activation, a.io_dtype = d.io_dtype;
+    a.x = x, a.w = weight, a.bias = bias, a.residual = residual, a.y = y;
+    a.tape = d.activation == QK_ACT_NONE ? nullptr : tape;
+    a.scratch = ws;
+    const cudaError_t e = qk::launch_linear_forward(a, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? QK_OK : cuda_fail(e, "linear forward launch");
+}
+
+size_t qk_linear_backward_workspace_bytes(const QkLinearDesc* desc) {
+    return check_linear(desc) ? 0 : qk::linear_backward_scratch(*desc);
+}
+
+int qk_linear_backward(const QkLinearDesc* desc, const void* x, const void* weight, const void* tape, const void* gy,
+                       void* gx, void* gw, void* gb, void* ws, size_t ws_bytes, void* stream) {
+    int rc = check_linear(desc);
+    if (rc) return rc;
+    const QkLinearDesc& d = *desc;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (d.in_features == 0) gx = gw = nullptr;  // empty tensors
+    if (d.rows == 0 || d.out_features == 0) {  // sums over nothing
+        cudaError_t e = zero(gx, (size_t)d.rows * d.in_features, d.io_dtype, st);
+        if (e == cudaSuccess) e = zero(gw, (size_t)d.out_features * d.in_features, d.io_dtype, st);
+        if (e == cudaSuccess) e = zero(gb, d.out_features, d.io_dtype, st);
+        return e == cudaSuccess ? QK_OK : cuda_fail(e, "memset gradients");
+    }
+    if (!gx && !gw && !gb) return QK_OK;
+    if (!gy) return fail(QK_ERR_BAD_ARGUMENT, "grad_y is NULL");
+    if (d.activation != QK_ACT_NONE && !tape) return fail(QK_ERR_BAD_ARGUMENT, "tape is NULL");
+    if ((gx && !weight) || (gw && !x)) return fail(QK_ERR_BAD_ARGUMENT, "x or weight is NULL");
+    rc = check_buffer(ws, ws_bytes, qk::linear_backward_scratch(d), "workspace");
+    if (rc) return rc;
+    qk::LinearArgs a{};
+    a.rows = d.rows, a.in = d.in_features, a.out = d.out_features, a.act = d.activation, a.io_dtype = d.io_dtype;
+    a.x = x, a.w = weight, a.tape = const_cast<void*>(tape), a.gy = gy;
+    a.gx = gx, a.gw = gw, a.gb = gb, a.scratch = ws;
+    const cudaError_t e = qk::launch_linear_backward(a, st);
+    return e == cudaSuccess ? QK_OK : cuda_fail(e, "linear backward launch");
+}
+
+int qk_layer_norm_forward(const QkNormDesc* desc, const void* x, const void* weight, const void* bias, void* y,
+                          float* stats, void* stream) {
+    const int rc = check_norm(desc);
+    if (rc) return rc;
+    const QkNormDesc& d = *desc;
+    if (d.rows == 0) return QK_OK;
+    if (!x || !y) return fail(QK_ERR_BAD_ARGUMENT, "x or y is NULL");
+    qk::NormArgs a{};
+    a.rows = d.rows, a.dim = d.dim, a.io_dtype = d.io_dtype, a.param_dtype = d.param_dtype, a.eps = d.eps;
+    a.x = x, a.w = weight, a.b = bias, a.y = y;
+    a.stats_out = reinterpret_cast<float2*>(stats);
+    const cudaError_t e = qk::launch_norm_forward(a, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? QK_OK : cuda_fail(e, "layer norm forward launch");
+}
+
+size_t qk_layer_norm_backward_workspace_bytes(const QkNormDesc* desc) {
+    if (check_norm(desc)) return 0;
+    return desc->rows == 0 ? 256 : norm_scratch(*desc);
+}
+
+int qk_layer_norm_backward(const QkNormDesc* desc, const void* x, const void* weight, const float* stats,
+                           const void* gy, void* gx, void* gw, void* gb, void* ws, size_t ws_bytes, void* stream) {
+    int rc = check_norm(desc);
+    if (rc) return rc;
+    const QkNormDesc& d = *desc;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (d.rows == 0) {
+        cudaError_t e = zero(gw, d.dim, d.param_dtype, st);
+        if (e == cudaSuccess) e = zero(gb, d.dim, d.param_dtype, st);
+        return e == cudaSuccess ? QK_OK : cuda_fail(e, "memset gradients");
+    }
+    if (!gx && !gw && !gb) return QK_OK;
+    if (!x || !stats || !gy) return fail(QK_ERR_BAD_ARGUMENT, "x, stats or grad_y is NULL");
+    qk::NormArgs a{};
+    a.rows = d.rows, a.dim = d.dim, a.io_dtype = d.io_dtype, a.param_dtype = d.param_dtype, a.eps = d.eps;
+    a.x = x, a.w = weight, a.gy = gy, a.gx = gx, a.gw = gw, a.gb = gb;
+    a.stats = reinterpret_cast<const float2*>(stats);
+    if (gw || gb) {
+        rc = check_buffer(ws, ws_bytes, norm_scratch(d), "workspace");
+        if (rc) return rc;
+        a.part = static_cast<float*>(ws);
+    }
+    const cudaError_t e = qk::launch_norm_backward(a, st);
+    return e == cudaSuccess ? QK_OK : cuda_fail(e, "layer norm backward launch");
+}
+
+}  // extern "C"

@@ -5,6 +5,11 @@
 
 namespace qk {
 
+// Error reporting of the C entry points (qk_api.cu): sets the text behind qk_last_error() and returns `code`.
+int fail(int code, const char* fmt, ...);
+int cuda_fail(cudaError_t e, const char* what);
+int check_buffer(const void* p, size_t have, size_t need, const char* what);
+
 struct PrepArgs {
     int in_dim, out_dim, reps, ipad;
     int rk;      // compiled_reps(ansatz, reps): the table is laid out for this repetition count

@@ -475,3 +475,232 @@ def qkan_postacts(x, theta, preacts_weight, preacts_bias, *, preact_trainable: b
     O = theta.shape[0] if theta.dim() == 4 else out_dim
     return _PostactsFunction.apply(x, theta, preacts_weight, preacts_bias, preact_trainable,
                                    fast_measure, ansatz, resolve_precise(precise, x, O), out_dim)
+
+
+# ---------------------------------------------------------------------------- dense operators
+def _activation_code(activation) -> int:
+    try:
+        return _abi.ACTIVATION_CODES["none" if activation is None else activation.lower()]
+    except (KeyError, AttributeError):
+        raise ValueError(
+            f"Unknown activation {activation!r}. Supported: {sorted(_abi.ACTIVATION_CODES)}") from None
+
+
+def _check_like(t: Optional[torch.Tensor], name: str, shape, dtype: torch.dtype, dev: torch.device) -> None:
+    if t is not None and (t.shape != shape or t.dtype != dtype or t.device != dev):
+        raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)} on {dev}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _rows_of(x: torch.Tensor, name: str) -> int:
+    """Number of rows of ``x`` seen as a matrix over its last axis; the kernels count rows and columns in 32 bits."""
+    if x.dim() < 1:
+        raise ValueError(f"{name} must have at least one dimension")
+    rows = 1
+    for n in x.shape[:-1]:
+        rows *= n
+    if max(rows, x.shape[-1]) >= 1 << 31:
+        raise ValueError(f"{name} {tuple(x.shape)}: rows and columns must stay below 2**31")
+    return rows
+
+
+def _call(dev: torch.device, fn, what: str, *args) -> None:
+    """Run a C entry point, its last argument the current stream of ``dev``, with that device current."""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _abi.check(rc, what)
+
+
+def _linear_desc(x: torch.Tensor, weight: torch.Tensor, code: int) -> _abi.QkLinearDesc:
+    _require_cuda(x, "x")
+    io = _io_dtype(x)
+    if weight.dim() != 2:
+        raise ValueError(f"weight must be (out_features, in_features), got {tuple(weight.shape)}")
+    rows = _rows_of(x, "x")
+    N, K = weight.shape
+    if x.shape[-1] != K:
+        raise ValueError(f"x {tuple(x.shape)} does not match weight {tuple(weight.shape)}")
+    _check_like(weight, "weight", weight.shape, x.dtype, x.device)
+    if N >= 1 << 31:
+        raise ValueError("out_features must stay below 2**31")
+    return _abi.QkLinearDesc(rows, K, N, io, code, 0)
+
+
+def linear_forward(x, weight, bias=None, *, activation="none", residual=None, return_tape: bool = False):
+    """``act(x weight^T + bias) + residual`` on the last axis of ``x``; no autograd (see ``fused_linear``).
+
+    ``x (..., K)``, ``weight (N, K)``, ``bias (N,)`` and ``residual (..., N)`` share one dtype, float32 or bfloat16.
+    ``return_tape=True`` returns ``(y, tape)``: what ``linear_backward`` needs of the activation's argument (None for
+    ``activation="none"``).
+    """
+    lib = _abi.load()
+    code = _activation_code(activation)
+    desc = _linear_desc(x, weight, code)
+    dev, dt = x.device, x.dtype
+    shape = x.shape[:-1] + weight.shape[:1]
+    _check_like(bias, "bias", weight.shape[:1], dt, dev)
+    _check_like(residual, "residual", shape, dt, dev)
+    x, weight = x.detach().contiguous(), weight.detach().contiguous()
+    bias = None if bias is None else bias.detach().contiguous()
+    residual = None if residual is None else residual.detach().contiguous()
+    y = torch.empty(shape, dtype=dt, device=dev)
+    tape = None
+    if return_tape and code != _abi.QK_ACT_NONE:
+        tape = torch.empty(shape, dtype=torch.float32 if dt == torch.float32 else torch.float16, device=dev)
+    dp = _abi.desc_pointer(desc)
+    ws = _workspace(dev, lib.qk_linear_forward_workspace_bytes(dp))
+    _call(dev, lib.qk_linear_forward, "qk_linear_forward", dp, _ptr(x), _ptr(weight), _ptr(bias), _ptr(residual),
+          _ptr(y), _ptr(tape), _ptr(ws), ws.numel())
+    return (y, tape) if return_tape else y
+
+
+def linear_backward(x, weight, gy, *, tape=None, activation="none", want=("x", "weight", "bias")) -> dict:
+    """Gradients of ``sum(linear_forward(x, weight, bias, ...) * gy)`` by name; the residual's is ``gy`` itself.
+
+    ``tape`` is what the forward returned with the same ``activation``.
+    """
+    lib = _abi.load()
+    code = _activation_code(activation)
+    desc = _linear_desc(x, weight, code)
+    dev, dt = x.device, x.dtype
+    unknown = set(want) - {"x", "weight", "bias"}
+    if unknown:
+        raise ValueError(f"unknown gradients {sorted(unknown)}")
+    shape = x.shape[:-1] + weight.shape[:1]
+    _check_like(gy, "gy", shape, dt, dev)
+    if code != _abi.QK_ACT_NONE:
+        if tape is None:
+            raise ValueError(f"activation {activation!r} needs the tape of its forward (return_tape=True)")
+        _check_like(tape, "tape", shape, torch.float32 if dt == torch.float32 else torch.float16, dev)
+        tape = tape.contiguous()
+    else:
+        tape = None
+    x, weight, gy = x.detach().contiguous(), weight.detach().contiguous(), gy.detach().contiguous()
+    shapes = {"x": x.shape, "weight": weight.shape, "bias": weight.shape[:1]}
+    out = {n: torch.empty(shapes[n], dtype=dt, device=dev) for n in want}
+    dp = _abi.desc_pointer(desc)
+    ws = _workspace(dev, lib.qk_linear_backward_workspace_bytes(dp))
+    _call(dev, lib.qk_linear_backward, "qk_linear_backward", dp, _ptr(x), _ptr(weight), _ptr(tape), _ptr(gy),
+          _ptr(out.get("x")), _ptr(out.get("weight")), _ptr(out.get("bias")), _ptr(ws), ws.numel())
+    return out
+
+
+class _LinearFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        y, tape = linear_forward(x, weight, bias, activation=activation, residual=residual, return_tape=True)
+        ctx.save_for_backward(x, weight, tape)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, weight, tape = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        want = tuple(n for n, wanted in zip(("x", "weight", "bias"), need) if wanted)
+        g = linear_backward(x, weight, gy, tape=tape, activation=ctx.activation, want=want) if want else {}
+        return g.get("x"), g.get("weight"), g.get("bias"), gy if need[3] else None, None
+
+
+def fused_linear(x, weight, bias=None, *, activation="none", residual=None) -> torch.Tensor:
+    """Differentiable ``act(x weight^T + bias) + residual`` as one kernel (``linear_forward`` / ``linear_backward``).
+
+    ``activation``: the names of ``layer.make_base_activation``, or "none". With a residual this is the closing
+    projection of a pre-norm block, without one the projections of the reference's ``FusedHQKAN``
+    (``src/qkan/solver/cute/cute_ops.py:449-490``).
+    """
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _LinearFunction.apply(x, weight, bias, residual, activation)
+    return linear_forward(x, weight, bias, activation=activation, residual=residual)
+
+
+def _norm_desc(x: torch.Tensor, weight, bias, eps: float) -> _abi.QkNormDesc:
+    _require_cuda(x, "x")
+    io = _io_dtype(x)
+    rows = _rows_of(x, "x")
+    D = x.shape[-1]
+    if D < 1:
+        raise ValueError("layer_norm needs at least one element per row")
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"eps must be finite and >= 0, got {eps}")
+    param = next((t for t in (weight, bias) if t is not None), x)
+    pdt = _io_dtype(param)
+    _check_like(weight, "weight", x.shape[-1:], param.dtype, x.device)
+    _check_like(bias, "bias", x.shape[-1:], param.dtype, x.device)
+    return _abi.QkNormDesc(rows, D, io, pdt, eps, 0)
+
+
+def layer_norm_forward(x, weight=None, bias=None, *, eps: float = 1e-5, return_stats: bool = True):
+    """Layer norm over the last axis; no autograd (see ``layer_norm``). Returns ``(y, stats)``.
+
+    ``weight`` and ``bias`` ``(D,)`` are float32 or bfloat16, whatever ``x`` is, and share one dtype. ``stats (..., 2)``
+    float32 holds each row's mean and ``1 / sqrt(var + eps)`` for ``layer_norm_backward`` (None without ``return_stats``).
+    """
+    lib = _abi.load()
+    desc = _norm_desc(x, weight, bias, eps)
+    x = x.detach().contiguous()
+    weight = None if weight is None else weight.detach().contiguous()
+    bias = None if bias is None else bias.detach().contiguous()
+    y = torch.empty_like(x)
+    stats = torch.empty(x.shape[:-1] + (2,), dtype=torch.float32, device=x.device) if return_stats else None
+    _call(x.device, lib.qk_layer_norm_forward, "qk_layer_norm_forward", _abi.desc_pointer(desc), _ptr(x), _ptr(weight),
+          _ptr(bias), _ptr(y), _ptr(stats))
+    return y, stats
+
+
+def layer_norm_backward(x, weight, stats, gy, *, want=("x", "weight", "bias"), param_dtype=None) -> dict:
+    """Gradients of ``sum(layer_norm(x, weight, bias) * gy)`` by name, from the statistics of the forward.
+
+    ``weight`` None stands for ones; the parameters' gradients have the weight's dtype, or ``param_dtype`` where there is
+    no weight (default: that of ``x``).
+    """
+    lib = _abi.load()
+    desc = _norm_desc(x, weight, None, 0.0)
+    dev = x.device
+    unknown = set(want) - {"x", "weight", "bias"}
+    if unknown:
+        raise ValueError(f"unknown gradients {sorted(unknown)}")
+    _check_like(gy, "gy", x.shape, x.dtype, dev)
+    _check_like(stats, "stats", x.shape[:-1] + (2,), torch.float32, dev)
+    pdt = weight.dtype if weight is not None else (param_dtype or x.dtype)
+    if pdt not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"parameters are float32 or bfloat16, got {pdt}")
+    desc.param_dtype = _abi.QK_F32 if pdt == torch.float32 else _abi.QK_BF16
+    x, gy, stats = x.detach().contiguous(), gy.detach().contiguous(), stats.contiguous()
+    weight = None if weight is None else weight.detach().contiguous()
+    out = {n: torch.empty_like(x) if n == "x" else torch.empty(x.shape[-1:], dtype=pdt, device=dev) for n in want}
+    dp = _abi.desc_pointer(desc)
+    ws = _workspace(dev, lib.qk_layer_norm_backward_workspace_bytes(dp))
+    _call(dev, lib.qk_layer_norm_backward, "qk_layer_norm_backward", dp, _ptr(x), _ptr(weight), _ptr(stats), _ptr(gy),
+          _ptr(out.get("x")), _ptr(out.get("weight")), _ptr(out.get("bias")), _ptr(ws), ws.numel())
+    return out
+
+
+class _LayerNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, stats = layer_norm_forward(x, weight, bias, eps=eps)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, weight, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        want = tuple(n for n, wanted in zip(("x", "weight", "bias"), need) if wanted)
+        g = layer_norm_backward(x, weight, stats, gy, want=want, param_dtype=ctx.bias_dtype)
+        return g.get("x"), g.get("weight"), g.get("bias"), None
+
+
+def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5) -> torch.Tensor:
+    """Differentiable layer norm over the last axis (``layer_norm_forward`` / ``layer_norm_backward``)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _LayerNormFunction.apply(x, weight, bias, eps)
+    return layer_norm_forward(x, weight, bias, eps=eps, return_stats=False)[0]

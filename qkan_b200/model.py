@@ -20,6 +20,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from .dense import Linear
 from .layer import SOLVER_NAME, QKANLayer, make_base_activation
 from .parallel import get_dist_info, print0
 
@@ -81,7 +82,14 @@ class QKAN(nn.Module):
         # dr_preacts / dr_postacts of shape (B, O, I) that the reference also stores are only materialised
         # when this is switched on (the plotting tools that read them are not part of this package).
         self.keep_edge_acts = bool(kwargs.get("keep_edge_acts", False))
-        if is_map:
+        # fused_head runs the Linear-SiLU-Linear head on the package's kernels, SiLU in the first one's epilogue;
+        # nn.Identity keeps the parameters' names
+        self.fused_head = bool(kwargs.get("fused_head", False))
+        if is_map and self.fused_head:
+            self.layers.append(Linear(width[-2], hidden, device=device, dtype=p_dtype, activation="silu"))
+            self.layers.append(nn.Identity())
+            self.layers.append(Linear(hidden, width[-1], device=device, dtype=p_dtype))
+        elif is_map:
             self.layers.append(nn.Linear(width[-2], hidden, device=device, dtype=p_dtype))
             self.layers.append(nn.SiLU())
             self.layers.append(nn.Linear(hidden, width[-1], device=device, dtype=p_dtype))
@@ -201,7 +209,7 @@ class QKAN(nn.Module):
             ba_trainable=self.ba_trainable, is_batchnorm=self.is_batchnorm, is_map=self.is_map,
             hidden=self.hidden, fast_measure=self.fast_measure, save_act=self.save_act, c_dtype=self.c_dtype,
             p_dtype=self.p_dtype, seed=self.seed, solver_kwargs=self.solver_kwargs, p_dim=self.p_dim,
-            theta_init=self.theta_init)
+            theta_init=self.theta_init, fused_head=self.fused_head)
         return new_model.initialize_from_another_model(self)
 
     def layer_extension(self, new_reps: int) -> "QKAN":
