@@ -223,8 +223,9 @@ int qk_pz_forward_noalloc(const QkDesc* desc, const void* x, const float* theta,
  * Dense operators of the hybrid block (Linear -> QKAN -> Linear, src/qkan/solver/cute/cute_ops.py:449-490) and of the
  * Linear-SiLU-Linear head (src/qkan/qkan.py:1170-1211): the linear map with bias, activation and residual in its
  * epilogue, and layer norm, each with its backward pass. All tensors are contiguous and row-major; pointers need the
- * alignment of their element only (16-byte aligned rows take faster paths). Gradients are OVERWRITTEN, summed in a
- * fixed order (run-to-run bitwise reproducible), and written in the type of the tensor that they belong to.
+ * alignment of their element (stats: 8 bytes), and bfloat16 x, weight and grad_y of the linear map whose rows are a
+ * multiple of 16 bytes have to start on a 16-byte boundary. Gradients are OVERWRITTEN, summed in a fixed order
+ * (run-to-run bitwise reproducible), and written in the type of the tensor that they belong to.
  */
 enum QkActivation {
     QK_ACT_NONE = 0,
@@ -267,6 +268,12 @@ size_t qk_linear_backward_workspace_bytes(const QkLinearDesc* desc);
 int qk_linear_backward(const QkLinearDesc* desc, const void* x, const void* weight, const void* tape,
                        const void* grad_y, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
                        size_t workspace_bytes, void* cuda_stream);
+
+/*
+ * The linear map's kernels bound every wait inside them. QK_OK if none ran out on the current device since the last
+ * call, QK_ERR_LAUNCH otherwise (results since then are not valid). Synchronises `cuda_stream`; not for captures.
+ */
+int qk_dense_status(void* cuda_stream);
 
 typedef struct QkNormDesc {
     int32_t rows;        /* M */

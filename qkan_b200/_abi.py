@@ -65,6 +65,7 @@ SYMBOLS = {
     "qk_linear_forward": (c_int, [_P] * 7 + [_P, c_size_t, _P]),
     "qk_linear_backward_workspace_bytes": (c_size_t, [_P]),
     "qk_linear_backward": (c_int, [_P] * 8 + [_P, c_size_t, _P]),
+    "qk_dense_status": (c_int, [_P]),
     "qk_layer_norm_forward": (c_int, [_P] * 7),
     "qk_layer_norm_backward_workspace_bytes": (c_size_t, [_P]),
     "qk_layer_norm_backward": (c_int, [_P] * 8 + [_P, c_size_t, _P]),

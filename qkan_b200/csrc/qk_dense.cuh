@@ -13,6 +13,7 @@ constexpr int kSms = 148;
 
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
 template <typename T>
 __device__ __forceinline__ T from_float(float v);
 template <>

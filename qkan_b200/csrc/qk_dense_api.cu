@@ -31,6 +31,13 @@ int check_norm(const QkNormDesc* d) {
     return QK_OK;
 }
 
+// The products read bfloat16 rows of whole 16-byte words where they lie, by TMA, which wants them aligned.
+int check_aligned(const void* p, int width, int io_dtype, const char* what) {
+    if (qk::reads_in_place(width, io_dtype) && (uintptr_t)p % 16)
+        return fail(QK_ERR_BAD_ARGUMENT, "%s must be 16-byte aligned (its rows are whole 16-byte words)", what);
+    return QK_OK;
+}
+
 size_t norm_scratch(const QkNormDesc& d) {
     return qk::align256((size_t)2 * qk::norm_slices(d.rows, d.dim) * d.dim * sizeof(float));
 }
@@ -56,6 +63,8 @@ int qk_linear_forward(const QkLinearDesc* desc, const void* x, const void* weigh
     if (d.rows == 0 || d.out_features == 0) return QK_OK;
     if (!y) return fail(QK_ERR_BAD_ARGUMENT, "y is NULL");
     if (d.in_features && (!x || !weight)) return fail(QK_ERR_BAD_ARGUMENT, "x or weight is NULL");
+    if ((rc = check_aligned(x, d.in_features, d.io_dtype, "x"))) return rc;
+    if ((rc = check_aligned(weight, d.in_features, d.io_dtype, "weight"))) return rc;
     rc = check_buffer(ws, ws_bytes, qk::linear_forward_scratch(d), "workspace");
     if (rc) return rc;
     qk::LinearArgs a{};
@@ -88,6 +97,9 @@ int qk_linear_backward(const QkLinearDesc* desc, const void* x, const void* weig
     if (!gy) return fail(QK_ERR_BAD_ARGUMENT, "grad_y is NULL");
     if (d.activation != QK_ACT_NONE && !tape) return fail(QK_ERR_BAD_ARGUMENT, "tape is NULL");
     if ((gx && !weight) || (gw && !x)) return fail(QK_ERR_BAD_ARGUMENT, "x or weight is NULL");
+    if (gw && (rc = check_aligned(x, d.in_features, d.io_dtype, "x"))) return rc;
+    if (gx && (rc = check_aligned(weight, d.in_features, d.io_dtype, "weight"))) return rc;
+    if ((gx || gw) && (rc = check_aligned(gy, d.out_features, d.io_dtype, "grad_y"))) return rc;
     rc = check_buffer(ws, ws_bytes, qk::linear_backward_scratch(d), "workspace");
     if (rc) return rc;
     qk::LinearArgs a{};
@@ -96,6 +108,13 @@ int qk_linear_backward(const QkLinearDesc* desc, const void* x, const void* weig
     a.gx = gx, a.gw = gw, a.gb = gb, a.scratch = ws;
     const cudaError_t e = qk::launch_linear_backward(a, st);
     return e == cudaSuccess ? QK_OK : cuda_fail(e, "linear backward launch");
+}
+
+int qk_dense_status(void* stream) {
+    unsigned n = 0;
+    const cudaError_t e = qk::gemm_gave_up(&n, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "dense status");
+    return n ? fail(QK_ERR_LAUNCH, "%u waits of the linear map's kernels ran out; their results are not valid", n) : QK_OK;
 }
 
 int qk_layer_norm_forward(const QkNormDesc* desc, const void* x, const void* weight, const void* bias, void* y,

@@ -1,137 +1,469 @@
-// The linear map y = act(x W^T + b) + r and its backward pass: C entry points' launch sequence and the plain kernels.
+// The linear map y = act(x W^T + b) + r and its backward pass: choice of tiles, scratch, launch sequence, and the small
+// kernels around the products of qk_gemm.cu.
+//
+//   prepare   operands that the products cannot read where they lie: float32 is split into three bfloat16 parts, rows
+//             that are no multiple of 16 bytes are padded, and in the backward gz = gy * act'(tape) is formed, with
+//             its column sums for grad_bias on the way
+//   products  forward: one; backward: grad_x and grad_weight in one launch, so that either fills the other's last wave
+//   reduce    adds the slices of a depth that was cut for want of tiles, then the epilogue; adds grad_bias' slabs
 #include "qk_linear.cuh"
 
 namespace qk {
 namespace {
 
-constexpr int kTile = 64, kStep = 16, kThreads = 256;
+constexpr int kThreads = 256;
 
-// C[r,c] = sum_k P[r,k] Q[c,k], any strides: one 64 x 64 tile per CTA, 4 x 4 sums per thread.
+struct PrepJob {
+    const void* src;
+    const void* tape;      // nullptr: the source as it is
+    __nv_bfloat16* dst;    // [parts][rows][ld]; nullptr: column sums only
+    float* colpart;        // [slabs][cols]; nullptr: not wanted
+    int rows, cols, ld, act;
+    int slab_rows, cblocks, tx_log2, blocks;
+    bool vec;              // whole 8-column groups, 16-byte aligned
+};
+struct PrepArgsL {
+    PrepJob job[3];
+    int count;
+};
+
+// x = h + m + l. h is x rounded to nearest, except that a finite x stays finite; m and l round what is left, which
+// is exact in float32. An infinity or a NaN is all in h.
+__device__ __forceinline__ void split3(float x, __nv_bfloat16& h, __nv_bfloat16& m, __nv_bfloat16& l) {
+    h = __float2bfloat16_rn(x);
+    if (__hisinf(h) && isfinite(x)) h = __ushort_as_bfloat16(x < 0.f ? 0xff7f : 0x7f7f);
+    if (!isfinite(x)) {
+        m = l = __float2bfloat16_rn(0.f);
+        return;
+    }
+    const float r = x - __bfloat162float(h);
+    m = __float2bfloat16_rn(r);
+    l = __float2bfloat16_rn(r - __bfloat162float(m));
+}
+
 template <typename IO>
-__global__ void __launch_bounds__(kThreads) product_kernel(const Product g) {
-    __shared__ float ps[kStep][kTile + 1], qs[kStep][kTile + 1];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const long r0 = (long)blockIdx.y * kTile, c0 = (long)blockIdx.x * kTile;
-    const IO* p = static_cast<const IO*>(g.p);
-    const IO* q = static_cast<const IO*>(g.q);
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < g.depth; k0 += kStep) {
-        for (int t = threadIdx.x; t < kTile * kStep; t += kThreads) {
-            // neighbouring threads along the contiguous axis of each operand
-            const int pr = g.p_kmajor ? t / kStep : t % kTile, pk = g.p_kmajor ? t % kStep : t / kTile;
-            const int qc = g.q_kmajor ? t / kStep : t % kTile, qk_ = g.q_kmajor ? t % kStep : t / kTile;
-            const bool pin = r0 + pr < g.rows && k0 + pk < g.depth, qin = c0 + qc < g.cols && k0 + qk_ < g.depth;
-            const size_t pat = g.p_kmajor ? (size_t)(r0 + pr) * g.depth + k0 + pk : (size_t)(k0 + pk) * g.rows + r0 + pr;
-            const size_t qat = g.q_kmajor ? (size_t)(c0 + qc) * g.depth + k0 + qk_ : (size_t)(k0 + qk_) * g.cols + c0 + qc;
-            ps[pk][pr] = pin ? as_float(p[pat]) : 0.f;
-            qs[qk_][qc] = qin ? as_float(q[qat]) : 0.f;
+__device__ __forceinline__ void load8(const void* p, size_t at, bool vec, int n, float (&v)[8]) {
+    const IO* s = static_cast<const IO*>(p) + at;
+    if (vec) {
+        if constexpr (sizeof(IO) == 4) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(s)), b = __ldg(reinterpret_cast<const float4*>(s) + 1);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+            const uint4 a = __ldg(reinterpret_cast<const uint4*>(s));
+            const unsigned u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const IO* q = reinterpret_cast<const IO*>(&u[i]);
+                v[2 * i] = as_float(q[0]), v[2 * i + 1] = as_float(q[1]);
+            }
         }
-        __syncthreads();
+    } else {
 #pragma unroll
-        for (int k = 0; k < kStep; ++k) {
-            float pv[4], qv[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) pv[i] = ps[k][ty * 4 + i], qv[i] = qs[k][tx + 16 * i];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(pv[i], qv[j], acc[i][j]);
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long r = r0 + ty * 4 + i;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const long c = c0 + tx + 16 * j;
-            if (r < g.rows && c < g.cols) finish_element(g.epi, (size_t)r * g.cols + c, (int)c, acc[i][j]);
-        }
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? as_float(s[i]) : 0.f;
     }
 }
 
-// gz = gy * act'(tape)
-__global__ void slope_kernel(const void* gy, const void* tape, void* gz, size_t n, int act, int io_dtype) {
-    for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x)
-        store_dt(gz, i, io_dtype, load_dt(gy, i, io_dtype) * act_slope(load_tape(tape, i, io_dtype), act));
-}
-
-// grad_bias[n] = sum_m gy[m,n] * act'(tape[m,n]): 32 columns per CTA, 32 row slices
-__global__ void __launch_bounds__(1024) column_sum_kernel(const void* gy, const void* tape, void* gb, int rows, int cols,
-                                                          int act, int io_dtype) {
-    __shared__ float tile[32][33];
-    const int c = blockIdx.x * 32 + threadIdx.x;
-    float s = 0.f;
-    if (c < cols)
-        for (long r = threadIdx.y; r < rows; r += 32) {
-            const size_t at = (size_t)r * cols + c;
-            const float g = load_dt(gy, at, io_dtype);
-            s += tape ? g * act_slope(load_tape(tape, at, io_dtype), act) : g;
+// Bound by memory: reads the source once, writes 2 (bfloat16) or 6 (float32) bytes per element. A thread owns eight
+// columns and walks the rows of a slab, so that column sums stay in its registers.
+template <typename IO>
+__global__ void __launch_bounds__(kThreads) prepare_kernel(const PrepArgsL a) {
+    __shared__ float sums[kThreads * 8];
+    int b = blockIdx.x, which = 0;
+    while (which + 1 < a.count && b >= a.job[which].blocks) b -= a.job[which++].blocks;
+    const PrepJob& j = a.job[which];
+    const int tx = threadIdx.x & ((1 << j.tx_log2) - 1), ty = threadIdx.x >> j.tx_log2, ny = kThreads >> j.tx_log2;
+    const int slab = b / j.cblocks, c = ((b - slab * j.cblocks) << j.tx_log2 | tx) * 8;
+    const long end = min((long)j.rows, (long)(slab + 1) * j.slab_rows);
+    const size_t plane = (size_t)j.rows * j.ld;
+    float sum[8] = {};
+    if (c < j.ld) {
+        const int n = min(8, j.cols - c);
+#pragma unroll 2
+        for (long r = (long)slab * j.slab_rows + ty; r < end; r += ny) {
+            const size_t at = (size_t)r * j.cols + c;
+            float v[8];
+            load8<IO>(j.src, at, j.vec, n, v);
+            if (j.tape) {
+                float z[8];
+                if constexpr (sizeof(IO) == 4) load8<float>(j.tape, at, j.vec, n, z);
+                else load8<__half>(j.tape, at, j.vec, n, z);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = i < n ? v[i] * act_slope(z[i], j.act) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += v[i];
+            if (!j.dst) continue;
+            __align__(16) __nv_bfloat16 h[8];
+            uint4* out = reinterpret_cast<uint4*>(j.dst + (size_t)r * j.ld + c);
+            if constexpr (sizeof(IO) == 4) {
+                __align__(16) __nv_bfloat16 m[8], l[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) split3(v[i], h[i], m[i], l[i]);
+                out[plane / 8] = *reinterpret_cast<uint4*>(m);
+                out[plane / 4] = *reinterpret_cast<uint4*>(l);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[i] = __float2bfloat16_rn(v[i]);
+            }
+            out[0] = *reinterpret_cast<uint4*>(h);
         }
-    tile[threadIdx.y][threadIdx.x] = s;
+    }
+    if (!j.colpart) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sums[(ty << j.tx_log2 | tx) * 8 + i] = sum[i];
     __syncthreads();
-    if (threadIdx.y == 0 && c < cols) {
-        for (int k = 1; k < 32; ++k) s += tile[k][threadIdx.x];
-        store_dt(gb, c, io_dtype, s);
+    const int width = 8 << j.tx_log2;
+    for (int t = threadIdx.x; t < width; t += kThreads) {
+        const int col = (b - slab * j.cblocks) * width + t;
+        if (col >= j.cols) break;
+        float s = 0.f;
+        for (int y = 0; y < ny; ++y) s += sums[y * width + t];
+        j.colpart[(size_t)slab * j.cols + col] = s;
     }
 }
 
-cudaError_t launch_product(const Product& g, cudaStream_t st) {
-    if (g.rows == 0 || g.cols == 0) return cudaSuccess;
-    const dim3 grid((g.cols + kTile - 1) / kTile, (g.rows + kTile - 1) / kTile);
-    if (grid.y > 65535) return cudaErrorInvalidConfiguration;
-    if (g.epi.io_dtype == QK_BF16) product_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(g);
-    else product_kernel<float><<<grid, kThreads, 0, st>>>(g);
+struct ReduceJob {
+    const float* part;  // [splits][rows][cols]; splits 0: sums of nothing
+    int splits, cols, blocks;
+    size_t n;
+    Epilogue epi;
+};
+struct ReduceArgs {
+    ReduceJob job[2];
+    int count;
+    const float* colpart;  // [slabs][cols]
+    void* gb;
+    int slabs, cols, io_dtype;
+};
+
+// One element per thread: the slices of its sum in order, then the epilogue. The blocks behind those add grad_bias'
+// slabs, 32 columns each.
+__global__ void __launch_bounds__(kThreads) reduce_kernel(const ReduceArgs a) {
+    int b = blockIdx.x, which = 0;
+    while (which < a.count && b >= a.job[which].blocks) b -= a.job[which++].blocks;
+    if (which < a.count) {
+        const ReduceJob& j = a.job[which];
+        const size_t i = (size_t)b * kThreads + threadIdx.x;
+        if (i >= j.n) return;
+        float s = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < j.splits; ++k) s += __ldg(j.part + (size_t)k * j.n + i);
+        finish_element(j.epi, i, (int)(i % j.cols), s);
+        return;
+    }
+    __shared__ float tile[8][33];
+    const int x = threadIdx.x % 32, y = threadIdx.x / 32, c = b * 32 + x;
+    float s = 0.f;
+    if (c < a.cols)
+        for (int k = y; k < a.slabs; k += 8) s += __ldg(a.colpart + (size_t)k * a.cols + c);
+    tile[y][x] = s;
+    __syncthreads();
+    if (y == 0 && c < a.cols) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) s += tile[k][x];
+        store_dt(a.gb, c, a.io_dtype, s);
+    }
+}
+
+// ---- choice of tiles -----------------------------------------------------------
+// Clocks of one SM, from the rates of its parts: the tensor core takes 2 BN clocks for a 128 x BN x 64 block, six times
+// that in float32; L2 feeds some 56 bytes per clock; the epilogue writes about one row of 128 columns per 12 clocks.
+struct Cut {
+    int splits, kper;
+};
+
+struct Size {
+    long rows, cols;
+    int kblocks;
+    long tiles(int bn) const { return (rows + bn - 1) / bn * ((cols + 127) / 128); }
+};
+
+double block_clocks(int bn, int planes) {
+    const double mma = 2.0 * bn * (planes == 3 ? 6 : 1), load = planes * (16384.0 + (bn < 64 ? 64 : bn) * 128) / 56;
+    return mma > load ? mma : load;
+}
+double drain_clocks(int bn) { return 12.0 * bn + 200; }
+
+Cut cut_into(int kblocks, int splits) {
+    Cut c;
+    c.kper = (kblocks + splits - 1) / splits;
+    c.splits = (kblocks + c.kper - 1) / c.kper;
+    return c;
+}
+
+constexpr int kCuts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 148};
+constexpr long kMostPart = 64l << 20;  // floats of partial sums: 256 MB
+
+// time of `s` alone when it is cut this way, with `other` clocks of work per SM beside it
+double cost_of(const Size& s, int bn, int planes, const Cut& c, double other) {
+    const double units = (double)s.tiles(bn) * c.splits;
+    const double mainloop = c.kper * block_clocks(bn, planes), drain = drain_clocks(bn);
+    const double unit = mainloop > drain ? mainloop : drain;
+    double waves = units * unit / kSms + other;  // filled evenly
+    const double even = (double)((long)(units + kSms - 1) / kSms) * unit;
+    if (other == 0 && even > waves) waves = even;
+    if (unit > waves) waves = unit;
+    double t = waves + drain + 2500;
+    if (c.splits > 1) t += 3500 + 2.0 * c.splits * s.rows * s.cols * 4 / (kSms * 24.0);
+    return t;
+}
+
+Cut best_cut(const Size& s, int bn, int planes, double other, double* cost) {
+    Cut best{1, s.kblocks};
+    *cost = cost_of(s, bn, planes, best, other);
+    for (int k : kCuts) {
+        if (k > s.kblocks || (double)k * s.rows * s.cols > kMostPart) break;
+        if (k > 1 && s.tiles(bn) * k > 4l * kSms) break;
+        const Cut c = cut_into(s.kblocks, k);
+        const double t = cost_of(s, bn, planes, c, other);
+        if (t < *cost) *cost = t, best = c;
+    }
+    return best;
+}
+
+struct Plan {
+    int bn;
+    Cut cut[2];
+    double cost;
+};
+
+// one product, or two in one launch
+Plan plan_for(const Size* s, int count, int planes) {
+    Plan best{};
+    best.cost = 1e300;
+    for (int bn = planes == 3 ? 128 : 256; bn >= 32; bn /= 2) {
+        Plan p{};
+        p.bn = bn;
+        double c0 = 0, c1 = 0;
+        if (count == 1) {
+            p.cut[0] = best_cut(s[0], bn, planes, 0, &c0);
+            p.cost = c0;
+        } else {
+            const double w1 = (double)s[1].tiles(bn) * s[1].kblocks * block_clocks(bn, planes) / kSms;
+            p.cut[0] = best_cut(s[0], bn, planes, w1, &c0);
+            const double w0 = (double)s[0].tiles(bn) * s[0].kblocks * block_clocks(bn, planes) / kSms;
+            p.cut[1] = best_cut(s[1], bn, planes, w0, &c1);
+            p.cost = c0 > c1 ? c0 : c1;
+        }
+        if (p.cost < best.cost) best = p;
+    }
+    return best;
+}
+
+// ---- scratch -------------------------------------------------------------------
+int planes_of(int io_dtype) { return io_dtype == QK_F32 ? 3 : 1; }
+long padded(long n) { return (n + 7) / 8 * 8; }
+size_t packed_bytes(long rows, long cols, int planes) { return align256((size_t)planes * rows * padded(cols) * 2); }
+int blocks_of(long depth) { return (int)((depth + 63) / 64); }
+
+struct Slabs {
+    int rows, count, cblocks, tx_log2;
+};
+// 256 threads as 2^tx_log2 groups of eight columns by the rest in rows; enough slabs of rows for four CTAs per SM, each
+// of eight rows per thread at least
+Slabs slabs_of(long rows, long cols) {
+    const long groups = padded(cols) / 8;
+    Slabs s{};
+    while (s.tx_log2 < 5 && (1 << s.tx_log2) < groups) ++s.tx_log2;
+    s.cblocks = (int)((groups + (1 << s.tx_log2) - 1) >> s.tx_log2);
+    const long ny = kThreads >> s.tx_log2;
+    long want = (4l * kSms + s.cblocks - 1) / s.cblocks;
+    const long most = (rows + 8 * ny - 1) / (8 * ny);
+    if (want > most) want = most;
+    if (want < 1) want = 1;
+    s.rows = (int)((rows + want - 1) / want);
+    s.count = (int)((rows + s.rows - 1) / s.rows);
+    return s;
+}
+
+struct ForwardScratch {
+    Plan plan;
+    size_t x, w, part, total;
+};
+ForwardScratch forward_scratch(const QkLinearDesc& d) {
+    ForwardScratch s{};
+    const int planes = planes_of(d.io_dtype);
+    const bool pack = !reads_in_place(d.in_features, d.io_dtype);
+    const Size size{d.rows, d.out_features, blocks_of(d.in_features)};
+    s.plan = plan_for(&size, 1, planes);
+    s.x = 0;
+    s.w = pack ? packed_bytes(d.rows, d.in_features, planes) : 0;
+    s.part = s.w + (pack ? packed_bytes(d.out_features, d.in_features, planes) : 0);
+    s.total = s.part;
+    if (s.plan.cut[0].splits > 1) s.total += align256((size_t)s.plan.cut[0].splits * d.rows * d.out_features * 4);
+    return s;
+}
+
+// Products 0: grad_weight (its units are the long ones and go first), 1: grad_x. The layout is that of both, whatever
+// is asked for.
+struct BackwardScratch {
+    Plan plan;
+    Slabs slabs;
+    size_t gz, x, w, colpart, part0, part1, total;
+};
+BackwardScratch backward_scratch(const QkLinearDesc& d) {
+    BackwardScratch s{};
+    const int planes = planes_of(d.io_dtype);
+    const long M = d.rows, K = d.in_features, N = d.out_features;
+    const bool pack_gz = d.activation != QK_ACT_NONE || !reads_in_place(N, d.io_dtype);
+    const bool pack = !reads_in_place(K, d.io_dtype);
+    const Size size[2] = {{N, K, blocks_of(M)}, {M, K, blocks_of(N)}};
+    s.plan = plan_for(size, 2, planes);
+    s.slabs = slabs_of(M, N);
+    s.gz = 0;
+    s.x = pack_gz ? packed_bytes(M, N, planes) : 0;
+    s.w = s.x + (pack ? packed_bytes(M, K, planes) : 0);
+    s.colpart = s.w + (pack ? packed_bytes(N, K, planes) : 0);
+    s.part0 = s.colpart + align256((size_t)s.slabs.count * N * 4);
+    s.part1 = s.part0 + (s.plan.cut[0].splits > 1 ? align256((size_t)s.plan.cut[0].splits * N * K * 4) : 0);
+    s.total = s.part1 + (s.plan.cut[1].splits > 1 ? align256((size_t)s.plan.cut[1].splits * M * K * 4) : 0);
+    return s;
+}
+
+// ---- launches ------------------------------------------------------------------
+PrepJob prep_job(const void* src, const void* tape, void* dst, float* colpart, int rows, int cols, int act, int io_dtype) {
+    PrepJob j{};
+    const Slabs s = slabs_of(rows, cols);
+    j.src = src, j.tape = tape, j.dst = static_cast<__nv_bfloat16*>(dst), j.colpart = colpart;
+    j.rows = rows, j.cols = cols, j.ld = (int)padded(cols), j.act = act;
+    j.slab_rows = s.rows, j.cblocks = s.cblocks, j.tx_log2 = s.tx_log2, j.blocks = s.cblocks * s.count;
+    j.vec = cols % 8 == 0 && (uintptr_t)src % 16 == 0 && (uintptr_t)tape % 16 == 0;
+    return j;
+}
+
+cudaError_t launch_prepare(const PrepArgsL& p, int io_dtype, cudaStream_t st) {
+    long blocks = 0;
+    for (int i = 0; i < p.count; ++i) blocks += p.job[i].blocks;
+    if (blocks == 0) return cudaSuccess;
+    if (io_dtype == QK_BF16) prepare_kernel<__nv_bfloat16><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+    else prepare_kernel<float><<<(unsigned)blocks, kThreads, 0, st>>>(p);
     return cudaPeekAtLastError();
+}
+
+cudaError_t launch_reduce(const ReduceArgs& r, cudaStream_t st) {
+    long blocks = 0;
+    for (int i = 0; i < r.count; ++i) blocks += r.job[i].blocks;
+    if (r.gb) blocks += (r.cols + 31) / 32;
+    if (blocks == 0) return cudaSuccess;
+    if (blocks > 0x7fffffffl) return cudaErrorInvalidConfiguration;
+    reduce_kernel<<<(unsigned)blocks, kThreads, 0, st>>>(r);
+    return cudaPeekAtLastError();
+}
+
+void add_reduce(ReduceArgs& r, const float* part, int splits, int rows, int cols, const Epilogue& epi) {
+    ReduceJob& j = r.job[r.count++];
+    j.part = part, j.splits = splits, j.cols = cols, j.epi = epi;
+    j.n = (size_t)rows * cols;
+    j.blocks = (int)((j.n + kThreads - 1) / kThreads);
+}
+
+// an operand of `rows` x `cols`, packed or as it is
+Operand operand(const void* base, int rows, int cols, bool packed, bool mn_major) {
+    return {base, cols, rows, packed ? padded(cols) : (long)cols, mn_major};
+}
+
+bool set_problem(GemmProblem& g, int rows, int cols, int kblocks, const Plan& plan, const Cut& cut, const Operand& p,
+                 const Operand& q, int planes, float* part, const Epilogue& epi) {
+    g.rows = rows, g.cols = cols;
+    g.kblocks = kblocks, g.kper = cut.kper, g.splits = cut.splits;
+    g.tiles_r = (rows + plan.bn - 1) / plan.bn, g.tiles_c = (cols + 127) / 128;
+    const long units = (long)g.tiles_r * g.tiles_c * g.splits;
+    if (units > 0x3fffffff) return false;
+    g.units = (int)units;
+    g.part = cut.splits > 1 ? part : nullptr;
+    g.epi = epi;
+    return gemm_bind(g, p, q, planes, plan.bn);
 }
 
 }  // namespace
 
-size_t linear_forward_scratch(const QkLinearDesc&) { return 256; }
+size_t linear_forward_scratch(const QkLinearDesc& d) {
+    if (d.rows == 0 || d.out_features == 0 || d.in_features == 0) return 256;
+    const size_t n = forward_scratch(d).total;
+    return n ? n : 256;
+}
 
 size_t linear_backward_scratch(const QkLinearDesc& d) {
-    if (d.activation == QK_ACT_NONE) return 256;
-    return align256((size_t)d.rows * d.out_features * dtype_bytes(d.io_dtype));
+    if (d.rows == 0 || d.out_features == 0) return 256;
+    return backward_scratch(d).total;
 }
 
 cudaError_t launch_linear_forward(const LinearArgs& a, cudaStream_t st) {
-    Product g{};
-    g.rows = a.rows, g.cols = a.out, g.depth = a.in;
-    g.p = a.x, g.q = a.w;
-    g.p_kmajor = g.q_kmajor = true;
-    g.epi = {a.bias, a.residual, a.y, a.tape, a.act, a.io_dtype};
-    return launch_product(g, st);
+    const int M = a.rows, K = a.in, N = a.out, planes = planes_of(a.io_dtype);
+    const Epilogue epi{a.bias, a.residual, a.y, a.tape, a.act, a.io_dtype};
+    ReduceArgs red{};
+    if (K == 0) {
+        add_reduce(red, nullptr, 0, M, N, epi);
+        return launch_reduce(red, st);
+    }
+    const QkLinearDesc d{M, K, N, a.io_dtype, a.act, 0};
+    const ForwardScratch s = forward_scratch(d);
+    char* ws = static_cast<char*>(a.scratch);
+    const bool pack = !reads_in_place(K, a.io_dtype);
+    const void *x = a.x, *w = a.w;
+    cudaError_t e = cudaSuccess;
+    if (pack) {
+        PrepArgsL p{};
+        p.job[p.count++] = prep_job(a.x, nullptr, ws + s.x, nullptr, M, K, 0, a.io_dtype);
+        p.job[p.count++] = prep_job(a.w, nullptr, ws + s.w, nullptr, N, K, 0, a.io_dtype);
+        e = launch_prepare(p, a.io_dtype, st);
+        if (e != cudaSuccess) return e;
+        x = ws + s.x, w = ws + s.w;
+    }
+    GemmArgs g{};
+    float* part = reinterpret_cast<float*>(ws + s.part);
+    if (!set_problem(g.g[0], M, N, blocks_of(K), s.plan, s.plan.cut[0], operand(x, M, K, pack, false),
+                     operand(w, N, K, pack, false), planes, part, epi))
+        return cudaErrorInvalidValue;
+    g.count = 1, g.units = g.g[0].units;
+    e = launch_gemm(g, planes, s.plan.bn, st);
+    if (e != cudaSuccess || g.g[0].splits == 1) return e;
+    add_reduce(red, part, g.g[0].splits, M, N, epi);
+    return launch_reduce(red, st);
 }
 
 cudaError_t launch_linear_backward(const LinearArgs& a, cudaStream_t st) {
-    cudaError_t e = cudaSuccess;
-    const void* gz = a.gy;
-    if (a.act != QK_ACT_NONE && (a.gx || a.gw)) {
-        slope_kernel<<<4 * kSms, 256, 0, st>>>(a.gy, a.tape, a.scratch, (size_t)a.rows * a.out, a.act, a.io_dtype);
-        e = cudaPeekAtLastError();
-        gz = a.scratch;
+    const int M = a.rows, K = a.in, N = a.out, planes = planes_of(a.io_dtype);
+    const QkLinearDesc d{M, K, N, a.io_dtype, a.act, 0};
+    const BackwardScratch s = backward_scratch(d);
+    char* ws = static_cast<char*>(a.scratch);
+    const bool pack = !reads_in_place(K, a.io_dtype);
+    const bool pack_gz = (a.gx || a.gw) && (a.act != QK_ACT_NONE || !reads_in_place(N, a.io_dtype));
+    float* colpart = a.gb ? reinterpret_cast<float*>(ws + s.colpart) : nullptr;
+    PrepArgsL p{};
+    if (pack_gz || a.gb)
+        p.job[p.count++] = prep_job(a.gy, a.act == QK_ACT_NONE ? nullptr : a.tape, pack_gz ? ws + s.gz : nullptr, colpart, M,
+                                    N, a.act, a.io_dtype);
+    if (pack && a.gw) p.job[p.count++] = prep_job(a.x, nullptr, ws + s.x, nullptr, M, K, 0, a.io_dtype);
+    if (pack && a.gx) p.job[p.count++] = prep_job(a.w, nullptr, ws + s.w, nullptr, N, K, 0, a.io_dtype);
+    cudaError_t e = launch_prepare(p, a.io_dtype, st);
+    if (e != cudaSuccess) return e;
+    const void* gz = pack_gz ? ws + s.gz : a.gy;
+    GemmArgs g{};
+    ReduceArgs red{};
+    if (a.gw) {
+        float* part = reinterpret_cast<float*>(ws + s.part0);
+        const Epilogue epi{nullptr, nullptr, a.gw, nullptr, QK_ACT_NONE, a.io_dtype};
+        if (!set_problem(g.g[g.count++], N, K, blocks_of(M), s.plan, s.plan.cut[0], operand(gz, M, N, pack_gz, true),
+                         operand(pack ? ws + s.x : a.x, M, K, pack, true), planes, part, epi))
+            return cudaErrorInvalidValue;
+        if (s.plan.cut[0].splits > 1) add_reduce(red, part, s.plan.cut[0].splits, N, K, epi);
     }
-    if (e == cudaSuccess && a.gx) {
-        Product g{};
-        g.rows = a.rows, g.cols = a.in, g.depth = a.out;
-        g.p = gz, g.q = a.w;
-        g.p_kmajor = true, g.q_kmajor = false;
-        g.epi = {nullptr, nullptr, a.gx, nullptr, QK_ACT_NONE, a.io_dtype};
-        e = launch_product(g, st);
+    if (a.gx) {
+        float* part = reinterpret_cast<float*>(ws + s.part1);
+        const Epilogue epi{nullptr, nullptr, a.gx, nullptr, QK_ACT_NONE, a.io_dtype};
+        if (!set_problem(g.g[g.count++], M, K, blocks_of(N), s.plan, s.plan.cut[1], operand(gz, M, N, pack_gz, false),
+                         operand(pack ? ws + s.w : a.w, N, K, pack, true), planes, part, epi))
+            return cudaErrorInvalidValue;
+        if (s.plan.cut[1].splits > 1) add_reduce(red, part, s.plan.cut[1].splits, M, K, epi);
     }
-    if (e == cudaSuccess && a.gw) {
-        Product g{};
-        g.rows = a.out, g.cols = a.in, g.depth = a.rows;
-        g.p = gz, g.q = a.x;
-        g.epi = {nullptr, nullptr, a.gw, nullptr, QK_ACT_NONE, a.io_dtype};
-        e = launch_product(g, st);
+    if (g.count) {
+        g.units = g.g[0].units + (g.count > 1 ? g.g[1].units : 0);
+        e = launch_gemm(g, planes, s.plan.bn, st);
+        if (e != cudaSuccess) return e;
     }
-    if (e == cudaSuccess && a.gb && a.out) {
-        column_sum_kernel<<<(a.out + 31) / 32, dim3(32, 32), 0, st>>>(
-            a.gy, a.act == QK_ACT_NONE ? nullptr : a.tape, a.gb, a.rows, a.out, a.act, a.io_dtype);
-        e = cudaPeekAtLastError();
-    }
-    return e;
+    red.colpart = colpart, red.gb = a.gb, red.slabs = s.slabs.count, red.cols = N, red.io_dtype = a.io_dtype;
+    return launch_reduce(red, st);
 }
 
 }  // namespace qk

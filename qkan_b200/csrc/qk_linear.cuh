@@ -1,20 +1,44 @@
 // Argument blocks of the linear map's kernels.
 #pragma once
 
+#include <cuda.h>
+
 #include "qk_dense.cuh"
 
 namespace qk {
 
-// One matrix product: C[r,c] = sum_k P[r,k] Q[c,k], C row-major (rows, cols). P is stored (rows, depth) when p_kmajor
-// and (depth, rows) otherwise; Q likewise with cols.
-struct Product {
-    int rows, cols, depth;
-    const void* p;
-    const void* q;
-    bool p_kmajor, q_kmajor;
+// ---- tensor-core products (qk_gemm.cu) -----------------------------------------
+// C[r,c] = sum_k P[r,k] Q[c,k], C row-major (rows, cols).
+
+// A matrix of bfloat16 as it lies in memory, rows 16-byte aligned; for float32 the three parts follow one another.
+struct Operand {
+    const void* base;
+    long inner, outer, ld;  // contiguous elements, rows, elements from row to row
+    bool mn_major;          // the contiguous axis is the product's row (column), not the summed one
+};
+
+struct alignas(64) GemmProblem {
+    CUtensorMap p_map, q_map;
+    int rows, cols;
+    int kblocks, kper, splits;  // 64-deep blocks in all, per slice of the depth, slices
+    int tiles_r, tiles_c, units;
+    bool p_mn, q_mn;
+    float* part;  // splits > 1: [splits][rows][cols] sums, no epilogue; nullptr otherwise
     Epilogue epi;
 };
 
+struct GemmArgs {
+    GemmProblem g[2];
+    int count, units;
+};
+
+// fills in the operands' tensor maps; false: the driver refused one
+bool gemm_bind(GemmProblem& g, const Operand& p, const Operand& q, int planes, int bn);
+cudaError_t launch_gemm(const GemmArgs& a, int planes, int bn, cudaStream_t st);
+// waits that ran out on the current device since the last call; synchronises the stream
+cudaError_t gemm_gave_up(unsigned* count, cudaStream_t st);
+
+// ---- the map (qk_linear.cu) ----------------------------------------------------
 struct LinearArgs {
     int rows, in, out, act, io_dtype;
     const void* x;
@@ -30,9 +54,11 @@ struct LinearArgs {
     void* scratch;
 };
 
-// bytes of scratch (0: a product too large for the launch grid)
+// bytes of scratch
 size_t linear_forward_scratch(const QkLinearDesc& d);
 size_t linear_backward_scratch(const QkLinearDesc& d);
+// whether the products read rows of `width` elements in place, which then have to start on a 16-byte boundary
+inline bool reads_in_place(int width, int io_dtype) { return io_dtype == QK_BF16 && width % 8 == 0; }
 cudaError_t launch_linear_forward(const LinearArgs& a, cudaStream_t st);
 cudaError_t launch_linear_backward(const LinearArgs& a, cudaStream_t st);
 

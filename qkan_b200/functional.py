@@ -515,6 +515,20 @@ def _call(dev: torch.device, fn, what: str, *args) -> None:
         _abi.check(rc, what)
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and on a 16-byte boundary (a view may start anywhere in its storage)."""
+    t = t.detach().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def dense_status() -> None:
+    """Raise if a wait inside the linear map's kernels ran out on the current device since the last call.
+
+    Synchronises the current stream; results computed since then are not valid in that case.
+    """
+    _abi.check(_abi.load().qk_dense_status(torch.cuda.current_stream().cuda_stream), "qk_dense_status")
+
+
 def _linear_desc(x: torch.Tensor, weight: torch.Tensor, code: int) -> _abi.QkLinearDesc:
     _require_cuda(x, "x")
     io = _io_dtype(x)
@@ -544,7 +558,7 @@ def linear_forward(x, weight, bias=None, *, activation="none", residual=None, re
     shape = x.shape[:-1] + weight.shape[:1]
     _check_like(bias, "bias", weight.shape[:1], dt, dev)
     _check_like(residual, "residual", shape, dt, dev)
-    x, weight = x.detach().contiguous(), weight.detach().contiguous()
+    x, weight = _aligned(x), _aligned(weight)
     bias = None if bias is None else bias.detach().contiguous()
     residual = None if residual is None else residual.detach().contiguous()
     y = torch.empty(shape, dtype=dt, device=dev)
@@ -579,7 +593,7 @@ def linear_backward(x, weight, gy, *, tape=None, activation="none", want=("x", "
         tape = tape.contiguous()
     else:
         tape = None
-    x, weight, gy = x.detach().contiguous(), weight.detach().contiguous(), gy.detach().contiguous()
+    x, weight, gy = _aligned(x), _aligned(weight), _aligned(gy)
     shapes = {"x": x.shape, "weight": weight.shape, "bias": weight.shape[:1]}
     out = {n: torch.empty(shapes[n], dtype=dt, device=dev) for n in want}
     dp = _abi.desc_pointer(desc)

@@ -54,6 +54,17 @@ def test_linear_pointers_and_workspaces_that_are_refused():
     assert lib.qk_linear_forward(None, one, one, None, None, one, None, one, big, None) == _abi.QK_ERR_BAD_ARGUMENT
 
 
+def test_misaligned_rows_are_refused_where_they_are_read_in_place():
+    lib = _lib()
+    one, odd, big = ctypes.c_void_p(256), ctypes.c_void_p(258), 1 << 40
+    dp = _abi.desc_pointer(_abi.QkLinearDesc(64, 64, 64, _abi.QK_BF16, 0, 0))
+    for x, w in ((odd, one), (one, odd)):
+        assert lib.qk_linear_forward(dp, x, w, None, None, one, None, one, big, None) == _abi.QK_ERR_BAD_ARGUMENT
+        assert b"aligned" in lib.qk_last_error()
+        assert lib.qk_linear_backward(dp, x, w, None, one, one, one, one, one, big, None) == _abi.QK_ERR_BAD_ARGUMENT
+    assert lib.qk_linear_backward(dp, one, one, None, odd, one, one, one, one, big, None) == _abi.QK_ERR_BAD_ARGUMENT
+
+
 @pytest.mark.parametrize("fields,text", [
     ((-1, 4, 0, 0, 1e-5, 0), b"rows"), ((4, 0, 0, 0, 1e-5, 0), b"dim"), ((4, 4, 5, 0, 1e-5, 0), b"io_dtype"),
     ((4, 4, 0, 5, 1e-5, 0), b"param_dtype"), ((4, 4, 0, 0, -1.0, 0), b"eps"), ((4, 4, 0, 0, float("nan"), 0), b"eps"),

@@ -8,6 +8,12 @@ from tests.dense_util import ACTS, linear64, linear64_grads, norm64, norm64_grad
 
 pytestmark = pytest.mark.gpu
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    F.dense_status()
+
+
 DTYPES = [torch.float32, torch.bfloat16]
 
 
