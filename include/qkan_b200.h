@@ -225,7 +225,8 @@ int qk_pz_forward_noalloc(const QkDesc* desc, const void* x, const float* theta,
  * epilogue, and layer norm, each with its backward pass. All tensors are contiguous and row-major; pointers need the
  * alignment of their element (stats: 8 bytes), and bfloat16 x, weight and grad_y of the linear map whose rows are a
  * multiple of 16 bytes have to start on a 16-byte boundary. Gradients are OVERWRITTEN, summed in a fixed order
- * (run-to-run bitwise reproducible), and written in the type of the tensor that they belong to.
+ * (run-to-run bitwise reproducible), and written in the type of the tensor that they belong to. A workspace size of 1
+ * says that none is needed (its pointer may be NULL), 0 that the descriptor is refused.
  */
 enum QkActivation {
     QK_ACT_NONE = 0,

@@ -42,6 +42,12 @@ size_t norm_scratch(const QkNormDesc& d) {
     return qk::align256((size_t)2 * qk::norm_slices(d.rows, d.dim) * d.dim * sizeof(float));
 }
 
+// a size of 0 says that the descriptor was refused, so "none" is 1
+size_t at_least_one(size_t n) { return n ? n : 1; }
+int check_scratch(const void* p, size_t have, size_t need) {
+    return need ? check_buffer(p, have, need, "workspace") : QK_OK;
+}
+
 // zeros for a gradient that sums over nothing
 cudaError_t zero(void* p, size_t n, int dtype, cudaStream_t st) {
     return p && n ? cudaMemsetAsync(p, 0, n * qk::dtype_bytes(dtype), st) : cudaSuccess;
@@ -52,7 +58,7 @@ cudaError_t zero(void* p, size_t n, int dtype, cudaStream_t st) {
 extern "C" {
 
 size_t qk_linear_forward_workspace_bytes(const QkLinearDesc* desc) {
-    return check_linear(desc) ? 0 : qk::linear_forward_scratch(*desc);
+    return check_linear(desc) ? 0 : at_least_one(qk::linear_forward_scratch(*desc));
 }
 
 int qk_linear_forward(const QkLinearDesc* desc, const void* x, const void* weight, const void* bias,
@@ -65,7 +71,7 @@ int qk_linear_forward(const QkLinearDesc* desc, const void* x, const void* weigh
     if (d.in_features && (!x || !weight)) return fail(QK_ERR_BAD_ARGUMENT, "x or weight is NULL");
     if ((rc = check_aligned(x, d.in_features, d.io_dtype, "x"))) return rc;
     if ((rc = check_aligned(weight, d.in_features, d.io_dtype, "weight"))) return rc;
-    rc = check_buffer(ws, ws_bytes, qk::linear_forward_scratch(d), "workspace");
+    rc = check_scratch(ws, ws_bytes, qk::linear_forward_scratch(d));
     if (rc) return rc;
     qk::LinearArgs a{};
     a.rows = d.rows, a.in = d.in_features, a.out = d.out_features, a.act = d.activation, a.io_dtype = d.io_dtype;
@@ -77,7 +83,7 @@ int qk_linear_forward(const QkLinearDesc* desc, const void* x, const void* weigh
 }
 
 size_t qk_linear_backward_workspace_bytes(const QkLinearDesc* desc) {
-    return check_linear(desc) ? 0 : qk::linear_backward_scratch(*desc);
+    return check_linear(desc) ? 0 : at_least_one(qk::linear_backward_scratch(*desc));
 }
 
 int qk_linear_backward(const QkLinearDesc* desc, const void* x, const void* weight, const void* tape, const void* gy,
@@ -100,7 +106,7 @@ int qk_linear_backward(const QkLinearDesc* desc, const void* x, const void* weig
     if (gw && (rc = check_aligned(x, d.in_features, d.io_dtype, "x"))) return rc;
     if (gx && (rc = check_aligned(weight, d.in_features, d.io_dtype, "weight"))) return rc;
     if ((gx || gw) && (rc = check_aligned(gy, d.out_features, d.io_dtype, "grad_y"))) return rc;
-    rc = check_buffer(ws, ws_bytes, qk::linear_backward_scratch(d), "workspace");
+    rc = check_scratch(ws, ws_bytes, qk::linear_backward_scratch(d));
     if (rc) return rc;
     qk::LinearArgs a{};
     a.rows = d.rows, a.in = d.in_features, a.out = d.out_features, a.act = d.activation, a.io_dtype = d.io_dtype;
@@ -134,7 +140,7 @@ int qk_layer_norm_forward(const QkNormDesc* desc, const void* x, const void* wei
 
 size_t qk_layer_norm_backward_workspace_bytes(const QkNormDesc* desc) {
     if (check_norm(desc)) return 0;
-    return desc->rows == 0 ? 256 : norm_scratch(*desc);
+    return desc->rows == 0 ? 1 : norm_scratch(*desc);
 }
 
 int qk_layer_norm_backward(const QkNormDesc* desc, const void* x, const void* weight, const float* stats,

@@ -134,6 +134,17 @@ __device__ __forceinline__ void tmem_load16(unsigned addr, float (&v)[16]) {
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(u[i]);
 }
 
+template <int N>
+__device__ __forceinline__ void tmem_load(unsigned addr, float (&v)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; j += 16) {
+        float u[16];
+        tmem_load16(addr + j, u);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[j + i] = u[i];
+    }
+}
+
 // Shared-memory matrix descriptor, 128-byte swizzle. K-major: rows of 128 bytes, 8-row groups 1024 bytes apart, a
 // 16-deep step is 32 bytes on. MN-major: 64-wide boxes (8 KB each) of 64 rows of the depth, 8-row groups 1024 bytes
 // apart, a 16-deep step is 16 rows on.
@@ -142,24 +153,19 @@ __device__ __forceinline__ unsigned long long smem_desc(unsigned addr, bool mn) 
     return (unsigned long long)((addr & 0x3ffff) >> 4) | lead << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
 }
 
+// One unit of work: a tile of C and a slice of the depth.
 struct Unit {
-    const GemmProblem* g;
-    int r0, c0, kb0, kbs, split;
+    int r0, c0, kb0, kbs, split;  // first row in tiles, first column, first block and number of blocks of the slice
 };
-__device__ __forceinline__ Unit unit_at(const GemmArgs& a, int u) {
+__device__ __forceinline__ Unit unit_at(const GemmProblem& g, int u) {
     Unit t;
-    t.g = &a.g[0];
-    if (a.count > 1 && u >= a.g[0].units) {
-        u -= a.g[0].units;
-        t.g = &a.g[1];
-    }
-    const int tiles = t.g->tiles_r * t.g->tiles_c;
+    const int tiles = g.tiles_r * g.tiles_c;
     t.split = u / tiles;
     u -= t.split * tiles;
-    t.r0 = u / t.g->tiles_c;  // in tiles; columns run fastest, so that neighbouring CTAs share P
-    t.c0 = (u - t.r0 * t.g->tiles_c) * kTileC;
-    t.kb0 = t.split * t.g->kper;
-    t.kbs = min(t.g->kper, t.g->kblocks - t.kb0);
+    t.r0 = u / g.tiles_c;  // columns run fastest, so that neighbouring CTAs share P
+    t.c0 = (u - t.r0 * g.tiles_c) * kTileC;
+    t.kb0 = t.split * g.kper;
+    t.kbs = min(g.kper, g.kblocks - t.kb0);
     return t;
 }
 
@@ -181,48 +187,46 @@ __device__ __forceinline__ void activate_all(float (&v)[N], int act) {
     }
 }
 
-// 16 sums of column c, rows r .. r + 15
-template <typename IO>
-__device__ __forceinline__ void write_out(const GemmProblem& g, int split, long r, int c, float (&v)[16]) {
-    if (c >= g.cols) return;
-    const int n = (int)min(16L, g.rows - r);
-    if (n <= 0) return;
-    const size_t at = (size_t)r * g.cols + c;
-    if (g.part) {
-        float* out = g.part + (size_t)split * g.rows * g.cols + at;
+// The residual of column c, rows r .. r + N - 1, fetched before the sums are waited for. Row and column are held inside
+// the matrix, so that every load is good by itself; what lies behind its edge is never stored.
+template <typename IO, int N>
+__device__ __forceinline__ void load_residual(const GemmProblem& g, long r, int c, float (&q)[N]) {
+    const long first = min(r, g.rows - 1L);
+    const int last = (int)min(N - 1L, g.rows - 1 - first);
+    const IO* res = static_cast<const IO*>(g.residual) + (size_t)first * g.cols + min(c, g.cols - 1);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i < n) out[(size_t)i * g.cols] = v[i];
+    for (int i = 0; i < N; ++i) q[i] = as_float(res[(size_t)min(i, last) * g.cols]);
+}
+
+// N sums of column c, rows r .. r + N - 1, of which n exist (none for a lane behind the last column: the warp stays
+// together, since it has to be whole when it reads tensor memory again).
+template <typename IO, int N>
+__device__ __forceinline__ void write_out(const GemmProblem& g, int split, long r, int c, int n, float bias,
+                                          const float (&q)[N], float (&v)[N]) {
+    const size_t cols = g.cols, at = (size_t)r * cols + c;
+    if (g.part) {
+        float* out = g.part + (size_t)split * g.rows * cols + at;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < n) out[i * cols] = v[i];
         return;
     }
-    const Epilogue& e = g.epi;
-    if (e.bias) {
-        const float b = as_float(static_cast<const IO*>(e.bias)[c]);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] += b;
+    for (int i = 0; i < N; ++i) v[i] += bias;
+    if (g.tape) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < n) store_tape(g.tape, at + i * cols, sizeof(IO) == 2 ? QK_BF16 : QK_F32, v[i]);
     }
-    if (e.tape) {
+    activate_all(v, g.act);
+    IO* out = static_cast<IO*>(g.out) + at;
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i < n) store_tape(e.tape, at + (size_t)i * g.cols, sizeof(IO) == 2 ? QK_BF16 : QK_F32, v[i]);
-    }
-    activate_all(v, e.act);
-    if (e.residual) {
-        const IO* res = static_cast<const IO*>(e.residual) + at;
-        float q[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) q[i] = i < n ? as_float(__ldg(res + (size_t)i * g.cols)) : 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] += q[i];
-    }
-    IO* out = static_cast<IO*>(e.out) + at;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (i < n) out[(size_t)i * g.cols] = from_float<IO>(v[i]);
+    for (int i = 0; i < N; ++i)
+        if (i < n) out[i * cols] = from_float<IO>(v[i] + q[i]);
 }
 
 template <int BN, int PLANES>
-__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs a) {
+__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmProblem g) {
     using S = Shape<BN, PLANES>;
     using IO = std::conditional_t<PLANES == 3, float, __nv_bfloat16>;
     extern __shared__ char raw[];
@@ -257,9 +261,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             int stage = 0;
             unsigned phase = 0, issued = 0;
             bool ok = true;
-            for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
-                const Unit t = unit_at(a, u);
-                const GemmProblem& g = *t.g;
+            for (int u = blockIdx.x; ok && u < g.units; u += gridDim.x) {
+                const Unit t = unit_at(g, u);
                 const int r0 = t.r0 * BN;
                 const unsigned bytes = PLANES * (S::kABytes + (g.p_mn ? S::kBBytes : BN * 128));
                 for (int kb = t.kb0; kb < t.kb0 + t.kbs; ++kb) {
@@ -301,9 +304,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             int stage = 0, acc = 0, corr = 0;
             unsigned phase = 0, acc_phase = 0, corr_phase = 0;
             bool ok = true;
-            for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
-                const Unit t = unit_at(a, u);
-                const GemmProblem& g = *t.g;
+            for (int u = blockIdx.x; ok && u < g.units; u += gridDim.x) {
+                const Unit t = unit_at(g, u);
                 const unsigned idesc = 1u << 4 | 1u << 7 | 1u << 10 | (unsigned)g.q_mn << 15 | (unsigned)g.p_mn << 16 |
                                        (BN / 8) << 17 | (kTileC / 16) << 24;
                 const unsigned a_step = g.q_mn ? 2048 >> 4 : 32 >> 4, b_step = g.p_mn ? 2048 >> 4 : 32 >> 4;
@@ -363,27 +365,40 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         int acc = 0, corr = 0;
         unsigned acc_phase = 0, corr_phase = 0;
         bool ok = true;
-        for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
-            const Unit t = unit_at(a, u);
-            const GemmProblem& g = *t.g;
+        for (int u = blockIdx.x; ok && u < g.units; u += gridDim.x) {
+            const Unit t = unit_at(g, u);
             const int c = t.c0 + quad * 32 + lane;
             const long r0 = (long)t.r0 * BN + half * (BN / 2);
+            const bool live = c < g.cols;
+            float bias = as_float(static_cast<const IO*>(g.bias)[min(c, g.cols - 1)]);
+            if (!g.has_bias) bias = 0.f;
             if constexpr (PLANES == 1) {
-                ok = bar_wait(&bars.acc_full[acc], acc_phase, abort);
-                ok = __all_sync(~0u, ok);
-                if (!ok) break;
-                fence_after();
+                constexpr int N = BN / 2 < 32 ? BN / 2 : 32;
 #pragma unroll 1
-                for (int j = 0; j < BN / 2; j += 16) {
-                    float v[16];
-                    tmem_load16(tmem + lanes + acc * BN + half * (BN / 2) + j, v);
-                    if (j + 16 == BN / 2) {
+                for (int j = 0; j < BN / 2; j += N) {
+                    const int n = live ? (int)max(0L, min((long)N, g.rows - r0 - j)) : 0;
+                    float q[N], v[N];
+                    if (g.has_residual) {
+                        load_residual<IO, N>(g, r0 + j, c, q);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < N; ++i) q[i] = 0.f;
+                    }
+                    if (j == 0) {
+                        ok = bar_wait(&bars.acc_full[acc], acc_phase, abort);
+                        ok = __all_sync(~0u, ok);
+                        if (!ok) break;
+                        fence_after();
+                    }
+                    __syncwarp();
+                    tmem_load<N>(tmem + lanes + acc * BN + half * (BN / 2) + j, v);
+                    if (j + N == BN / 2) {
                         fence_before();
                         if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
                     }
-                    write_out<IO>(g, t.split, r0 + j, c, v);
-                    __syncwarp();
+                    write_out<IO, N>(g, t.split, r0 + j, c, n, bias, q, v);
                 }
+                if (!ok) break;
                 if (++acc == 2) acc = 0, acc_phase ^= 1;
             } else {
                 float sum[BN / 2];
@@ -397,7 +412,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
 #pragma unroll
                     for (int j = 0; j < BN / 2; j += 16) {
                         float v[16];
-                        tmem_load16(tmem + lanes + acc * BN + half * (BN / 2) + j, v);
+                        tmem_load<16>(tmem + lanes + acc * BN + half * (BN / 2) + j, v);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) sum[j + i] += v[i];
                     }
@@ -413,8 +428,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 fence_after();
 #pragma unroll
                 for (int j = 0; j < BN / 2; j += 16) {
-                    float v[16];
-                    tmem_load16(corr_base + lanes + corr * BN + half * (BN / 2) + j, v);
+                    const int n = live ? (int)max(0L, min(16L, g.rows - r0 - j)) : 0;
+                    float q[16], v[16];
+                    if (g.has_residual) {
+                        load_residual<IO, 16>(g, r0 + j, c, q);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) q[i] = 0.f;
+                    }
+                    __syncwarp();
+                    tmem_load<16>(corr_base + lanes + corr * BN + half * (BN / 2) + j, v);
                     if (j + 16 == BN / 2) {
                         fence_before();
                         __syncwarp();
@@ -422,8 +445,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) v[i] = isfinite(sum[j + i]) ? sum[j + i] + v[i] : sum[j + i];
-                    write_out<IO>(g, t.split, r0 + j, c, v);
-                    __syncwarp();
+                    write_out<IO, 16>(g, t.split, r0 + j, c, n, bias, q, v);
                 }
                 if (++corr == 2) corr = 0, corr_phase ^= 1;
             }
@@ -467,12 +489,12 @@ bool make_map(CUtensorMap* map, const void* base, long inner, long outer, long l
 }
 
 template <int BN, int PLANES>
-cudaError_t launch_shape(const GemmArgs& a, cudaStream_t st) {
+cudaError_t launch_shape(const GemmProblem& g, cudaStream_t st) {
     static unsigned long long opted = 0;
     cudaError_t e = opt_in_smem(gemm_kernel<BN, PLANES>, &opted);
     if (e != cudaSuccess) return e;
-    const int grid = a.units < kSms ? a.units : kSms;
-    gemm_kernel<BN, PLANES><<<grid, kGemmThreads, Shape<BN, PLANES>::kSmem, st>>>(a);
+    const int grid = g.units < kSms ? g.units : kSms;
+    gemm_kernel<BN, PLANES><<<grid, kGemmThreads, Shape<BN, PLANES>::kSmem, st>>>(g);
     return cudaPeekAtLastError();
 }
 
@@ -485,7 +507,7 @@ bool gemm_bind(GemmProblem& g, const Operand& p, const Operand& q, int planes, i
            make_map(&g.q_map, q.base, q.inner, q.outer, q.ld, planes, q.mn_major ? kBK : kTileC);
 }
 
-cudaError_t launch_gemm(const GemmArgs& a, int planes, int bn, cudaStream_t st) {
+cudaError_t launch_gemm(const GemmProblem& a, int planes, int bn, cudaStream_t st) {
     if (planes == 3) {
         if (bn == 128) return launch_shape<128, 3>(a, st);
         if (bn == 64) return launch_shape<64, 3>(a, st);

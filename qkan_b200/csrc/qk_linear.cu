@@ -4,7 +4,7 @@
 //   prepare   operands that the products cannot read where they lie: float32 is split into three bfloat16 parts, rows
 //             that are no multiple of 16 bytes are padded, and in the backward gz = gy * act'(tape) is formed, with
 //             its column sums for grad_bias on the way
-//   products  forward: one; backward: grad_x and grad_weight in one launch, so that either fills the other's last wave
+//   products  forward: one; backward: grad_weight and grad_x
 //   reduce    adds the slices of a depth that was cut for want of tiles, then the epilogue; adds grad_bias' slabs
 #include "qk_linear.cuh"
 
@@ -46,10 +46,10 @@ __device__ __forceinline__ void load8(const void* p, size_t at, bool vec, int n,
     const IO* s = static_cast<const IO*>(p) + at;
     if (vec) {
         if constexpr (sizeof(IO) == 4) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(s)), b = __ldg(reinterpret_cast<const float4*>(s) + 1);
+            const float4 a = *reinterpret_cast<const float4*>(s), b = reinterpret_cast<const float4*>(s)[1];
             v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
         } else {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(s));
+            const uint4 a = *reinterpret_cast<const uint4*>(s);
             const unsigned u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kThreads) reduce_kernel(const ReduceArgs a) {
         if (i >= j.n) return;
         float s = 0.f;
 #pragma unroll 4
-        for (int k = 0; k < j.splits; ++k) s += __ldg(j.part + (size_t)k * j.n + i);
+        for (int k = 0; k < j.splits; ++k) s += j.part[(size_t)k * j.n + i];
         finish_element(j.epi, i, (int)(i % j.cols), s);
         return;
     }
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kThreads) reduce_kernel(const ReduceArgs a) {
     const int x = threadIdx.x % 32, y = threadIdx.x / 32, c = b * 32 + x;
     float s = 0.f;
     if (c < a.cols)
-        for (int k = y; k < a.slabs; k += 8) s += __ldg(a.colpart + (size_t)k * a.cols + c);
+        for (int k = y; k < a.slabs; k += 8) s += a.colpart[(size_t)k * a.cols + c];
     tile[y][x] = s;
     __syncthreads();
     if (y == 0 && c < a.cols) {
@@ -194,59 +194,29 @@ Cut cut_into(int kblocks, int splits) {
 constexpr int kCuts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 148};
 constexpr long kMostPart = 64l << 20;  // floats of partial sums: 256 MB
 
-// time of `s` alone when it is cut this way, with `other` clocks of work per SM beside it
-double cost_of(const Size& s, int bn, int planes, const Cut& c, double other) {
-    const double units = (double)s.tiles(bn) * c.splits;
+struct Plan {
+    int bn;
+    Cut cut;
+};
+
+double cost_of(const Size& s, int bn, int planes, const Cut& c) {
+    const long units = s.tiles(bn) * c.splits;
     const double mainloop = c.kper * block_clocks(bn, planes), drain = drain_clocks(bn);
-    const double unit = mainloop > drain ? mainloop : drain;
-    double waves = units * unit / kSms + other;  // filled evenly
-    const double even = (double)((long)(units + kSms - 1) / kSms) * unit;
-    if (other == 0 && even > waves) waves = even;
-    if (unit > waves) waves = unit;
-    double t = waves + drain + 2500;
+    double t = (double)((units + kSms - 1) / kSms) * (mainloop > drain ? mainloop : drain) + drain + 2500;
     if (c.splits > 1) t += 3500 + 2.0 * c.splits * s.rows * s.cols * 4 / (kSms * 24.0);
     return t;
 }
 
-Cut best_cut(const Size& s, int bn, int planes, double other, double* cost) {
-    Cut best{1, s.kblocks};
-    *cost = cost_of(s, bn, planes, best, other);
-    for (int k : kCuts) {
-        if (k > s.kblocks || (double)k * s.rows * s.cols > kMostPart) break;
-        if (k > 1 && s.tiles(bn) * k > 4l * kSms) break;
-        const Cut c = cut_into(s.kblocks, k);
-        const double t = cost_of(s, bn, planes, c, other);
-        if (t < *cost) *cost = t, best = c;
-    }
-    return best;
-}
-
-struct Plan {
-    int bn;
-    Cut cut[2];
-    double cost;
-};
-
-// one product, or two in one launch
-Plan plan_for(const Size* s, int count, int planes) {
+Plan plan_for(const Size& s, int planes) {
     Plan best{};
-    best.cost = 1e300;
-    for (int bn = planes == 3 ? 128 : 256; bn >= 32; bn /= 2) {
-        Plan p{};
-        p.bn = bn;
-        double c0 = 0, c1 = 0;
-        if (count == 1) {
-            p.cut[0] = best_cut(s[0], bn, planes, 0, &c0);
-            p.cost = c0;
-        } else {
-            const double w1 = (double)s[1].tiles(bn) * s[1].kblocks * block_clocks(bn, planes) / kSms;
-            p.cut[0] = best_cut(s[0], bn, planes, w1, &c0);
-            const double w0 = (double)s[0].tiles(bn) * s[0].kblocks * block_clocks(bn, planes) / kSms;
-            p.cut[1] = best_cut(s[1], bn, planes, w0, &c1);
-            p.cost = c0 > c1 ? c0 : c1;
+    double least = 1e300;
+    for (int bn = planes == 3 ? 128 : 256; bn >= 32; bn /= 2)
+        for (int k : kCuts) {
+            if (k > 1 && (k > s.kblocks || s.tiles(bn) * k > 4l * kSms || (double)k * s.rows * s.cols > kMostPart)) break;
+            const Cut c = cut_into(s.kblocks, k);
+            const double t = cost_of(s, bn, planes, c);
+            if (t < least) least = t, best = {bn, c};
         }
-        if (p.cost < best.cost) best = p;
-    }
     return best;
 }
 
@@ -280,45 +250,68 @@ struct ForwardScratch {
     Plan plan;
     size_t x, w, part, total;
 };
-ForwardScratch forward_scratch(const QkLinearDesc& d) {
+ForwardScratch plan_forward(const QkLinearDesc& d) {
     ForwardScratch s{};
     const int planes = planes_of(d.io_dtype);
     const bool pack = !reads_in_place(d.in_features, d.io_dtype);
-    const Size size{d.rows, d.out_features, blocks_of(d.in_features)};
-    s.plan = plan_for(&size, 1, planes);
+    s.plan = plan_for({d.rows, d.out_features, blocks_of(d.in_features)}, planes);
     s.x = 0;
     s.w = pack ? packed_bytes(d.rows, d.in_features, planes) : 0;
     s.part = s.w + (pack ? packed_bytes(d.out_features, d.in_features, planes) : 0);
     s.total = s.part;
-    if (s.plan.cut[0].splits > 1) s.total += align256((size_t)s.plan.cut[0].splits * d.rows * d.out_features * 4);
+    if (s.plan.cut.splits > 1) s.total += align256((size_t)s.plan.cut.splits * d.rows * d.out_features * 4);
     return s;
 }
 
-// Products 0: grad_weight (its units are the long ones and go first), 1: grad_x. The layout is that of both, whatever
-// is asked for.
+// The layout is that of all gradients, whatever is asked for.
 struct BackwardScratch {
-    Plan plan;
+    Plan plan_w, plan_x;
     Slabs slabs;
-    size_t gz, x, w, colpart, part0, part1, total;
+    size_t gz, x, w, colpart, part_w, part_x, total;
 };
-BackwardScratch backward_scratch(const QkLinearDesc& d) {
+BackwardScratch plan_backward(const QkLinearDesc& d) {
     BackwardScratch s{};
     const int planes = planes_of(d.io_dtype);
     const long M = d.rows, K = d.in_features, N = d.out_features;
     const bool pack_gz = d.activation != QK_ACT_NONE || !reads_in_place(N, d.io_dtype);
     const bool pack = !reads_in_place(K, d.io_dtype);
-    const Size size[2] = {{N, K, blocks_of(M)}, {M, K, blocks_of(N)}};
-    s.plan = plan_for(size, 2, planes);
+    s.plan_w = plan_for({N, K, blocks_of(M)}, planes);
+    s.plan_x = plan_for({M, K, blocks_of(N)}, planes);
     s.slabs = slabs_of(M, N);
     s.gz = 0;
     s.x = pack_gz ? packed_bytes(M, N, planes) : 0;
     s.w = s.x + (pack ? packed_bytes(M, K, planes) : 0);
     s.colpart = s.w + (pack ? packed_bytes(N, K, planes) : 0);
-    s.part0 = s.colpart + align256((size_t)s.slabs.count * N * 4);
-    s.part1 = s.part0 + (s.plan.cut[0].splits > 1 ? align256((size_t)s.plan.cut[0].splits * N * K * 4) : 0);
-    s.total = s.part1 + (s.plan.cut[1].splits > 1 ? align256((size_t)s.plan.cut[1].splits * M * K * 4) : 0);
+    s.part_w = s.colpart + align256((size_t)s.slabs.count * N * 4);
+    s.part_x = s.part_w + (s.plan_w.cut.splits > 1 ? align256((size_t)s.plan_w.cut.splits * N * K * 4) : 0);
+    s.total = s.part_x + (s.plan_x.cut.splits > 1 ? align256((size_t)s.plan_x.cut.splits * M * K * 4) : 0);
     return s;
 }
+
+// The size query and the call that follows it plan the same problem: each thread keeps its last few plans, which
+// depend on the descriptor alone.
+template <typename S, S (*plan)(const QkLinearDesc&)>
+const S& remembered(const QkLinearDesc& d) {
+    constexpr int kKept = 8;
+    static thread_local struct {
+        bool set;
+        QkLinearDesc desc;
+        S s;
+    } kept[kKept];
+    static thread_local int next = 0;
+    for (auto& k : kept)
+        if (k.set && k.desc.rows == d.rows && k.desc.in_features == d.in_features &&
+            k.desc.out_features == d.out_features && k.desc.io_dtype == d.io_dtype && k.desc.activation == d.activation)
+            return k.s;
+    auto& k = kept[next];
+    next = (next + 1) % kKept;
+    k.s = plan(d);
+    k.desc = d;
+    k.set = true;
+    return k.s;
+}
+const ForwardScratch& forward_scratch(const QkLinearDesc& d) { return remembered<ForwardScratch, plan_forward>(d); }
+const BackwardScratch& backward_scratch(const QkLinearDesc& d) { return remembered<BackwardScratch, plan_backward>(d); }
 
 // ---- launches ------------------------------------------------------------------
 PrepJob prep_job(const void* src, const void* tape, void* dst, float* colpart, int rows, int cols, int act, int io_dtype) {
@@ -362,34 +355,40 @@ Operand operand(const void* base, int rows, int cols, bool packed, bool mn_major
     return {base, cols, rows, packed ? padded(cols) : (long)cols, mn_major};
 }
 
-bool set_problem(GemmProblem& g, int rows, int cols, int kblocks, const Plan& plan, const Cut& cut, const Operand& p,
-                 const Operand& q, int planes, float* part, const Epilogue& epi) {
+// C (rows, cols) = P Q^T over `depth`, with its epilogue; where the depth is cut, the sums wait in `part` for `red`
+cudaError_t run_product(int rows, int cols, int depth, const Plan& plan, const Operand& p, const Operand& q, float* part,
+                        const Epilogue& epi, ReduceArgs& red, cudaStream_t st) {
+    const int planes = planes_of(epi.io_dtype);
+    GemmProblem g{};
     g.rows = rows, g.cols = cols;
-    g.kblocks = kblocks, g.kper = cut.kper, g.splits = cut.splits;
+    g.kblocks = blocks_of(depth), g.kper = plan.cut.kper, g.splits = plan.cut.splits;
     g.tiles_r = (rows + plan.bn - 1) / plan.bn, g.tiles_c = (cols + 127) / 128;
     const long units = (long)g.tiles_r * g.tiles_c * g.splits;
-    if (units > 0x3fffffff) return false;
+    if (units > 0x3fffffff) return cudaErrorInvalidConfiguration;
     g.units = (int)units;
-    g.part = cut.splits > 1 ? part : nullptr;
-    g.epi = epi;
-    return gemm_bind(g, p, q, planes, plan.bn);
+    g.part = g.splits > 1 ? part : nullptr;
+    g.has_bias = epi.bias && !g.part, g.has_residual = epi.residual && !g.part;
+    g.bias = g.has_bias ? epi.bias : epi.out, g.residual = g.has_residual ? epi.residual : epi.out;
+    g.out = epi.out, g.tape = epi.tape, g.act = epi.act;
+    if (!gemm_bind(g, p, q, planes, plan.bn)) return cudaErrorInvalidValue;
+    if (g.splits > 1) add_reduce(red, part, g.splits, rows, cols, epi);
+    return launch_gemm(g, planes, plan.bn, st);
 }
 
 }  // namespace
 
 size_t linear_forward_scratch(const QkLinearDesc& d) {
-    if (d.rows == 0 || d.out_features == 0 || d.in_features == 0) return 256;
-    const size_t n = forward_scratch(d).total;
-    return n ? n : 256;
+    if (d.rows == 0 || d.out_features == 0 || d.in_features == 0) return 0;
+    return forward_scratch(d).total;
 }
 
 size_t linear_backward_scratch(const QkLinearDesc& d) {
-    if (d.rows == 0 || d.out_features == 0) return 256;
+    if (d.rows == 0 || d.out_features == 0) return 0;
     return backward_scratch(d).total;
 }
 
 cudaError_t launch_linear_forward(const LinearArgs& a, cudaStream_t st) {
-    const int M = a.rows, K = a.in, N = a.out, planes = planes_of(a.io_dtype);
+    const int M = a.rows, K = a.in, N = a.out;
     const Epilogue epi{a.bias, a.residual, a.y, a.tape, a.act, a.io_dtype};
     ReduceArgs red{};
     if (K == 0) {
@@ -397,7 +396,7 @@ cudaError_t launch_linear_forward(const LinearArgs& a, cudaStream_t st) {
         return launch_reduce(red, st);
     }
     const QkLinearDesc d{M, K, N, a.io_dtype, a.act, 0};
-    const ForwardScratch s = forward_scratch(d);
+    const ForwardScratch& s = forward_scratch(d);
     char* ws = static_cast<char*>(a.scratch);
     const bool pack = !reads_in_place(K, a.io_dtype);
     const void *x = a.x, *w = a.w;
@@ -410,22 +409,15 @@ cudaError_t launch_linear_forward(const LinearArgs& a, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         x = ws + s.x, w = ws + s.w;
     }
-    GemmArgs g{};
-    float* part = reinterpret_cast<float*>(ws + s.part);
-    if (!set_problem(g.g[0], M, N, blocks_of(K), s.plan, s.plan.cut[0], operand(x, M, K, pack, false),
-                     operand(w, N, K, pack, false), planes, part, epi))
-        return cudaErrorInvalidValue;
-    g.count = 1, g.units = g.g[0].units;
-    e = launch_gemm(g, planes, s.plan.bn, st);
-    if (e != cudaSuccess || g.g[0].splits == 1) return e;
-    add_reduce(red, part, g.g[0].splits, M, N, epi);
-    return launch_reduce(red, st);
+    e = run_product(M, N, K, s.plan, operand(x, M, K, pack, false), operand(w, N, K, pack, false),
+                    reinterpret_cast<float*>(ws + s.part), epi, red, st);
+    return e == cudaSuccess ? launch_reduce(red, st) : e;
 }
 
 cudaError_t launch_linear_backward(const LinearArgs& a, cudaStream_t st) {
-    const int M = a.rows, K = a.in, N = a.out, planes = planes_of(a.io_dtype);
+    const int M = a.rows, K = a.in, N = a.out;
     const QkLinearDesc d{M, K, N, a.io_dtype, a.act, 0};
-    const BackwardScratch s = backward_scratch(d);
+    const BackwardScratch& s = backward_scratch(d);
     char* ws = static_cast<char*>(a.scratch);
     const bool pack = !reads_in_place(K, a.io_dtype);
     const bool pack_gz = (a.gx || a.gw) && (a.act != QK_ACT_NONE || !reads_in_place(N, a.io_dtype));
@@ -439,29 +431,16 @@ cudaError_t launch_linear_backward(const LinearArgs& a, cudaStream_t st) {
     cudaError_t e = launch_prepare(p, a.io_dtype, st);
     if (e != cudaSuccess) return e;
     const void* gz = pack_gz ? ws + s.gz : a.gy;
-    GemmArgs g{};
     ReduceArgs red{};
-    if (a.gw) {
-        float* part = reinterpret_cast<float*>(ws + s.part0);
-        const Epilogue epi{nullptr, nullptr, a.gw, nullptr, QK_ACT_NONE, a.io_dtype};
-        if (!set_problem(g.g[g.count++], N, K, blocks_of(M), s.plan, s.plan.cut[0], operand(gz, M, N, pack_gz, true),
-                         operand(pack ? ws + s.x : a.x, M, K, pack, true), planes, part, epi))
-            return cudaErrorInvalidValue;
-        if (s.plan.cut[0].splits > 1) add_reduce(red, part, s.plan.cut[0].splits, N, K, epi);
-    }
-    if (a.gx) {
-        float* part = reinterpret_cast<float*>(ws + s.part1);
-        const Epilogue epi{nullptr, nullptr, a.gx, nullptr, QK_ACT_NONE, a.io_dtype};
-        if (!set_problem(g.g[g.count++], M, K, blocks_of(N), s.plan, s.plan.cut[1], operand(gz, M, N, pack_gz, false),
-                         operand(pack ? ws + s.w : a.w, N, K, pack, true), planes, part, epi))
-            return cudaErrorInvalidValue;
-        if (s.plan.cut[1].splits > 1) add_reduce(red, part, s.plan.cut[1].splits, M, K, epi);
-    }
-    if (g.count) {
-        g.units = g.g[0].units + (g.count > 1 ? g.g[1].units : 0);
-        e = launch_gemm(g, planes, s.plan.bn, st);
-        if (e != cudaSuccess) return e;
-    }
+    if (a.gw)
+        e = run_product(N, K, M, s.plan_w, operand(gz, M, N, pack_gz, true), operand(pack ? ws + s.x : a.x, M, K, pack, true),
+                        reinterpret_cast<float*>(ws + s.part_w), {nullptr, nullptr, a.gw, nullptr, QK_ACT_NONE, a.io_dtype},
+                        red, st);
+    if (e == cudaSuccess && a.gx)
+        e = run_product(M, K, N, s.plan_x, operand(gz, M, N, pack_gz, false), operand(pack ? ws + s.w : a.w, N, K, pack, true),
+                        reinterpret_cast<float*>(ws + s.part_x), {nullptr, nullptr, a.gx, nullptr, QK_ACT_NONE, a.io_dtype},
+                        red, st);
+    if (e != cudaSuccess) return e;
     red.colpart = colpart, red.gb = a.gb, red.slabs = s.slabs.count, red.cols = N, red.io_dtype = a.io_dtype;
     return launch_reduce(red, st);
 }

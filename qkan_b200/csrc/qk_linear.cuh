@@ -24,17 +24,19 @@ struct alignas(64) GemmProblem {
     int tiles_r, tiles_c, units;
     bool p_mn, q_mn;
     float* part;  // splits > 1: [splits][rows][cols] sums, no epilogue; nullptr otherwise
-    Epilogue epi;
-};
-
-struct GemmArgs {
-    GemmProblem g[2];
-    int count, units;
+    // The epilogue, as in Epilogue. What it lacks points to `out`, so that a load of either is good whether or not it is
+    // wanted: where a null pointer stood behind a test, hoisting the load over the test made it a fault.
+    bool has_bias, has_residual;
+    const void* bias;
+    const void* residual;
+    void* out;
+    void* tape;
+    int act;
 };
 
 // fills in the operands' tensor maps; false: the driver refused one
 bool gemm_bind(GemmProblem& g, const Operand& p, const Operand& q, int planes, int bn);
-cudaError_t launch_gemm(const GemmArgs& a, int planes, int bn, cudaStream_t st);
+cudaError_t launch_gemm(const GemmProblem& g, int planes, int bn, cudaStream_t st);
 // waits that ran out on the current device since the last call; synchronises the stream
 cudaError_t gemm_gave_up(unsigned* count, cudaStream_t st);
 

@@ -34,7 +34,7 @@ struct Piece {
         for (int j = 0; j < NV; ++j) {
             const int c = (j * T + lane) * VEC;
             v[j] = Raw{};
-            if (c < dim) v[j] = __ldg(reinterpret_cast<const Raw*>(row + c));
+            if (c < dim) v[j] = *reinterpret_cast<const Raw*>(row + c);
         }
     }
     __device__ __forceinline__ void unpack(float (&f)[kElems]) const {
@@ -91,13 +91,13 @@ __device__ __forceinline__ void load_params(const void* p, int dtype, int c, flo
     } else if (dtype == QK_F32) {
 #pragma unroll
         for (int i = 0; i < VEC; i += 4) {
-            const float4 v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + i));
+            const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + i);
             f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; i += 4) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + c + i));
+            const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + c + i);
             f[i] = __uint_as_float(v.x << 16), f[i + 1] = __uint_as_float(v.x & 0xffff0000u);
             f[i + 2] = __uint_as_float(v.y << 16), f[i + 3] = __uint_as_float(v.y & 0xffff0000u);
         }
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(block_of(T)) norm_backward_kernel(const NormAr
     if (row < a.rows) {
         px.load(xs + row * a.dim, a.dim, lane);
         pg.load(gys + row * a.dim, a.dim, lane);
-        st = __ldg(a.stats + row);
+        st = a.stats[row];
     }
     for (; row < a.rows; row += step) {
         float xh[kElems], g[kElems];
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(block_of(T)) norm_backward_kernel(const NormAr
         if (row + step < a.rows) {
             px.load(xs + (row + step) * a.dim, a.dim, lane);
             pg.load(gys + (row + step) * a.dim, a.dim, lane);
-            st = __ldg(a.stats + row + step);
+            st = a.stats[row + step];
         }
         float2 s = make_float2(0.f, 0.f);
 #pragma unroll

@@ -7,6 +7,8 @@ torch is used for device memory, the current stream and autograd bookkeeping onl
 """
 from __future__ import annotations
 
+import math
+from ctypes import byref
 from typing import Optional
 
 import torch
@@ -478,7 +480,16 @@ def qkan_postacts(x, theta, preacts_weight, preacts_bias, *, preact_trainable: b
 
 
 # ---------------------------------------------------------------------------- dense operators
+# Small problems of these operators are bound by the host, so the path from call to launch is kept short: descriptors
+# go by reference, tensors that are already as the kernels want them are passed as they are, one look at each argument.
+_DENSE_IO = {torch.float32: _abi.QK_F32, torch.bfloat16: _abi.QK_BF16}
+_GRADS = ("x", "weight", "bias")
+
+
 def _activation_code(activation) -> int:
+    code = _abi.ACTIVATION_CODES.get(activation) if type(activation) is str else None
+    if code is not None:
+        return code
     try:
         return _abi.ACTIVATION_CODES["none" if activation is None else activation.lower()]
     except (KeyError, AttributeError):
@@ -486,22 +497,41 @@ def _activation_code(activation) -> int:
             f"Unknown activation {activation!r}. Supported: {sorted(_abi.ACTIVATION_CODES)}") from None
 
 
-def _check_like(t: Optional[torch.Tensor], name: str, shape, dtype: torch.dtype, dev: torch.device) -> None:
-    if t is not None and (t.shape != shape or t.dtype != dtype or t.device != dev):
+def _check_like(t: torch.Tensor, name: str, shape, dtype: torch.dtype, dev: torch.device) -> None:
+    if t.shape != shape or t.dtype is not dtype or t.device != dev:
         raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)} on {dev}, "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _rows_of(x: torch.Tensor, name: str) -> int:
-    """Number of rows of ``x`` seen as a matrix over its last axis; the kernels count rows and columns in 32 bits."""
-    if x.dim() < 1:
-        raise ValueError(f"{name} must have at least one dimension")
-    rows = 1
-    for n in x.shape[:-1]:
-        rows *= n
-    if max(rows, x.shape[-1]) >= 1 << 31:
-        raise ValueError(f"{name} {tuple(x.shape)}: rows and columns must stay below 2**31")
+def _dense_io(t: torch.Tensor) -> int:
+    """The type's code; tensors off the GPU and other types are refused."""
+    _require_cuda(t, "x")
+    code = _DENSE_IO.get(t.dtype)
+    return _io_dtype(t) if code is None else code
+
+
+def _rows_of(shape) -> int:
+    """Number of rows of a tensor seen as a matrix over its last axis; the kernels count rows and columns in 32 bits."""
+    if len(shape) == 2:
+        rows = shape[0]
+    elif shape:
+        rows = math.prod(shape[:-1])
+    else:
+        raise ValueError("x must have at least one dimension")
+    if rows >= 1 << 31 or shape[-1] >= 1 << 31:
+        raise ValueError(f"x {tuple(shape)}: rows and columns must stay below 2**31")
     return rows
+
+
+def _packed(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and on a 16-byte boundary (a view may start anywhere in its storage)."""
+    if t.is_contiguous():
+        return t if t.data_ptr() % 16 == 0 else t.detach().clone()
+    return t.detach().contiguous()
 
 
 def _call(dev: torch.device, fn, what: str, *args) -> None:
@@ -515,10 +545,13 @@ def _call(dev: torch.device, fn, what: str, *args) -> None:
         _abi.check(rc, what)
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` contiguous and on a 16-byte boundary (a view may start anywhere in its storage)."""
-    t = t.detach().contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _scratch(dev: torch.device, nbytes: int, what: str):
+    """(tensor, address, bytes) of a call's scratch; a size of 1 says that none is needed, 0 that the call is refused."""
+    if nbytes <= 1:
+        _abi.check(0 if nbytes else _abi.QK_ERR_BAD_ARGUMENT, what)
+        return None, None, 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return ws, ws.data_ptr(), nbytes
 
 
 def dense_status() -> None:
@@ -529,19 +562,17 @@ def dense_status() -> None:
     _abi.check(_abi.load().qk_dense_status(torch.cuda.current_stream().cuda_stream), "qk_dense_status")
 
 
-def _linear_desc(x: torch.Tensor, weight: torch.Tensor, code: int) -> _abi.QkLinearDesc:
-    _require_cuda(x, "x")
-    io = _io_dtype(x)
-    if weight.dim() != 2:
-        raise ValueError(f"weight must be (out_features, in_features), got {tuple(weight.shape)}")
-    rows = _rows_of(x, "x")
-    N, K = weight.shape
-    if x.shape[-1] != K:
-        raise ValueError(f"x {tuple(x.shape)} does not match weight {tuple(weight.shape)}")
-    _check_like(weight, "weight", weight.shape, x.dtype, x.device)
-    if N >= 1 << 31:
-        raise ValueError("out_features must stay below 2**31")
-    return _abi.QkLinearDesc(rows, K, N, io, code, 0)
+def _linear_shape(x: torch.Tensor, weight: torch.Tensor):
+    """(io code, rows, K, N, shape of y), checked."""
+    io = _dense_io(x)
+    xs, wshape = x.shape, weight.shape
+    rows = _rows_of(xs)
+    if len(wshape) != 2 or wshape[1] != xs[-1]:
+        raise ValueError(f"weight must be (out_features, {xs[-1]}) for x {tuple(xs)}, got {tuple(wshape)}")
+    N, K = wshape
+    if weight.dtype is not x.dtype or weight.device != x.device or N >= 1 << 31:
+        _check_like(weight, "weight", (min(N, (1 << 31) - 1), K), x.dtype, x.device)
+    return io, rows, K, N, ((rows, N) if len(xs) == 2 else (*xs[:-1], N))
 
 
 def linear_forward(x, weight, bias=None, *, activation="none", residual=None, return_tape: bool = False):
@@ -553,53 +584,58 @@ def linear_forward(x, weight, bias=None, *, activation="none", residual=None, re
     """
     lib = _abi.load()
     code = _activation_code(activation)
-    desc = _linear_desc(x, weight, code)
+    io, rows, K, N, shape = _linear_shape(x, weight)
     dev, dt = x.device, x.dtype
-    shape = x.shape[:-1] + weight.shape[:1]
-    _check_like(bias, "bias", weight.shape[:1], dt, dev)
-    _check_like(residual, "residual", shape, dt, dev)
+    if bias is not None:
+        _check_like(bias, "bias", (N,), dt, dev)
+        bias = _packed(bias)
+    if residual is not None:
+        _check_like(residual, "residual", shape, dt, dev)
+        residual = _packed(residual)
     x, weight = _aligned(x), _aligned(weight)
-    bias = None if bias is None else bias.detach().contiguous()
-    residual = None if residual is None else residual.detach().contiguous()
     y = torch.empty(shape, dtype=dt, device=dev)
     tape = None
-    if return_tape and code != _abi.QK_ACT_NONE:
-        tape = torch.empty(shape, dtype=torch.float32 if dt == torch.float32 else torch.float16, device=dev)
-    dp = _abi.desc_pointer(desc)
-    ws = _workspace(dev, lib.qk_linear_forward_workspace_bytes(dp))
-    _call(dev, lib.qk_linear_forward, "qk_linear_forward", dp, _ptr(x), _ptr(weight), _ptr(bias), _ptr(residual),
-          _ptr(y), _ptr(tape), _ptr(ws), ws.numel())
+    if return_tape and code:
+        tape = torch.empty(shape, dtype=torch.float16 if io else torch.float32, device=dev)
+    desc = byref(_abi.QkLinearDesc(rows, K, N, io, code, 0))
+    ws, ws_at, nbytes = _scratch(dev, lib.qk_linear_forward_workspace_bytes(desc), "qk_linear_forward_workspace_bytes")
+    _call(dev, lib.qk_linear_forward, "qk_linear_forward", desc, x.data_ptr(), weight.data_ptr(), _ptr(bias),
+          _ptr(residual), y.data_ptr(), _ptr(tape), ws_at, nbytes)
     return (y, tape) if return_tape else y
 
 
-def linear_backward(x, weight, gy, *, tape=None, activation="none", want=("x", "weight", "bias")) -> dict:
+def _check_want(want) -> None:
+    for name in want:
+        if name not in _GRADS:
+            raise ValueError(f"unknown gradient {name!r}: {_GRADS} can be asked for")
+
+
+def linear_backward(x, weight, gy, *, tape=None, activation="none", want=_GRADS) -> dict:
     """Gradients of ``sum(linear_forward(x, weight, bias, ...) * gy)`` by name; the residual's is ``gy`` itself.
 
     ``tape`` is what the forward returned with the same ``activation``.
     """
     lib = _abi.load()
     code = _activation_code(activation)
-    desc = _linear_desc(x, weight, code)
+    io, rows, K, N, shape = _linear_shape(x, weight)
     dev, dt = x.device, x.dtype
-    unknown = set(want) - {"x", "weight", "bias"}
-    if unknown:
-        raise ValueError(f"unknown gradients {sorted(unknown)}")
-    shape = x.shape[:-1] + weight.shape[:1]
+    _check_want(want)
     _check_like(gy, "gy", shape, dt, dev)
-    if code != _abi.QK_ACT_NONE:
-        if tape is None:
-            raise ValueError(f"activation {activation!r} needs the tape of its forward (return_tape=True)")
-        _check_like(tape, "tape", shape, torch.float32 if dt == torch.float32 else torch.float16, dev)
-        tape = tape.contiguous()
-    else:
+    if not code:
         tape = None
+    elif tape is None:
+        raise ValueError(f"activation {activation!r} needs the tape of its forward (return_tape=True)")
+    else:
+        _check_like(tape, "tape", shape, torch.float16 if io else torch.float32, dev)
+        tape = _packed(tape)
     x, weight, gy = _aligned(x), _aligned(weight), _aligned(gy)
-    shapes = {"x": x.shape, "weight": weight.shape, "bias": weight.shape[:1]}
-    out = {n: torch.empty(shapes[n], dtype=dt, device=dev) for n in want}
-    dp = _abi.desc_pointer(desc)
-    ws = _workspace(dev, lib.qk_linear_backward_workspace_bytes(dp))
-    _call(dev, lib.qk_linear_backward, "qk_linear_backward", dp, _ptr(x), _ptr(weight), _ptr(tape), _ptr(gy),
-          _ptr(out.get("x")), _ptr(out.get("weight")), _ptr(out.get("bias")), _ptr(ws), ws.numel())
+    out = {}
+    for name in want:
+        out[name] = torch.empty(x.shape if name == "x" else (N, K) if name == "weight" else (N,), dtype=dt, device=dev)
+    desc = byref(_abi.QkLinearDesc(rows, K, N, io, code, 0))
+    ws, ws_at, nbytes = _scratch(dev, lib.qk_linear_backward_workspace_bytes(desc), "qk_linear_backward_workspace_bytes")
+    _call(dev, lib.qk_linear_backward, "qk_linear_backward", desc, x.data_ptr(), weight.data_ptr(), _ptr(tape),
+          gy.data_ptr(), _ptr(out.get("x")), _ptr(out.get("weight")), _ptr(out.get("bias")), ws_at, nbytes)
     return out
 
 
@@ -616,9 +652,13 @@ class _LinearFunction(torch.autograd.Function):
     def backward(ctx, gy):
         x, weight, tape = ctx.saved_tensors
         need = ctx.needs_input_grad
-        want = tuple(n for n, wanted in zip(("x", "weight", "bias"), need) if wanted)
+        want = tuple(n for n, wanted in zip(_GRADS, need) if wanted)
         g = linear_backward(x, weight, gy, tape=tape, activation=ctx.activation, want=want) if want else {}
         return g.get("x"), g.get("weight"), g.get("bias"), gy if need[3] else None, None
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def fused_linear(x, weight, bias=None, *, activation="none", residual=None) -> torch.Tensor:
@@ -628,25 +668,27 @@ def fused_linear(x, weight, bias=None, *, activation="none", residual=None) -> t
     projection of a pre-norm block, without one the projections of the reference's ``FusedHQKAN``
     (``src/qkan/solver/cute/cute_ops.py:449-490``).
     """
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if _wants_grad(x, weight, bias, residual):
         return _LinearFunction.apply(x, weight, bias, residual, activation)
     return linear_forward(x, weight, bias, activation=activation, residual=residual)
 
 
-def _norm_desc(x: torch.Tensor, weight, bias, eps: float) -> _abi.QkNormDesc:
-    _require_cuda(x, "x")
-    io = _io_dtype(x)
-    rows = _rows_of(x, "x")
+def _norm_shape(x: torch.Tensor, weight, bias, param_dtype=None):
+    """(io code, rows, D, code and dtype of the parameters), checked."""
+    io = _dense_io(x)
+    rows = _rows_of(x.shape)
     D = x.shape[-1]
     if D < 1:
         raise ValueError("layer_norm needs at least one element per row")
-    if not 0.0 <= eps < float("inf"):
-        raise ValueError(f"eps must be finite and >= 0, got {eps}")
-    param = next((t for t in (weight, bias) if t is not None), x)
-    pdt = _io_dtype(param)
-    _check_like(weight, "weight", x.shape[-1:], param.dtype, x.device)
-    _check_like(bias, "bias", x.shape[-1:], param.dtype, x.device)
-    return _abi.QkNormDesc(rows, D, io, pdt, eps, 0)
+    pdt = weight.dtype if weight is not None else bias.dtype if bias is not None else param_dtype or x.dtype
+    code = _DENSE_IO.get(pdt)
+    if code is None:
+        raise TypeError(f"layer_norm parameters are float32 or bfloat16, got {pdt}")
+    if weight is not None:
+        _check_like(weight, "weight", (D,), pdt, x.device)
+    if bias is not None:
+        _check_like(bias, "bias", (D,), pdt, x.device)
+    return io, rows, D, code, pdt
 
 
 def layer_norm_forward(x, weight=None, bias=None, *, eps: float = 1e-5, return_stats: bool = True):
@@ -656,42 +698,38 @@ def layer_norm_forward(x, weight=None, bias=None, *, eps: float = 1e-5, return_s
     float32 holds each row's mean and ``1 / sqrt(var + eps)`` for ``layer_norm_backward`` (None without ``return_stats``).
     """
     lib = _abi.load()
-    desc = _norm_desc(x, weight, bias, eps)
-    x = x.detach().contiguous()
-    weight = None if weight is None else weight.detach().contiguous()
-    bias = None if bias is None else bias.detach().contiguous()
-    y = torch.empty_like(x)
-    stats = torch.empty(x.shape[:-1] + (2,), dtype=torch.float32, device=x.device) if return_stats else None
-    _call(x.device, lib.qk_layer_norm_forward, "qk_layer_norm_forward", _abi.desc_pointer(desc), _ptr(x), _ptr(weight),
-          _ptr(bias), _ptr(y), _ptr(stats))
+    io, rows, D, pcode, _ = _norm_shape(x, weight, bias)
+    if not 0.0 <= eps < math.inf:
+        raise ValueError(f"eps must be finite and >= 0, got {eps}")
+    dev = x.device
+    x, weight, bias = _packed(x), _packed(weight), _packed(bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    stats = torch.empty((*x.shape[:-1], 2), dtype=torch.float32, device=dev) if return_stats else None
+    _call(dev, lib.qk_layer_norm_forward, "qk_layer_norm_forward", byref(_abi.QkNormDesc(rows, D, io, pcode, eps, 0)),
+          x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(stats))
     return y, stats
 
 
-def layer_norm_backward(x, weight, stats, gy, *, want=("x", "weight", "bias"), param_dtype=None) -> dict:
+def layer_norm_backward(x, weight, stats, gy, *, want=_GRADS, param_dtype=None) -> dict:
     """Gradients of ``sum(layer_norm(x, weight, bias) * gy)`` by name, from the statistics of the forward.
 
     ``weight`` None stands for ones; the parameters' gradients have the weight's dtype, or ``param_dtype`` where there is
     no weight (default: that of ``x``).
     """
     lib = _abi.load()
-    desc = _norm_desc(x, weight, None, 0.0)
+    io, rows, D, pcode, pdt = _norm_shape(x, weight, None, param_dtype)
     dev = x.device
-    unknown = set(want) - {"x", "weight", "bias"}
-    if unknown:
-        raise ValueError(f"unknown gradients {sorted(unknown)}")
+    _check_want(want)
     _check_like(gy, "gy", x.shape, x.dtype, dev)
-    _check_like(stats, "stats", x.shape[:-1] + (2,), torch.float32, dev)
-    pdt = weight.dtype if weight is not None else (param_dtype or x.dtype)
-    if pdt not in (torch.float32, torch.bfloat16):
-        raise TypeError(f"parameters are float32 or bfloat16, got {pdt}")
-    desc.param_dtype = _abi.QK_F32 if pdt == torch.float32 else _abi.QK_BF16
-    x, gy, stats = x.detach().contiguous(), gy.detach().contiguous(), stats.contiguous()
-    weight = None if weight is None else weight.detach().contiguous()
-    out = {n: torch.empty_like(x) if n == "x" else torch.empty(x.shape[-1:], dtype=pdt, device=dev) for n in want}
-    dp = _abi.desc_pointer(desc)
-    ws = _workspace(dev, lib.qk_layer_norm_backward_workspace_bytes(dp))
-    _call(dev, lib.qk_layer_norm_backward, "qk_layer_norm_backward", dp, _ptr(x), _ptr(weight), _ptr(stats), _ptr(gy),
-          _ptr(out.get("x")), _ptr(out.get("weight")), _ptr(out.get("bias")), _ptr(ws), ws.numel())
+    _check_like(stats, "stats", (*x.shape[:-1], 2), torch.float32, dev)
+    x, gy, stats, weight = _packed(x), _packed(gy), _packed(stats), _packed(weight)
+    out = {}
+    for name in want:
+        out[name] = torch.empty(x.shape if name == "x" else (D,), dtype=x.dtype if name == "x" else pdt, device=dev)
+    desc = byref(_abi.QkNormDesc(rows, D, io, pcode, 0.0, 0))
+    ws, ws_at, nbytes = _scratch(dev, lib.qk_layer_norm_backward_workspace_bytes(desc), "qk_layer_norm_backward_workspace_bytes")
+    _call(dev, lib.qk_layer_norm_backward, "qk_layer_norm_backward", desc, x.data_ptr(), _ptr(weight), stats.data_ptr(),
+          gy.data_ptr(), _ptr(out.get("x")), _ptr(out.get("weight")), _ptr(out.get("bias")), ws_at, nbytes)
     return out
 
 
@@ -708,13 +746,13 @@ class _LayerNormFunction(torch.autograd.Function):
     def backward(ctx, gy):
         x, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        want = tuple(n for n, wanted in zip(("x", "weight", "bias"), need) if wanted)
+        want = tuple(n for n, wanted in zip(_GRADS, need) if wanted)
         g = layer_norm_backward(x, weight, stats, gy, want=want, param_dtype=ctx.bias_dtype)
         return g.get("x"), g.get("weight"), g.get("bias"), None
 
 
 def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5) -> torch.Tensor:
     """Differentiable layer norm over the last axis (``layer_norm_forward`` / ``layer_norm_backward``)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _wants_grad(x, weight, bias):
         return _LayerNormFunction.apply(x, weight, bias, eps)
     return layer_norm_forward(x, weight, bias, eps=eps, return_stats=False)[0]
