@@ -6,6 +6,7 @@ import of a compute entry point raises, there is no eager or CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 from ctypes import Structure, c_char_p, c_float, c_int, c_int32, c_size_t, c_uint32, c_void_p
 
@@ -143,6 +144,30 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+_dense = None
+
+
+def dense():
+    """The binding of the dense operators (``csrc/dense_binding.cpp``), loaded once beside the library."""
+    global _dense
+    if _dense is None:
+        load()
+        path = os.path.join(os.path.dirname(LIB_PATH), "_dense.so")
+        if not os.path.exists(path):
+            raise QkanLibraryError(f"{path} not found: build it with `python -m qkan_b200.build` "
+                                   "(this package has no fallback path)")
+        try:
+            spec = importlib.util.spec_from_file_location("_dense", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as exc:
+            raise QkanLibraryError(f"{path} does not load ({exc}); rebuild it against the installed torch") from exc
+        if module.abi_version() != QK_ABI_VERSION:
+            raise QkanLibraryError(f"ABI mismatch: {path} has {module.abi_version()}, this package {QK_ABI_VERSION}; rebuild")
+        _dense = module
+    return _dense
+
+
 def last_error() -> str:
     return load().qk_last_error().decode("utf-8", "replace")
 
@@ -163,4 +188,4 @@ def desc_pointer(desc: Structure):
 
 
 __all__ = [name for name in dir() if name.startswith("QK") or name in (
-    "QkDesc", "QkLinearDesc", "QkNormDesc", "QkanLibraryError", "ANSATZ_CODES", "ACTIVATION_CODES", "load", "last_error", "check", "desc_pointer", "SYMBOLS", "LIB_PATH")]
+    "QkDesc", "QkLinearDesc", "QkNormDesc", "QkanLibraryError", "ANSATZ_CODES", "ACTIVATION_CODES", "load", "dense", "last_error", "check", "desc_pointer", "SYMBOLS", "LIB_PATH")]

@@ -3,20 +3,26 @@
 ``python -m qkan_b200.build`` compiles every ``csrc/*.cu`` with nvcc for
 ``sm_100a`` only and links one shared library that exports the C ABI declared in
 ``include/qkan_b200.h``. nvcc cross-compiles, so no GPU is needed to build.
+The Python binding of the dense operators (``csrc/dense_binding.cpp`` ->
+``lib/_dense.so``, against torch's headers) is built beside it.
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
 import glob
 import os
+import importlib.util
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "lib", "obj")
 LIB = os.path.join(PKG, "lib", "libqkan_b200.so")
+BINDING_SRC = os.path.join(CSRC, "dense_binding.cpp")
+BINDING = os.path.join(PKG, "lib", "_dense.so")
 INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 
 NVCC_FLAGS = [
@@ -43,10 +49,34 @@ def _deps():
 
 
 def is_stale() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(BINDING):
         return True
     t = os.path.getmtime(LIB)
-    return any(os.path.getmtime(p) > t for p in _deps())
+    return any(os.path.getmtime(p) > t for p in _deps()) or _binding_is_stale()
+
+
+def _binding_is_stale() -> bool:
+    deps = [BINDING_SRC, *glob.glob(os.path.join(INCLUDE, "*.h"))]
+    return not os.path.exists(BINDING) or os.path.getmtime(BINDING) <= max(os.path.getmtime(p) for p in deps)
+
+
+def _build_binding(force: bool = False) -> str:
+    """Host code only: compiled and linked by g++ against torch and, by symbol, against the kernel library."""
+    if not force and not _binding_is_stale():
+        return BINDING
+    torch_dir = list(importlib.util.find_spec("torch").submodule_search_locations)[0]
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+               os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    lib = os.path.join(torch_dir, "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+           *[f"-I{d}" for d in include], BINDING_SRC, "-o", BINDING, f"-L{lib}", f"-L{os.path.dirname(LIB)}",
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-lqkan_b200",
+           "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib}"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING_SRC}:\n{res.stderr[-4000:]}")
+    return BINDING
 
 
 # per-repetition template instantiations (csrc/*_inst.cu): 0 is the "real" ansatz, 12 and 16 serve 9..16 by padding
@@ -93,6 +123,7 @@ def build(force: bool = False, extra_flags=()) -> str:
                           "arch=compute_100a,code=sm_100a"], capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr[-4000:]}")
+    _build_binding(force)
     return LIB
 
 

@@ -53,27 +53,37 @@ cudaError_t launch_norm_forward(const NormArgs& a, cudaStream_t st);
 cudaError_t launch_norm_backward(const NormArgs& a, cudaStream_t st);
 
 // ---- linear map --------------------------------------------------------------
-// act(z) and its derivative, float32, by CUDA's own functions
-__device__ __forceinline__ float sigmoid_of(float z) { return 1.f / (1.f + expf(-z)); }
+// act(z) and its derivative in float32, by CUDA's own functions. FAST, for values that are rounded to bfloat16 next: exp
+// and division by the special-function unit (off by some 2^-20 where bfloat16 is off by 2^-9). tanh and erf are the full
+// ones throughout: near zero theirs is a relative error.
+template <bool FAST>
+__device__ __forceinline__ float over_one_plus_exp(float num, float z) {  // num / (1 + exp(-z))
+    if constexpr (FAST) return __fdividef(num, 1.f + __expf(-z));
+    else return num / (1.f + expf(-z));
+}
+template <bool FAST>
 __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {
-        case QK_ACT_SILU: return z / (1.f + expf(-z));
+        case QK_ACT_SILU: return over_one_plus_exp<FAST>(z, z);
         case QK_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
         case QK_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(0.79788456080286536f * fmaf(0.044715f * z * z, z, z)));
         case QK_ACT_RELU: return z < 0.f ? 0.f : z;  // a NaN stays one
         case QK_ACT_TANH: return tanhf(z);
-        case QK_ACT_SIGMOID: return sigmoid_of(z);
+        case QK_ACT_SIGMOID: return over_one_plus_exp<FAST>(1.f, z);
         default: return z;
     }
 }
+template <bool FAST>
 __device__ __forceinline__ float act_slope(float z, int act) {
     switch (act) {
         case QK_ACT_SILU: {
-            const float s = sigmoid_of(z);
+            const float s = over_one_plus_exp<FAST>(1.f, z);
             return s * fmaf(z, 1.f - s, 1.f);
         }
-        case QK_ACT_GELU:
-            return fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
+        case QK_ACT_GELU: {
+            const float e = FAST ? __expf(-0.5f * z * z) : expf(-0.5f * z * z);
+            return fmaf(z * 0.39894228040143268f, e, 0.5f * (1.f + erff(z * 0.70710678118654752f)));
+        }
         case QK_ACT_GELU_TANH: {
             const float t = tanhf(0.79788456080286536f * fmaf(0.044715f * z * z, z, z));
             return 0.5f * (1.f + t) +
@@ -85,10 +95,45 @@ __device__ __forceinline__ float act_slope(float z, int act) {
             return 1.f - t * t;
         }
         case QK_ACT_SIGMOID: {
-            const float s = sigmoid_of(z);
+            const float s = over_one_plus_exp<FAST>(1.f, z);
             return s * (1.f - s);
         }
         default: return 1.f;
+    }
+}
+// the same for N values at once, one test of `act` for all
+template <bool FAST, int N>
+__device__ __forceinline__ void activate_all(float (&v)[N], int act) {
+    switch (act) {
+#define QK_CASE(code)                                                                 \
+    case code:                                                                        \
+        _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] = activate<FAST>(v[i], code); \
+        break;
+        QK_CASE(QK_ACT_SILU)
+        QK_CASE(QK_ACT_GELU)
+        QK_CASE(QK_ACT_GELU_TANH)
+        QK_CASE(QK_ACT_RELU)
+        QK_CASE(QK_ACT_TANH)
+        QK_CASE(QK_ACT_SIGMOID)
+        default: break;
+    }
+}
+template <bool FAST, int N>
+__device__ __forceinline__ void times_slope(float (&v)[N], const float (&z)[N], int act) {
+    switch (act) {
+#undef QK_CASE
+#define QK_CASE(code)                                                                      \
+    case code:                                                                             \
+        _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] *= act_slope<FAST>(z[i], code); \
+        break;
+        QK_CASE(QK_ACT_SILU)
+        QK_CASE(QK_ACT_GELU)
+        QK_CASE(QK_ACT_GELU_TANH)
+        QK_CASE(QK_ACT_RELU)
+        QK_CASE(QK_ACT_TANH)
+        QK_CASE(QK_ACT_SIGMOID)
+#undef QK_CASE
+        default: break;
     }
 }
 
@@ -124,7 +169,7 @@ __device__ __forceinline__ void finish_element(const Epilogue& e, size_t at, int
     float z = acc;
     if (e.bias) z += load_dt(e.bias, c, e.io_dtype);
     if (e.tape) store_tape(e.tape, at, e.io_dtype, z);
-    float y = activate(z, e.act);
+    float y = e.io_dtype == QK_BF16 ? activate<true>(z, e.act) : activate<false>(z, e.act);
     if (e.residual) y += load_dt(e.residual, at, e.io_dtype);
     store_dt(e.out, at, e.io_dtype, y);
 }

@@ -14,8 +14,7 @@
 // the nine products are kept: hh | hm mh hl lh mm; what is dropped is below 2^-22 of |x||w|. hh goes to one accumulator
 // and the five small ones to another. The tensor core truncates where it adds to its accumulator, which over a long
 // sum would drift by more than float32 rounding does: so hh is drained every kChunk blocks and added in registers, with
-// rounding. Only hh can be infinite or NaN (the other parts of such a value are zero), and where it is, the small
-// products are left out: float32's own infinities come out.
+// rounding. Where hh's sum is not finite the small products are left out: float32's own infinities come out.
 #include <cuda.h>
 
 #include "qk_linear.cuh"
@@ -169,24 +168,6 @@ __device__ __forceinline__ Unit unit_at(const GemmProblem& g, int u) {
     return t;
 }
 
-template <int N>
-__device__ __forceinline__ void activate_all(float (&v)[N], int act) {
-    switch (act) {
-#define QK_CASE(code) \
-    case code: \
-        _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] = activate(v[i], code); \
-        break;
-        QK_CASE(QK_ACT_SILU)
-        QK_CASE(QK_ACT_GELU)
-        QK_CASE(QK_ACT_GELU_TANH)
-        QK_CASE(QK_ACT_RELU)
-        QK_CASE(QK_ACT_TANH)
-        QK_CASE(QK_ACT_SIGMOID)
-#undef QK_CASE
-        default: break;
-    }
-}
-
 // The residual of column c, rows r .. r + N - 1, fetched before the sums are waited for. Row and column are held inside
 // the matrix, so that every load is good by itself; what lies behind its edge is never stored.
 template <typename IO, int N>
@@ -218,7 +199,7 @@ __device__ __forceinline__ void write_out(const GemmProblem& g, int split, long 
         for (int i = 0; i < N; ++i)
             if (i < n) store_tape(g.tape, at + i * cols, sizeof(IO) == 2 ? QK_BF16 : QK_F32, v[i]);
     }
-    activate_all(v, g.act);
+    activate_all<sizeof(IO) == 2>(v, g.act);
     IO* out = static_cast<IO*>(g.out) + at;
 #pragma unroll
     for (int i = 0; i < N; ++i)

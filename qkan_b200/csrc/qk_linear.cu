@@ -27,18 +27,15 @@ struct PrepArgsL {
     int count;
 };
 
-// x = h + m + l. h is x rounded to nearest, except that a finite x stays finite; m and l round what is left, which
-// is exact in float32. An infinity or a NaN is all in h.
-__device__ __forceinline__ void split3(float x, __nv_bfloat16& h, __nv_bfloat16& m, __nv_bfloat16& l) {
-    h = __float2bfloat16_rn(x);
-    if (__hisinf(h) && isfinite(x)) h = __ushort_as_bfloat16(x < 0.f ? 0xff7f : 0x7f7f);
-    if (!isfinite(x)) {
-        m = l = __float2bfloat16_rn(0.f);
-        return;
-    }
-    const float r = x - __bfloat162float(h);
-    m = __float2bfloat16_rn(r);
-    l = __float2bfloat16_rn(r - __bfloat162float(m));
+// x = h + m + l, two values at a time. h is x cut off after eight bits (rounding could reach infinity), m and l round
+// what is left, which is exact in float32 until l has it all. For an infinity or a NaN h is that, and m and l are NaN:
+// the products leave theirs out where h's are not finite.
+__device__ __forceinline__ void split3(float x, float y, unsigned& h, unsigned& m, unsigned& l) {
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(y), "f"(x));
+    x -= __uint_as_float(h << 16), y -= __uint_as_float(h & 0xffff0000u);
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(m) : "f"(y), "f"(x));
+    x -= __uint_as_float(m << 16), y -= __uint_as_float(m & 0xffff0000u);
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(l) : "f"(y), "f"(x));
 }
 
 template <typename IO>
@@ -68,9 +65,16 @@ __device__ __forceinline__ void load8(const void* p, size_t at, bool vec, int n,
 template <typename IO>
 __global__ void __launch_bounds__(kThreads) prepare_kernel(const PrepArgsL a) {
     __shared__ float sums[kThreads * 8];
-    int b = blockIdx.x, which = 0;
-    while (which + 1 < a.count && b >= a.job[which].blocks) b -= a.job[which++].blocks;
-    const PrepJob& j = a.job[which];
+    int b = blockIdx.x;
+    PrepJob j = a.job[0];  // in registers: a reference would be read again behind every store
+    if (a.count > 1 && b >= a.job[0].blocks) {
+        b -= a.job[0].blocks;
+        j = a.job[1];
+        if (a.count > 2 && b >= a.job[1].blocks) {
+            b -= a.job[1].blocks;
+            j = a.job[2];
+        }
+    }
     const int tx = threadIdx.x & ((1 << j.tx_log2) - 1), ty = threadIdx.x >> j.tx_log2, ny = kThreads >> j.tx_log2;
     const int slab = b / j.cblocks, c = ((b - slab * j.cblocks) << j.tx_log2 | tx) * 8;
     const long end = min((long)j.rows, (long)(slab + 1) * j.slab_rows);
@@ -87,25 +91,24 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const PrepArgsL a) {
                 float z[8];
                 if constexpr (sizeof(IO) == 4) load8<float>(j.tape, at, j.vec, n, z);
                 else load8<__half>(j.tape, at, j.vec, n, z);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = i < n ? v[i] * act_slope(z[i], j.act) : 0.f;
+                times_slope<sizeof(IO) == 2>(v, z, j.act);  // columns past the end: 0 times a slope at 0
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[i] += v[i];
             if (!j.dst) continue;
-            __align__(16) __nv_bfloat16 h[8];
             uint4* out = reinterpret_cast<uint4*>(j.dst + (size_t)r * j.ld + c);
+            unsigned h[4];
             if constexpr (sizeof(IO) == 4) {
-                __align__(16) __nv_bfloat16 m[8], l[8];
+                unsigned m[4], l[4];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) split3(v[i], h[i], m[i], l[i]);
-                out[plane / 8] = *reinterpret_cast<uint4*>(m);
-                out[plane / 4] = *reinterpret_cast<uint4*>(l);
+                for (int i = 0; i < 4; ++i) split3(v[2 * i], v[2 * i + 1], h[i], m[i], l[i]);
+                out[plane / 8] = make_uint4(m[0], m[1], m[2], m[3]);
+                out[plane / 4] = make_uint4(l[0], l[1], l[2], l[3]);
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) h[i] = __float2bfloat16_rn(v[i]);
+                for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(h[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
             }
-            out[0] = *reinterpret_cast<uint4*>(h);
+            out[0] = make_uint4(h[0], h[1], h[2], h[3]);
         }
     }
     if (!j.colpart) return;
@@ -139,10 +142,16 @@ struct ReduceArgs {
 // One element per thread: the slices of its sum in order, then the epilogue. The blocks behind those add grad_bias'
 // slabs, 32 columns each.
 __global__ void __launch_bounds__(kThreads) reduce_kernel(const ReduceArgs a) {
-    int b = blockIdx.x, which = 0;
-    while (which < a.count && b >= a.job[which].blocks) b -= a.job[which++].blocks;
-    if (which < a.count) {
-        const ReduceJob& j = a.job[which];
+    int b = blockIdx.x;
+    ReduceJob j = a.job[0];
+    bool sums = a.count > 0 && b < j.blocks;
+    if (a.count > 0 && !sums) {
+        b -= j.blocks;
+        j = a.job[1];
+        sums = a.count > 1 && b < j.blocks;
+        if (a.count > 1 && !sums) b -= j.blocks;
+    }
+    if (sums) {
         const size_t i = (size_t)b * kThreads + threadIdx.x;
         if (i >= j.n) return;
         float s = 0.f;
@@ -229,16 +238,16 @@ int blocks_of(long depth) { return (int)((depth + 63) / 64); }
 struct Slabs {
     int rows, count, cblocks, tx_log2;
 };
-// 256 threads as 2^tx_log2 groups of eight columns by the rest in rows; enough slabs of rows for four CTAs per SM, each
-// of eight rows per thread at least
+// 256 threads as 2^tx_log2 groups of eight columns by the rest in rows; enough slabs of rows for eight CTAs per SM, each
+// of two rows per thread at least
 Slabs slabs_of(long rows, long cols) {
     const long groups = padded(cols) / 8;
     Slabs s{};
     while (s.tx_log2 < 5 && (1 << s.tx_log2) < groups) ++s.tx_log2;
     s.cblocks = (int)((groups + (1 << s.tx_log2) - 1) >> s.tx_log2);
     const long ny = kThreads >> s.tx_log2;
-    long want = (4l * kSms + s.cblocks - 1) / s.cblocks;
-    const long most = (rows + 8 * ny - 1) / (8 * ny);
+    long want = (8l * kSms + s.cblocks - 1) / s.cblocks;
+    const long most = (rows + 2 * ny - 1) / (2 * ny);
     if (want > most) want = most;
     if (want < 1) want = 1;
     s.rows = (int)((rows + want - 1) / want);

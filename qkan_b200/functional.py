@@ -7,8 +7,6 @@ torch is used for device memory, the current stream and autograd bookkeeping onl
 """
 from __future__ import annotations
 
-import math
-from ctypes import byref
 from typing import Optional
 
 import torch
@@ -480,10 +478,10 @@ def qkan_postacts(x, theta, preacts_weight, preacts_bias, *, preact_trainable: b
 
 
 # ---------------------------------------------------------------------------- dense operators
-# Small problems of these operators are bound by the host, so the path from call to launch is kept short: descriptors
-# go by reference, tensors that are already as the kernels want them are passed as they are, one look at each argument.
-_DENSE_IO = {torch.float32: _abi.QK_F32, torch.bfloat16: _abi.QK_BF16}
+# Arguments are checked, and results and scratch allocated, in the compiled binding (``csrc/dense_binding.cpp``): small
+# problems of these operators are bound by the host.
 _GRADS = ("x", "weight", "bias")
+_GRAD_BITS = {"x": 1, "weight": 2, "bias": 4}
 
 
 def _activation_code(activation) -> int:
@@ -497,61 +495,21 @@ def _activation_code(activation) -> int:
             f"Unknown activation {activation!r}. Supported: {sorted(_abi.ACTIVATION_CODES)}") from None
 
 
-def _check_like(t: torch.Tensor, name: str, shape, dtype: torch.dtype, dev: torch.device) -> None:
-    if t.shape != shape or t.dtype is not dtype or t.device != dev:
-        raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)} on {dev}, "
-                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _want_bits(want) -> int:
+    bits = 0
+    for name in want:
+        if name not in _GRAD_BITS:
+            raise ValueError(f"unknown gradient {name!r}: {_GRADS} can be asked for")
+        bits |= _GRAD_BITS[name]
+    return bits
 
 
-def _dense_io(t: torch.Tensor) -> int:
-    """The type's code; tensors off the GPU and other types are refused."""
-    _require_cuda(t, "x")
-    code = _DENSE_IO.get(t.dtype)
-    return _io_dtype(t) if code is None else code
+def _named(grads, want) -> dict:
+    return {name: grads[_GRADS.index(name)] for name in want}
 
 
-def _rows_of(shape) -> int:
-    """Number of rows of a tensor seen as a matrix over its last axis; the kernels count rows and columns in 32 bits."""
-    if len(shape) == 2:
-        rows = shape[0]
-    elif shape:
-        rows = math.prod(shape[:-1])
-    else:
-        raise ValueError("x must have at least one dimension")
-    if rows >= 1 << 31 or shape[-1] >= 1 << 31:
-        raise ValueError(f"x {tuple(shape)}: rows and columns must stay below 2**31")
-    return rows
-
-
-def _packed(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return t if t is None or t.is_contiguous() else t.contiguous()
-
-
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` contiguous and on a 16-byte boundary (a view may start anywhere in its storage)."""
-    if t.is_contiguous():
-        return t if t.data_ptr() % 16 == 0 else t.detach().clone()
-    return t.detach().contiguous()
-
-
-def _call(dev: torch.device, fn, what: str, *args) -> None:
-    """Run a C entry point, its last argument the current stream of ``dev``, with that device current."""
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-    if rc:
-        _abi.check(rc, what)
-
-
-def _scratch(dev: torch.device, nbytes: int, what: str):
-    """(tensor, address, bytes) of a call's scratch; a size of 1 says that none is needed, 0 that the call is refused."""
-    if nbytes <= 1:
-        _abi.check(0 if nbytes else _abi.QK_ERR_BAD_ARGUMENT, what)
-        return None, None, 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    return ws, ws.data_ptr(), nbytes
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def dense_status() -> None:
@@ -562,19 +520,6 @@ def dense_status() -> None:
     _abi.check(_abi.load().qk_dense_status(torch.cuda.current_stream().cuda_stream), "qk_dense_status")
 
 
-def _linear_shape(x: torch.Tensor, weight: torch.Tensor):
-    """(io code, rows, K, N, shape of y), checked."""
-    io = _dense_io(x)
-    xs, wshape = x.shape, weight.shape
-    rows = _rows_of(xs)
-    if len(wshape) != 2 or wshape[1] != xs[-1]:
-        raise ValueError(f"weight must be (out_features, {xs[-1]}) for x {tuple(xs)}, got {tuple(wshape)}")
-    N, K = wshape
-    if weight.dtype is not x.dtype or weight.device != x.device or N >= 1 << 31:
-        _check_like(weight, "weight", (min(N, (1 << 31) - 1), K), x.dtype, x.device)
-    return io, rows, K, N, ((rows, N) if len(xs) == 2 else (*xs[:-1], N))
-
-
 def linear_forward(x, weight, bias=None, *, activation="none", residual=None, return_tape: bool = False):
     """``act(x weight^T + bias) + residual`` on the last axis of ``x``; no autograd (see ``fused_linear``).
 
@@ -582,32 +527,8 @@ def linear_forward(x, weight, bias=None, *, activation="none", residual=None, re
     ``return_tape=True`` returns ``(y, tape)``: what ``linear_backward`` needs of the activation's argument (None for
     ``activation="none"``).
     """
-    lib = _abi.load()
-    code = _activation_code(activation)
-    io, rows, K, N, shape = _linear_shape(x, weight)
-    dev, dt = x.device, x.dtype
-    if bias is not None:
-        _check_like(bias, "bias", (N,), dt, dev)
-        bias = _packed(bias)
-    if residual is not None:
-        _check_like(residual, "residual", shape, dt, dev)
-        residual = _packed(residual)
-    x, weight = _aligned(x), _aligned(weight)
-    y = torch.empty(shape, dtype=dt, device=dev)
-    tape = None
-    if return_tape and code:
-        tape = torch.empty(shape, dtype=torch.float16 if io else torch.float32, device=dev)
-    desc = byref(_abi.QkLinearDesc(rows, K, N, io, code, 0))
-    ws, ws_at, nbytes = _scratch(dev, lib.qk_linear_forward_workspace_bytes(desc), "qk_linear_forward_workspace_bytes")
-    _call(dev, lib.qk_linear_forward, "qk_linear_forward", desc, x.data_ptr(), weight.data_ptr(), _ptr(bias),
-          _ptr(residual), y.data_ptr(), _ptr(tape), ws_at, nbytes)
-    return (y, tape) if return_tape else y
-
-
-def _check_want(want) -> None:
-    for name in want:
-        if name not in _GRADS:
-            raise ValueError(f"unknown gradient {name!r}: {_GRADS} can be asked for")
+    out = _abi.dense().linear_forward(x, weight, bias, residual, _activation_code(activation), return_tape)
+    return out if return_tape else out[0]
 
 
 def linear_backward(x, weight, gy, *, tape=None, activation="none", want=_GRADS) -> dict:
@@ -615,36 +536,15 @@ def linear_backward(x, weight, gy, *, tape=None, activation="none", want=_GRADS)
 
     ``tape`` is what the forward returned with the same ``activation``.
     """
-    lib = _abi.load()
-    code = _activation_code(activation)
-    io, rows, K, N, shape = _linear_shape(x, weight)
-    dev, dt = x.device, x.dtype
-    _check_want(want)
-    _check_like(gy, "gy", shape, dt, dev)
-    if not code:
-        tape = None
-    elif tape is None:
-        raise ValueError(f"activation {activation!r} needs the tape of its forward (return_tape=True)")
-    else:
-        _check_like(tape, "tape", shape, torch.float16 if io else torch.float32, dev)
-        tape = _packed(tape)
-    x, weight, gy = _aligned(x), _aligned(weight), _aligned(gy)
-    out = {}
-    for name in want:
-        out[name] = torch.empty(x.shape if name == "x" else (N, K) if name == "weight" else (N,), dtype=dt, device=dev)
-    desc = byref(_abi.QkLinearDesc(rows, K, N, io, code, 0))
-    ws, ws_at, nbytes = _scratch(dev, lib.qk_linear_backward_workspace_bytes(desc), "qk_linear_backward_workspace_bytes")
-    _call(dev, lib.qk_linear_backward, "qk_linear_backward", desc, x.data_ptr(), weight.data_ptr(), _ptr(tape),
-          gy.data_ptr(), _ptr(out.get("x")), _ptr(out.get("weight")), _ptr(out.get("bias")), ws_at, nbytes)
-    return out
+    return _named(_abi.dense().linear_backward(x, weight, gy, tape, _activation_code(activation), _want_bits(want)), want)
 
 
 class _LinearFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation):
-        y, tape = linear_forward(x, weight, bias, activation=activation, residual=residual, return_tape=True)
+    def forward(ctx, x, weight, bias, residual, code):
+        y, tape = _abi.dense().linear_forward(x, weight, bias, residual, code, True)
         ctx.save_for_backward(x, weight, tape)
-        ctx.activation = activation
+        ctx.code = code
         return y
 
     @staticmethod
@@ -652,13 +552,9 @@ class _LinearFunction(torch.autograd.Function):
     def backward(ctx, gy):
         x, weight, tape = ctx.saved_tensors
         need = ctx.needs_input_grad
-        want = tuple(n for n, wanted in zip(_GRADS, need) if wanted)
-        g = linear_backward(x, weight, gy, tape=tape, activation=ctx.activation, want=want) if want else {}
-        return g.get("x"), g.get("weight"), g.get("bias"), gy if need[3] else None, None
-
-
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+        want = need[0] + 2 * need[1] + 4 * need[2]
+        grads = _abi.dense().linear_backward(x, weight, gy, tape, ctx.code, want) if want else (None, None, None)
+        return (*grads, gy if need[3] else None, None)
 
 
 def fused_linear(x, weight, bias=None, *, activation="none", residual=None) -> torch.Tensor:
@@ -668,27 +564,10 @@ def fused_linear(x, weight, bias=None, *, activation="none", residual=None) -> t
     projection of a pre-norm block, without one the projections of the reference's ``FusedHQKAN``
     (``src/qkan/solver/cute/cute_ops.py:449-490``).
     """
+    code = _activation_code(activation)
     if _wants_grad(x, weight, bias, residual):
-        return _LinearFunction.apply(x, weight, bias, residual, activation)
-    return linear_forward(x, weight, bias, activation=activation, residual=residual)
-
-
-def _norm_shape(x: torch.Tensor, weight, bias, param_dtype=None):
-    """(io code, rows, D, code and dtype of the parameters), checked."""
-    io = _dense_io(x)
-    rows = _rows_of(x.shape)
-    D = x.shape[-1]
-    if D < 1:
-        raise ValueError("layer_norm needs at least one element per row")
-    pdt = weight.dtype if weight is not None else bias.dtype if bias is not None else param_dtype or x.dtype
-    code = _DENSE_IO.get(pdt)
-    if code is None:
-        raise TypeError(f"layer_norm parameters are float32 or bfloat16, got {pdt}")
-    if weight is not None:
-        _check_like(weight, "weight", (D,), pdt, x.device)
-    if bias is not None:
-        _check_like(bias, "bias", (D,), pdt, x.device)
-    return io, rows, D, code, pdt
+        return _LinearFunction.apply(x, weight, bias, residual, code)
+    return _abi.dense().linear_forward(x, weight, bias, residual, code, False)[0]
 
 
 def layer_norm_forward(x, weight=None, bias=None, *, eps: float = 1e-5, return_stats: bool = True):
@@ -697,17 +576,7 @@ def layer_norm_forward(x, weight=None, bias=None, *, eps: float = 1e-5, return_s
     ``weight`` and ``bias`` ``(D,)`` are float32 or bfloat16, whatever ``x`` is, and share one dtype. ``stats (..., 2)``
     float32 holds each row's mean and ``1 / sqrt(var + eps)`` for ``layer_norm_backward`` (None without ``return_stats``).
     """
-    lib = _abi.load()
-    io, rows, D, pcode, _ = _norm_shape(x, weight, bias)
-    if not 0.0 <= eps < math.inf:
-        raise ValueError(f"eps must be finite and >= 0, got {eps}")
-    dev = x.device
-    x, weight, bias = _packed(x), _packed(weight), _packed(bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = torch.empty((*x.shape[:-1], 2), dtype=torch.float32, device=dev) if return_stats else None
-    _call(dev, lib.qk_layer_norm_forward, "qk_layer_norm_forward", byref(_abi.QkNormDesc(rows, D, io, pcode, eps, 0)),
-          x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(stats))
-    return y, stats
+    return _abi.dense().norm_forward(x, weight, bias, eps, return_stats)
 
 
 def layer_norm_backward(x, weight, stats, gy, *, want=_GRADS, param_dtype=None) -> dict:
@@ -716,27 +585,13 @@ def layer_norm_backward(x, weight, stats, gy, *, want=_GRADS, param_dtype=None) 
     ``weight`` None stands for ones; the parameters' gradients have the weight's dtype, or ``param_dtype`` where there is
     no weight (default: that of ``x``).
     """
-    lib = _abi.load()
-    io, rows, D, pcode, pdt = _norm_shape(x, weight, None, param_dtype)
-    dev = x.device
-    _check_want(want)
-    _check_like(gy, "gy", x.shape, x.dtype, dev)
-    _check_like(stats, "stats", (*x.shape[:-1], 2), torch.float32, dev)
-    x, gy, stats, weight = _packed(x), _packed(gy), _packed(stats), _packed(weight)
-    out = {}
-    for name in want:
-        out[name] = torch.empty(x.shape if name == "x" else (D,), dtype=x.dtype if name == "x" else pdt, device=dev)
-    desc = byref(_abi.QkNormDesc(rows, D, io, pcode, 0.0, 0))
-    ws, ws_at, nbytes = _scratch(dev, lib.qk_layer_norm_backward_workspace_bytes(desc), "qk_layer_norm_backward_workspace_bytes")
-    _call(dev, lib.qk_layer_norm_backward, "qk_layer_norm_backward", desc, x.data_ptr(), _ptr(weight), stats.data_ptr(),
-          gy.data_ptr(), _ptr(out.get("x")), _ptr(out.get("weight")), _ptr(out.get("bias")), ws_at, nbytes)
-    return out
+    return _named(_abi.dense().norm_backward(x, weight, stats, gy, _want_bits(want), param_dtype), want)
 
 
 class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, stats = layer_norm_forward(x, weight, bias, eps=eps)
+        y, stats = _abi.dense().norm_forward(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, stats)
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
@@ -746,13 +601,11 @@ class _LayerNormFunction(torch.autograd.Function):
     def backward(ctx, gy):
         x, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        want = tuple(n for n, wanted in zip(_GRADS, need) if wanted)
-        g = layer_norm_backward(x, weight, stats, gy, want=want, param_dtype=ctx.bias_dtype)
-        return g.get("x"), g.get("weight"), g.get("bias"), None
+        return (*_abi.dense().norm_backward(x, weight, stats, gy, need[0] + 2 * need[1] + 4 * need[2], ctx.bias_dtype), None)
 
 
 def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5) -> torch.Tensor:
     """Differentiable layer norm over the last axis (``layer_norm_forward`` / ``layer_norm_backward``)."""
     if _wants_grad(x, weight, bias):
         return _LayerNormFunction.apply(x, weight, bias, eps)
-    return layer_norm_forward(x, weight, bias, eps=eps, return_stats=False)[0]
+    return _abi.dense().norm_forward(x, weight, bias, eps, False)[0]

@@ -3,7 +3,8 @@
 Bounds count roundings. A float32 sum of n products in any order is off by at most ``(n + 16) 2^-24`` of the sum of the
 products' magnitudes (16: the rounded operands' missing part, the epilogue). A value rounded to bfloat16 is off by at
 most 2^-8 of itself, the half-precision tape by 2^-11. CUDA's float32 exp, erf and tanh and the few operations around
-them are within 16 float32 steps.
+them are within 16 float32 steps; exp(z) of the special-function unit, which bfloat16 results are made of, is within
+2^-21 + 1.5 |z| 2^-24 of itself, 64 steps with what surrounds it for |z| < 32.
 """
 import math
 
@@ -48,7 +49,7 @@ def linear64(x, w, b=None, r=None, act="none"):
         z, mag = z + b.double(), mag + b.double().abs()
     zb = (K + 16) * U32 * mag
     y, _ = act64(z, act)
-    yb = zb * STEEP + 16 * U32 * (y.abs() + z.abs() + 1e-30)
+    yb = zb * STEEP + (64 if half else 16) * U32 * (y.abs() + z.abs() + 1e-30)
     if r is not None:
         y = y + r.double()
         yb = yb + U32 * y.abs()
@@ -67,7 +68,7 @@ def linear64_grads(x, w, b, gy, act="none"):
     gz = gy * slope
     gzb = torch.zeros_like(gz)
     if act != "none":
-        gzb = gy.abs() * (BEND * (zb + (UTAPE * z.abs() + 2.0 ** -24 if half else 0)) + 16 * U32 * (slope.abs() + 1))
+        gzb = gy.abs() * (BEND * (zb + (UTAPE * z.abs() + 2.0 ** -24 if half else 0)) + (64 if half else 16) * U32 * (slope.abs() + 1))
     sumb = gzb  # what the bias gradient adds: not rounded to bfloat16 on the way
     if half and act != "none":
         gzb = gzb + U16 * (gz.abs() + gzb)
