@@ -1,14 +1,16 @@
 // Matrix products of the linear map on the tensor cores (tcgen05): C[r,c] = sum_k P[r,k] Q[c,k] with the epilogue
 // act(C + bias[c]) + residual[r,c].
 //
-// The MMA's M side (the 128 lanes of tensor memory) is Q's side, so a thread of the epilogue owns one column c and its
-// warp 32 neighbouring ones: bias sits in a register, and residual, output and tape are read and written along rows
-// without a detour through shared memory, whatever the width or alignment of a row.
+// One CTA per SM walks units of work (a tile of 128 rows and BN columns, a slice of the depth). Warp 0 copies 64-deep
+// blocks of both operands into a ring of stages (TMA, 128-byte swizzle), warp 1 issues the MMAs, eight warps drain the
+// sums from one of two accumulators in tensor memory while the other one is filled. An operand is read as it lies in
+// memory: "K-major" when the summed axis is contiguous (forward: x and W), "MN-major" when it is the other axis (W in
+// grad_x, x and gz in grad_weight).
 //
-// One CTA per SM walks units of work (tile, slice of the depth). Warp 0 copies 64-deep blocks of both operands into a
-// ring of stages (TMA, 128-byte swizzle), warp 1 issues the MMAs, eight warps drain the sums from one of two
-// accumulators while the other one is filled. An operand is read as it lies in memory: "K-major" when the summed axis is
-// contiguous (forward: x and W), "MN-major" when it is the other axis (W in grad_x, x and gz in grad_weight).
+// A lane of tensor memory is a row of C, so a thread of the epilogue has one row and reads the residual along it. Results
+// go through 64-byte rows in shared memory, from where TMA stores them (rows of whole 16-byte words) or the warp does,
+// row by row. Stored straight from the registers, two bytes per lane and row, a 64 x 128 tile took 1.4 us; that was the
+// whole time of a product with a short depth.
 //
 // float32 (PLANES == 3): x = h + m + l exactly, each part a bfloat16 (8 significant bits, float32's exponents). Six of
 // the nine products are kept: hh | hm mh hl lh mm; what is dropped is below 2^-22 of |x||w|. hh goes to one accumulator
@@ -23,24 +25,26 @@ namespace qk {
 namespace {
 
 constexpr int kBK = 64;             // depth of a stage: 128 bytes of bfloat16, one swizzle row
-constexpr int kTileC = 128;         // the MMA's M
+constexpr int kTileR = 128;         // the MMA's M
 constexpr int kChunk = 2;           // stages between two drains of hh (float32)
 constexpr int kGemmThreads = 320;   // producer, MMA issuer, 8 epilogue warps
 constexpr int kDrainWarps = 8;
 constexpr unsigned long long kGiveUpNs = 10ull * 1000 * 1000 * 1000;  // the longest that a wait may take
 
+constexpr int kStoreBytes = 2048;   // 32 rows of 64 bytes: what a warp stages for one store; two of them per warp
+
 template <int BN, int PLANES>
 struct Shape {
-    static constexpr int kABytes = kTileC * 128;
-    static constexpr int kBBytes = (BN < 64 ? 64 : BN) * 128;  // an MN-major box is 64 wide at least
+    static constexpr int kABytes = kTileR * 128;
+    static constexpr int kBBytes = BN * 128;
     static constexpr int kStageBytes = PLANES * (kABytes + kBBytes);
-    static constexpr int kStagesFit = (196 * 1024) / kStageBytes;
+    static constexpr int kStagingBytes = kDrainWarps * 2 * kStoreBytes;
+    static constexpr int kStagesFit = (225 * 1024 - kStagingBytes) / kStageBytes;
     static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
     static constexpr int kAccCols = 2 * BN;
-    static constexpr int kColsWanted = PLANES == 3 ? 2 * kAccCols : kAccCols;
-    static constexpr int kTmemCols = kColsWanted < 32 ? 32 : kColsWanted;
-    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024 + 256;
-    static_assert(kStages >= 2 && kTmemCols <= 512 && kSmem <= kSmemCap, "does not fit an SM");
+    static constexpr int kTmemCols = PLANES == 3 ? 2 * kAccCols : kAccCols;
+    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kStagingBytes + 1024 + 256;
+    static_assert(kStages >= 2 && kTmemCols <= 512 && kSmem <= 227 * 1024, "does not fit an SM");
 };
 
 struct Barriers {
@@ -105,6 +109,11 @@ __device__ __forceinline__ void tma_load(const CUtensorMap* map, unsigned dst, u
         ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, unsigned src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(src),
+                 "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
 __device__ __forceinline__ void mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, bool add) {
     asm volatile(
         "{\n.reg .pred p;\n"
@@ -154,56 +163,133 @@ __device__ __forceinline__ unsigned long long smem_desc(unsigned addr, bool mn) 
 
 // One unit of work: a tile of C and a slice of the depth.
 struct Unit {
-    int r0, c0, kb0, kbs, split;  // first row in tiles, first column, first block and number of blocks of the slice
+    int r0, c0, kb0, kbs, split;  // first row and column, first block and number of blocks of the slice
 };
+template <int BN>
 __device__ __forceinline__ Unit unit_at(const GemmProblem& g, int u) {
     Unit t;
     const int tiles = g.tiles_r * g.tiles_c;
     t.split = u / tiles;
     u -= t.split * tiles;
     t.r0 = u / g.tiles_c;  // columns run fastest, so that neighbouring CTAs share P
-    t.c0 = (u - t.r0 * g.tiles_c) * kTileC;
+    t.c0 = (u - t.r0 * g.tiles_c) * BN;
+    t.r0 *= kTileR;
     t.kb0 = t.split * g.kper;
     t.kbs = min(g.kper, g.kblocks - t.kb0);
     return t;
 }
 
-// The residual of column c, rows r .. r + N - 1, fetched before the sums are waited for. Row and column are held inside
-// the matrix, so that every load is good by itself; what lies behind its edge is never stored.
+// N values of a row of IO elements from column c on. Row and column are held inside the matrix, so that every load is good
+// by itself, whether or not its value is wanted; what lies behind the edge is never stored.
 template <typename IO, int N>
-__device__ __forceinline__ void load_residual(const GemmProblem& g, long r, int c, float (&q)[N]) {
-    const long first = min(r, g.rows - 1L);
-    const int last = (int)min(N - 1L, g.rows - 1 - first);
-    const IO* res = static_cast<const IO*>(g.residual) + (size_t)first * g.cols + min(c, g.cols - 1);
+__device__ __forceinline__ void load_row(const void* base, size_t row, int c, int cols, bool vec, float (&v)[N]) {
+    const IO* p = static_cast<const IO*>(base) + row * cols;
+    if (vec && c + N <= cols) {
+        const uint4* q = reinterpret_cast<const uint4*>(p + c);
 #pragma unroll
-    for (int i = 0; i < N; ++i) q[i] = as_float(res[(size_t)min(i, last) * g.cols]);
+        for (int i = 0; i < N * (int)sizeof(IO) / 16; ++i) {
+            const uint4 w = q[i];
+            const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (sizeof(IO) == 4) {
+                    v[4 * i + k] = __uint_as_float(u[k]);
+                } else {
+                    v[8 * i + 2 * k] = __uint_as_float(u[k] << 16);
+                    v[8 * i + 2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = as_float(p[min(c + i, cols - 1)]);
+    }
 }
 
-// N sums of column c, rows r .. r + N - 1, of which n exist (none for a lane behind the last column: the warp stays
-// together, since it has to be whole when it reads tensor memory again).
-template <typename IO, int N>
-__device__ __forceinline__ void write_out(const GemmProblem& g, int split, long r, int c, int n, float bias,
-                                          const float (&q)[N], float (&v)[N]) {
-    const size_t cols = g.cols, at = (size_t)r * cols + c;
-    if (g.part) {
-        float* out = g.part + (size_t)split * g.rows * cols + at;
+// 64 bytes of this lane's row as words; T: float, __nv_bfloat16, or __half for the tape
+template <typename T, int N>
+__device__ __forceinline__ void pack_row(const float (&v)[N], unsigned (&u)[16]) {
+    static_assert(N * sizeof(T) == 64, "a staged row");
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i < n) out[i * cols] = v[i];
-        return;
+    for (int i = 0; i < 16; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            u[i] = __float_as_uint(v[i]);
+        } else if constexpr (std::is_same_v<T, __half>) {
+            u[i] = (unsigned)__half_as_ushort(tape_half(v[2 * i])) | (unsigned)__half_as_ushort(tape_half(v[2 * i + 1])) << 16;
+        } else {
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+        }
     }
+}
+
+// A warp's way from its registers to 32 rows of a matrix in global memory: two 2 KB pieces of shared memory in turn, rows
+// of 64 bytes, 16-byte words swizzled by the row (the 64-byte swizzle of a tensor map), so that lanes meet no bank twice.
+struct Store {
+    char* buf;
+    unsigned flip;
+    __device__ __forceinline__ char* next() {
+        // all but the latest store have been read out of shared memory: the piece of the one before that is free
+        if (threadIdx.x % 32 == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        __syncwarp();
+        char* b = buf + flip * kStoreBytes;
+        flip ^= 1;
+        return b;
+    }
+    // N elements per lane, rows r .. r + 31, columns c .. c + N - 1 of slice z; `size` rows by `cols`
+    template <typename T, int N>
+    __device__ __forceinline__ void operator()(const CUtensorMap* map, void* out, bool tma, const float (&v)[N], long r,
+                                               int c, int z, int rows, int cols) {
+        const int lane = threadIdx.x % 32;
+        char* b = next();
+        unsigned u[16];
+        pack_row<T>(v, u);
+        uint4* row = reinterpret_cast<uint4*>(b + lane * 64);
+        const int x = lane >> 1 & 3;
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += bias;
+        for (int i = 0; i < 4; ++i) row[i ^ x] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+        if (tma) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                if (r < rows && c < cols) tma_store(map, smem_u32(b), c, (int)r, z);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+        } else {
+            __syncwarp();
+            T* at = static_cast<T*>(out) + (size_t)z * rows * cols;
+            constexpr int kRows = 32 / N;  // rows of one pass of the warp
+            const int j = lane % N;
+#pragma unroll 8
+            for (int i = lane / N; i < 32; i += kRows) {
+                const T e = *reinterpret_cast<const T*>(b + i * 64 + ((j * (int)sizeof(T) / 16) ^ (i >> 1 & 3)) * 16 +
+                                                        j * (int)sizeof(T) % 16);
+                if (r + i < rows && c + j < cols) at[(size_t)(r + i) * cols + c + j] = e;
+            }
+            __syncwarp();
+        }
+    }
+};
+
+// The epilogue of one piece: N sums per lane, which has row r + lane, from column c on; q: its residual.
+template <typename IO, int N>
+__device__ __forceinline__ void write_out(const GemmProblem& g, Store& store, long r, int c, const float (&q)[N],
+                                          float (&v)[N]) {
+    float b[N];
+    load_row<IO, N>(g.bias, 0, min(c, g.cols - 1), g.cols, g.vec, b);
+    if (g.has_bias) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += b[i];
+    }
     if (g.tape) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i < n) store_tape(g.tape, at + i * cols, sizeof(IO) == 2 ? QK_BF16 : QK_F32, v[i]);
+        using T = std::conditional_t<sizeof(IO) == 2, __half, float>;
+        store.operator()<T>(&g.tape_map, g.tape, g.tma_out, v, r, c, 0, g.rows, g.cols);
     }
     activate_all<sizeof(IO) == 2>(v, g.act);
-    IO* out = static_cast<IO*>(g.out) + at;
+    if (g.has_residual) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (i < n) out[i * cols] = from_float<IO>(v[i] + q[i]);
+        for (int i = 0; i < N; ++i) v[i] += q[i];
+    }
+    store.operator()<IO>(&g.out_map, g.out, g.tma_out, v, r, c, 0, g.rows, g.cols);
 }
 
 template <int BN, int PLANES>
@@ -212,7 +298,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     using IO = std::conditional_t<PLANES == 3, float, __nv_bfloat16>;
     extern __shared__ char raw[];
     char* stages = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
-    Barriers& bars = *reinterpret_cast<Barriers*>(stages + (size_t)S::kStages * S::kStageBytes);
+    char* staging = stages + (size_t)S::kStages * S::kStageBytes;
+    Barriers& bars = *reinterpret_cast<Barriers*>(staging + S::kStagingBytes);
     static_assert(sizeof(Barriers) <= 256, "barriers");
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     volatile int* abort = &bars.abort;
@@ -242,31 +329,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             int stage = 0;
             unsigned phase = 0, issued = 0;
             bool ok = true;
+            const unsigned bytes = PLANES * (g.p_boxes * g.p_box_bytes + g.q_boxes * g.q_box_bytes);
             for (int u = blockIdx.x; ok && u < g.units; u += gridDim.x) {
-                const Unit t = unit_at(g, u);
-                const int r0 = t.r0 * BN;
-                const unsigned bytes = PLANES * (S::kABytes + (g.p_mn ? S::kBBytes : BN * 128));
+                const Unit t = unit_at<BN>(g, u);
                 for (int kb = t.kb0; kb < t.kb0 + t.kbs; ++kb) {
                     ok = bar_wait(&bars.empty[stage], phase ^ 1, abort);
                     if (!ok) break;
                     unsigned long long* bar = &bars.full[stage];
                     bar_expect(bar, bytes);
                     unsigned dst = smem_u32(stages) + stage * S::kStageBytes;
+                    // K-major: one box of a tile's rows. MN-major: boxes 64 wide, 8 KB each.
                     for (int p = 0; p < PLANES; ++p, dst += S::kABytes) {
-                        if (g.q_mn) {
-                            tma_load(&g.q_map, dst, bar, t.c0, kb * kBK, p);
-                            tma_load(&g.q_map, dst + 8192, bar, t.c0 + 64, kb * kBK, p);
-                        } else {
-                            tma_load(&g.q_map, dst, bar, kb * kBK, t.c0, p);
-                        }
+                        for (int b = 0; b < g.p_boxes; ++b)
+                            tma_load(&g.p_map, dst + b * 8192, bar, g.p_mn ? t.r0 + b * 64 : kb * kBK,
+                                     g.p_mn ? kb * kBK : t.r0, p);
                     }
                     for (int p = 0; p < PLANES; ++p, dst += S::kBBytes) {
-                        if (g.p_mn) {
-                            for (int b = 0; b < S::kBBytes / 8192; ++b)
-                                tma_load(&g.p_map, dst + b * 8192, bar, r0 + b * 64, kb * kBK, p);
-                        } else {
-                            tma_load(&g.p_map, dst, bar, kb * kBK, r0, p);
-                        }
+                        for (int b = 0; b < g.q_boxes; ++b)
+                            tma_load(&g.q_map, dst + b * 8192, bar, g.q_mn ? t.c0 + b * 64 : kb * kBK,
+                                     g.q_mn ? kb * kBK : t.c0, p);
                     }
                     ++issued;
                     if (++stage == S::kStages) stage = 0, phase ^= 1;
@@ -285,11 +366,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             int stage = 0, acc = 0, corr = 0;
             unsigned phase = 0, acc_phase = 0, corr_phase = 0;
             bool ok = true;
+            // D float32, A and B bfloat16, which of them MN-major, N / 8, M / 16
+            const unsigned idesc = 1u << 4 | 1u << 7 | 1u << 10 | (unsigned)g.p_mn << 15 | (unsigned)g.q_mn << 16 |
+                                   (BN / 8) << 17 | (kTileR / 16) << 24;
+            const unsigned a_step = g.p_mn ? 2048 >> 4 : 32 >> 4, b_step = g.q_mn ? 2048 >> 4 : 32 >> 4;
             for (int u = blockIdx.x; ok && u < g.units; u += gridDim.x) {
-                const Unit t = unit_at(g, u);
-                const unsigned idesc = 1u << 4 | 1u << 7 | 1u << 10 | (unsigned)g.q_mn << 15 | (unsigned)g.p_mn << 16 |
-                                       (BN / 8) << 17 | (kTileC / 16) << 24;
-                const unsigned a_step = g.q_mn ? 2048 >> 4 : 32 >> 4, b_step = g.p_mn ? 2048 >> 4 : 32 >> 4;
+                const Unit t = unit_at<BN>(g, u);
                 if (PLANES == 3) {
                     ok = bar_wait(&bars.corr_empty[corr], corr_phase ^ 1, abort);
                     if (!ok) break;
@@ -304,8 +386,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     if (!ok) break;
                     fence_after();
                     const unsigned base = smem_u32(stages) + stage * S::kStageBytes;
-                    const unsigned long long da = smem_desc(base, g.q_mn);
-                    const unsigned long long db = smem_desc(base + PLANES * S::kABytes, g.p_mn);
+                    const unsigned long long da = smem_desc(base, g.p_mn);
+                    const unsigned long long db = smem_desc(base + PLANES * S::kABytes, g.q_mn);
                     const unsigned d = tmem + acc * BN;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) mma(d, da + k * a_step, db + k * b_step, idesc, !(opens && k == 0));
@@ -341,45 +423,56 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             }
         }
     } else {
+        // a warp reads the 32 lanes of its number mod 4; two warps share them, half of the columns each
         const int quad = warp % 4, half = (warp - 2) / 4;
         const unsigned lanes = (unsigned)(quad * 32) << 16;
+        Store store{staging + (warp - 2) * 2 * kStoreBytes, 0};
         int acc = 0, corr = 0;
         unsigned acc_phase = 0, corr_phase = 0;
         bool ok = true;
         for (int u = blockIdx.x; ok && u < g.units; u += gridDim.x) {
-            const Unit t = unit_at(g, u);
-            const int c = t.c0 + quad * 32 + lane;
-            const long r0 = (long)t.r0 * BN + half * (BN / 2);
-            const bool live = c < g.cols;
-            float bias = as_float(static_cast<const IO*>(g.bias)[min(c, g.cols - 1)]);
-            if (!g.has_bias) bias = 0.f;
+            const Unit t = unit_at<BN>(g, u);
+            const int c0 = t.c0 + half * (BN / 2);
+            const long r0 = t.r0 + quad * 32;
+            const size_t row = (size_t)min(r0 + lane, g.rows - 1L);
             if constexpr (PLANES == 1) {
-                constexpr int N = BN / 2 < 32 ? BN / 2 : 32;
-#pragma unroll 1
-                for (int j = 0; j < BN / 2; j += N) {
-                    const int n = live ? (int)max(0L, min((long)N, g.rows - r0 - j)) : 0;
-                    float q[N], v[N];
-                    if (g.has_residual) {
-                        load_residual<IO, N>(g, r0 + j, c, q);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < N; ++i) q[i] = 0.f;
-                    }
-                    if (j == 0) {
-                        ok = bar_wait(&bars.acc_full[acc], acc_phase, abort);
-                        ok = __all_sync(~0u, ok);
-                        if (!ok) break;
-                        fence_after();
-                    }
-                    __syncwarp();
-                    tmem_load<N>(tmem + lanes + acc * BN + half * (BN / 2) + j, v);
-                    if (j + N == BN / 2) {
-                        fence_before();
-                        if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
-                    }
-                    write_out<IO, N>(g, t.split, r0 + j, c, n, bias, q, v);
-                }
+                constexpr int N = 32;
+                float q[N];
+                if (g.has_residual) load_row<IO, N>(g.residual, row, min(c0, g.cols - 1), g.cols, g.vec, q);
+                ok = bar_wait(&bars.acc_full[acc], acc_phase, abort);
+                ok = __all_sync(~0u, ok);
                 if (!ok) break;
+                fence_after();
+                const unsigned from = tmem + lanes + acc * BN + half * (BN / 2);
+                if (g.part) {
+#pragma unroll 1
+                    for (int j = 0; j < BN / 2; j += 16) {
+                        float v[16];
+                        __syncwarp();
+                        tmem_load<16>(from + j, v);
+                        if (j + 16 == BN / 2) {
+                            fence_before();
+                            if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
+                        }
+                        store.operator()<float>(&g.out_map, g.part, g.tma_out, v, r0, c0 + j, t.split, g.rows, g.cols);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int j = 0; j < BN / 2; j += N) {
+                        float v[N], next[N];
+                        __syncwarp();
+                        tmem_load<N>(from + j, v);
+                        if (j + N == BN / 2) {
+                            fence_before();
+                            if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
+                        } else if (g.has_residual) {
+                            load_row<IO, N>(g.residual, row, min(c0 + j + N, g.cols - 1), g.cols, g.vec, next);
+                        }
+                        write_out<IO, N>(g, store, r0, c0 + j, q, v);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) q[i] = next[i];
+                    }
+                }
                 if (++acc == 2) acc = 0, acc_phase ^= 1;
             } else {
                 float sum[BN / 2];
@@ -409,14 +502,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 fence_after();
 #pragma unroll
                 for (int j = 0; j < BN / 2; j += 16) {
-                    const int n = live ? (int)max(0L, min(16L, g.rows - r0 - j)) : 0;
                     float q[16], v[16];
-                    if (g.has_residual) {
-                        load_residual<IO, 16>(g, r0 + j, c, q);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) q[i] = 0.f;
-                    }
+                    if (g.has_residual) load_row<IO, 16>(g.residual, row, min(c0 + j, g.cols - 1), g.cols, g.vec, q);
                     __syncwarp();
                     tmem_load<16>(corr_base + lanes + corr * BN + half * (BN / 2) + j, v);
                     if (j + 16 == BN / 2) {
@@ -426,11 +513,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) v[i] = isfinite(sum[j + i]) ? sum[j + i] + v[i] : sum[j + i];
-                    write_out<IO, 16>(g, t.split, r0 + j, c, n, bias, q, v);
+                    if (g.part)
+                        store.operator()<float>(&g.out_map, g.part, g.tma_out, v, r0, c0 + j, t.split, g.rows, g.cols);
+                    else
+                        write_out<IO, 16>(g, store, r0, c0 + j, q, v);
                 }
                 if (++corr == 2) corr = 0, corr_phase ^= 1;
             }
         }
+        // shared memory is given up once every store has read its piece
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     }
     __syncwarp();
     fence_before();
@@ -457,25 +549,37 @@ EncodeFn encode_fn() {
     return fn;
 }
 
-// `inner` contiguous elements per row, `outer` rows `ld` elements apart, `planes` of them; boxes of 64 x box_outer
-bool make_map(CUtensorMap* map, const void* base, long inner, long outer, long ld, int planes, int box_outer) {
+// `inner` contiguous elements of `el` bytes per row, `outer` rows `ld` elements apart, `planes` of them
+bool make_map(CUtensorMap* map, const void* base, int el, long inner, long outer, long ld, int planes, int box_inner,
+              int box_outer, CUtensorMapSwizzle swizzle) {
     const EncodeFn fn = encode_fn();
     if (!fn) return false;
     const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)planes};
-    const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)ld * outer * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)box_outer, 1}, step[3] = {1, 1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint64_t strides[2] = {(cuuint64_t)ld * el, (cuuint64_t)ld * outer * el};
+    const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer, 1}, step[3] = {1, 1, 1};
+    return fn(map, el == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+              const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// boxes that a stage takes of an operand whose tile has `tile` rows, of which `rows` exist at most: no more than there is
+// (what is left of the tile in shared memory is whatever was there; it reaches only rows of C that do not exist)
+bool bind_operand(CUtensorMap* map, const Operand& o, int planes, int tile, int rows, int* boxes, int* box_bytes) {
+    const int need = rows < tile ? (rows + 7) / 8 * 8 : tile;
+    *boxes = o.mn_major ? (need + 63) / 64 : 1;
+    const int outer = o.mn_major ? kBK : need;
+    *box_bytes = outer * 128;
+    return make_map(map, o.base, 2, o.inner, o.outer, o.ld, planes, 64, outer, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int BN, int PLANES>
 cudaError_t launch_shape(const GemmProblem& g, cudaStream_t st) {
+    using S = Shape<BN, PLANES>;
     static unsigned long long opted = 0;
-    cudaError_t e = opt_in_smem(gemm_kernel<BN, PLANES>, &opted);
+    cudaError_t e = opt_in_smem(gemm_kernel<BN, PLANES>, &opted, (int)S::kSmem);
     if (e != cudaSuccess) return e;
     const int grid = g.units < kSms ? g.units : kSms;
-    gemm_kernel<BN, PLANES><<<grid, kGemmThreads, Shape<BN, PLANES>::kSmem, st>>>(g);
+    gemm_kernel<BN, PLANES><<<grid, kGemmThreads, S::kSmem, st>>>(g);
     return cudaPeekAtLastError();
 }
 
@@ -484,20 +588,25 @@ cudaError_t launch_shape(const GemmProblem& g, cudaStream_t st) {
 bool gemm_bind(GemmProblem& g, const Operand& p, const Operand& q, int planes, int bn) {
     g.p_mn = p.mn_major;
     g.q_mn = q.mn_major;
-    return make_map(&g.p_map, p.base, p.inner, p.outer, p.ld, planes, p.mn_major ? kBK : bn) &&
-           make_map(&g.q_map, q.base, q.inner, q.outer, q.ld, planes, q.mn_major ? kBK : kTileC);
+    if (!bind_operand(&g.p_map, p, planes, kTileR, g.rows, &g.p_boxes, &g.p_box_bytes) ||
+        !bind_operand(&g.q_map, q, planes, bn, g.cols, &g.q_boxes, &g.q_box_bytes))
+        return false;
+    const int el = planes == 3 ? 4 : 2, out_el = g.part ? 4 : el;
+    auto words = [](const void* p) { return (uintptr_t)p % 16 == 0; };
+    g.vec = (long)g.cols * el % 16 == 0 && words(g.bias) && words(g.residual);
+    void* out = g.part ? static_cast<void*>(g.part) : g.out;
+    g.tma_out = (long)g.cols * out_el % 16 == 0 && words(out) && (!g.tape || words(g.tape));
+    if (!g.tma_out) return true;
+    if (!make_map(&g.out_map, out, out_el, g.cols, g.rows, g.cols, g.part ? g.splits : 1, 64 / out_el, 32,
+                  CU_TENSOR_MAP_SWIZZLE_64B))
+        return false;
+    return !g.tape || make_map(&g.tape_map, g.tape, el, g.cols, g.rows, g.cols, 1, 64 / el, 32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-cudaError_t launch_gemm(const GemmProblem& a, int planes, int bn, cudaStream_t st) {
-    if (planes == 3) {
-        if (bn == 128) return launch_shape<128, 3>(a, st);
-        if (bn == 64) return launch_shape<64, 3>(a, st);
-        return launch_shape<32, 3>(a, st);
-    }
-    if (bn == 256) return launch_shape<256, 1>(a, st);
-    if (bn == 128) return launch_shape<128, 1>(a, st);
-    if (bn == 64) return launch_shape<64, 1>(a, st);
-    return launch_shape<32, 1>(a, st);
+cudaError_t launch_gemm(const GemmProblem& g, int planes, int bn, cudaStream_t st) {
+    if (planes == 3) return bn == 128 ? launch_shape<128, 3>(g, st) : launch_shape<64, 3>(g, st);
+    if (bn == 256) return launch_shape<256, 1>(g, st);
+    return bn == 128 ? launch_shape<128, 1>(g, st) : launch_shape<64, 1>(g, st);
 }
 
 cudaError_t gemm_gave_up(unsigned* count, cudaStream_t st) {

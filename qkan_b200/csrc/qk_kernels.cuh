@@ -127,18 +127,18 @@ void debug_set(int key, int value);
 
 // Largest dynamic shared memory any tile chooser hands out; each kernel instantiation is opted in to it once per device.
 constexpr int kSmemCap = 200 * 1024;
-// Opts `kern` in to kSmemCap bytes of dynamic shared memory on the current device, once: `mask` is that
+// Opts `kern` in to `bytes` of dynamic shared memory on the current device, once: `mask` is that
 // instantiation's own set of devices already done. The attribute is set before the bit, so a second host thread
 // either sees the bit (attribute in place) or sets the same value again. A cudaDeviceReset() forgets the attribute
 // but not the bit: a process that resets a device must not call the library on it afterwards.
 template <typename K>
-inline cudaError_t opt_in_smem(K kern, unsigned long long* mask) {
+inline cudaError_t opt_in_smem(K kern, unsigned long long* mask, int bytes = kSmemCap) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const unsigned long long bit = 1ull << (dev & 63);
     if (__atomic_load_n(mask, __ATOMIC_ACQUIRE) & bit) return cudaSuccess;
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemCap);
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e == cudaSuccess) __atomic_fetch_or(mask, bit, __ATOMIC_RELEASE);
     return e;
 }

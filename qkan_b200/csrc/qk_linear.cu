@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) reduce_kernel(const ReduceArgs a) {
 
 // ---- choice of tiles -----------------------------------------------------------
 // Clocks of one SM, from the rates of its parts: the tensor core takes 2 BN clocks for a 128 x BN x 64 block, six times
-// that in float32; L2 feeds some 56 bytes per clock; the epilogue writes about one row of 128 columns per 12 clocks.
+// that in float32; L2 feeds some 56 bytes per clock; the epilogue takes about 12 clocks per column.
 struct Cut {
     int splits, kper;
 };
@@ -184,14 +184,15 @@ struct Cut {
 struct Size {
     long rows, cols;
     int kblocks;
-    long tiles(int bn) const { return (rows + bn - 1) / bn * ((cols + 127) / 128); }
+    long tiles(int bn) const { return (rows + 127) / 128 * ((cols + bn - 1) / bn); }
 };
 
-double block_clocks(int bn, int planes) {
-    const double mma = 2.0 * bn * (planes == 3 ? 6 : 1), load = planes * (16384.0 + (bn < 64 ? 64 : bn) * 128) / 56;
+double block_clocks(const Size& s, int bn, int planes) {
+    const double mma = 2.0 * bn * (planes == 3 ? 6 : 1);
+    const double rows = (s.rows < 128 ? s.rows : 128) + (s.cols < bn ? s.cols : bn), load = planes * rows * 128 / 56 + 100;
     return mma > load ? mma : load;
 }
-double drain_clocks(int bn) { return 12.0 * bn + 200; }
+double drain_clocks(int bn) { return 12.0 * bn + 500; }
 
 Cut cut_into(int kblocks, int splits) {
     Cut c;
@@ -210,7 +211,7 @@ struct Plan {
 
 double cost_of(const Size& s, int bn, int planes, const Cut& c) {
     const long units = s.tiles(bn) * c.splits;
-    const double mainloop = c.kper * block_clocks(bn, planes), drain = drain_clocks(bn);
+    const double mainloop = c.kper * block_clocks(s, bn, planes), drain = drain_clocks(bn);
     double t = (double)((units + kSms - 1) / kSms) * (mainloop > drain ? mainloop : drain) + drain + 2500;
     if (c.splits > 1) t += 3500 + 2.0 * c.splits * s.rows * s.cols * 4 / (kSms * 24.0);
     return t;
@@ -219,7 +220,7 @@ double cost_of(const Size& s, int bn, int planes, const Cut& c) {
 Plan plan_for(const Size& s, int planes) {
     Plan best{};
     double least = 1e300;
-    for (int bn = planes == 3 ? 128 : 256; bn >= 32; bn /= 2)
+    for (int bn = planes == 3 ? 128 : 256; bn >= 64; bn /= 2)
         for (int k : kCuts) {
             if (k > 1 && (k > s.kblocks || s.tiles(bn) * k > 4l * kSms || (double)k * s.rows * s.cols > kMostPart)) break;
             const Cut c = cut_into(s.kblocks, k);
@@ -371,7 +372,7 @@ cudaError_t run_product(int rows, int cols, int depth, const Plan& plan, const O
     GemmProblem g{};
     g.rows = rows, g.cols = cols;
     g.kblocks = blocks_of(depth), g.kper = plan.cut.kper, g.splits = plan.cut.splits;
-    g.tiles_r = (rows + plan.bn - 1) / plan.bn, g.tiles_c = (cols + 127) / 128;
+    g.tiles_r = (rows + 127) / 128, g.tiles_c = (cols + plan.bn - 1) / plan.bn;
     const long units = (long)g.tiles_r * g.tiles_c * g.splits;
     if (units > 0x3fffffff) return cudaErrorInvalidConfiguration;
     g.units = (int)units;

@@ -18,11 +18,14 @@ struct Operand {
 };
 
 struct alignas(64) GemmProblem {
-    CUtensorMap p_map, q_map;
+    CUtensorMap p_map, q_map, out_map, tape_map;  // out_map: of `part` where there is one
     int rows, cols;
     int kblocks, kper, splits;  // 64-deep blocks in all, per slice of the depth, slices
     int tiles_r, tiles_c, units;
     bool p_mn, q_mn;
+    int p_boxes, q_boxes, p_box_bytes, q_box_bytes;  // what one stage takes of each operand (and part)
+    bool vec;      // bias and residual can be read in 16-byte words
+    bool tma_out;  // out (part) and tape can be written by TMA
     float* part;  // splits > 1: [splits][rows][cols] sums, no epilogue; nullptr otherwise
     // The epilogue, as in Epilogue. What it lacks points to `out`, so that a load of either is good whether or not it is
     // wanted: where a null pointer stood behind a test, hoisting the load over the test made it a fault.
@@ -34,7 +37,7 @@ struct alignas(64) GemmProblem {
     int act;
 };
 
-// fills in the operands' tensor maps; false: the driver refused one
+// fills in the tensor maps and what goes with them; false: the driver refused one
 bool gemm_bind(GemmProblem& g, const Operand& p, const Operand& q, int planes, int bn);
 cudaError_t launch_gemm(const GemmProblem& g, int planes, int bn, cudaStream_t st);
 // waits that ran out on the current device since the last call; synchronises the stream
