@@ -1,9 +1,10 @@
 // Matrix products of the linear map on the tensor cores (tcgen05): C[r,c] = sum_k P[r,k] Q[c,k] with the epilogue
 // act(C + bias[c]) + residual[r,c].
 //
-// One CTA per SM walks units of work (a tile of 128 rows and BN columns, a slice of the depth). Warp 0 copies 64-deep
-// blocks of both operands into a ring of stages (TMA, 128-byte swizzle), warp 1 issues the MMAs, eight warps drain the
-// sums from one of two accumulators in tensor memory while the other one is filled. An operand is read as it lies in
+// One CTA per SM walks units of work (a tile of 128 rows and BN columns, a slice of the depth). Two warps copy 64-deep
+// blocks of the operands, one each, into a ring of stages (TMA, 128-byte swizzle; one thread for both, at 140 clocks a
+// copy, was slower than the MMAs of narrow tiles), warp 1 issues the MMAs, eight warps drain the sums from one of two
+// accumulators in tensor memory while the other one is filled. An operand is read as it lies in
 // memory: "K-major" when the summed axis is contiguous (forward: x and W), "MN-major" when it is the other axis (W in
 // grad_x, x and gz in grad_weight).
 //
@@ -27,8 +28,9 @@ namespace {
 constexpr int kBK = 64;             // depth of a stage: 128 bytes of bfloat16, one swizzle row
 constexpr int kTileR = 128;         // the MMA's M
 constexpr int kChunk = 2;           // stages between two drains of hh (float32)
-constexpr int kGemmThreads = 320;   // producer, MMA issuer, 8 epilogue warps
+constexpr int kGemmThreads = 352;   // copies of P, MMAs, 8 epilogue warps, copies of Q
 constexpr int kDrainWarps = 8;
+constexpr int kQWarp = 10;
 constexpr unsigned long long kGiveUpNs = 10ull * 1000 * 1000 * 1000;  // the longest that a wait may take
 
 constexpr int kStoreBytes = 2048;   // 32 rows of 64 bytes: what a warp stages for one store; two of them per warp
@@ -78,6 +80,17 @@ __device__ __forceinline__ bool bar_try(unsigned long long* b, unsigned parity) 
         : "r"(smem_u32(b)), "r"(parity)
         : "memory");
     return done != 0;
+}
+// One lane of a whole warp. The compiler knows what this instruction chooses: what stands behind it is issued once, its
+// operands in uniform registers. Behind "lane == 0" a copy took 150 clocks to issue and an MMA 72.
+__device__ __forceinline__ bool elect_one() {
+    unsigned chosen;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "elect.sync _|p, 0xffffffff;\n"
+        "selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(chosen));
+    return chosen != 0;
 }
 __device__ __forceinline__ unsigned long long now_ns() {
     unsigned long long t;
@@ -161,21 +174,36 @@ __device__ __forceinline__ unsigned long long smem_desc(unsigned addr, bool mn) 
     return (unsigned long long)((addr & 0x3ffff) >> 4) | lead << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
 }
 
+// The fields of the problem that the loops use, in registers. Read from the parameter itself they are fetched again after
+// every asm statement, since its address is taken for the tensor maps: the producer's loop took 320 ns per block that way.
+struct Fields {
+    int rows, cols, tiles, tiles_c, kper, kblocks, units, act;
+    bool has_bias, has_residual, vec, tma_out;
+    const void* bias;
+    const void* residual;
+    void* out;
+    void* tape;
+    float* part;
+    __device__ __forceinline__ explicit Fields(const GemmProblem& g)
+        : rows(g.rows), cols(g.cols), tiles(g.tiles_r * g.tiles_c), tiles_c(g.tiles_c), kper(g.kper), kblocks(g.kblocks),
+          units(g.units), act(g.act), has_bias(g.has_bias), has_residual(g.has_residual), vec(g.vec), tma_out(g.tma_out),
+          bias(g.bias), residual(g.residual), out(g.out), tape(g.tape), part(g.part) {}
+};
+
 // One unit of work: a tile of C and a slice of the depth.
 struct Unit {
     int r0, c0, kb0, kbs, split;  // first row and column, first block and number of blocks of the slice
 };
 template <int BN>
-__device__ __forceinline__ Unit unit_at(const GemmProblem& g, int u) {
+__device__ __forceinline__ Unit unit_at(const Fields& f, int u) {
     Unit t;
-    const int tiles = g.tiles_r * g.tiles_c;
-    t.split = u / tiles;
-    u -= t.split * tiles;
-    t.r0 = u / g.tiles_c;  // columns run fastest, so that neighbouring CTAs share P
-    t.c0 = (u - t.r0 * g.tiles_c) * BN;
+    t.split = u / f.tiles;
+    u -= t.split * f.tiles;
+    t.r0 = u / f.tiles_c;  // columns run fastest, so that neighbouring CTAs share P
+    t.c0 = (u - t.r0 * f.tiles_c) * BN;
     t.r0 *= kTileR;
-    t.kb0 = t.split * g.kper;
-    t.kbs = min(g.kper, g.kblocks - t.kb0);
+    t.kb0 = t.split * f.kper;
+    t.kbs = min(f.kper, f.kblocks - t.kb0);
     return t;
 }
 
@@ -227,9 +255,10 @@ __device__ __forceinline__ void pack_row(const float (&v)[N], unsigned (&u)[16])
 struct Store {
     char* buf;
     unsigned flip;
+    bool leader;  // the lane that issues the copies and waits for them
     __device__ __forceinline__ char* next() {
         // all but the latest store have been read out of shared memory: the piece of the one before that is free
-        if (threadIdx.x % 32 == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        if (leader) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
         __syncwarp();
         char* b = buf + flip * kStoreBytes;
         flip ^= 1;
@@ -250,7 +279,7 @@ struct Store {
         if (tma) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) {
+            if (leader) {
                 if (r < rows && c < cols) tma_store(map, smem_u32(b), c, (int)r, z);
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
@@ -270,26 +299,25 @@ struct Store {
     }
 };
 
-// The epilogue of one piece: N sums per lane, which has row r + lane, from column c on; q: its residual.
+// The epilogue of one piece: N sums per lane, which has row r + lane, from column c on. bias: lane i has that of column
+// c + i; q: the residual.
 template <typename IO, int N>
-__device__ __forceinline__ void write_out(const GemmProblem& g, Store& store, long r, int c, const float (&q)[N],
-                                          float (&v)[N]) {
-    float b[N];
-    load_row<IO, N>(g.bias, 0, min(c, g.cols - 1), g.cols, g.vec, b);
-    if (g.has_bias) {
+__device__ __forceinline__ void write_out(const GemmProblem& g, const Fields& f, Store& store, long r, int c, float bias,
+                                          const float (&q)[N], float (&v)[N]) {
+    if (f.has_bias) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += b[i];
+        for (int i = 0; i < N; ++i) v[i] += __shfl_sync(~0u, bias, i);
     }
-    if (g.tape) {
+    if (f.tape) {
         using T = std::conditional_t<sizeof(IO) == 2, __half, float>;
-        store.operator()<T>(&g.tape_map, g.tape, g.tma_out, v, r, c, 0, g.rows, g.cols);
+        store.operator()<T>(&g.tape_map, f.tape, f.tma_out, v, r, c, 0, f.rows, f.cols);
     }
-    activate_all<sizeof(IO) == 2>(v, g.act);
-    if (g.has_residual) {
+    if (f.act) activate_all<sizeof(IO) == 2>(v, f.act);
+    if (f.has_residual) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] += q[i];
     }
-    store.operator()<IO>(&g.out_map, g.out, g.tma_out, v, r, c, 0, g.rows, g.cols);
+    store.operator()<IO>(&g.out_map, f.out, f.tma_out, v, r, c, 0, f.rows, f.cols);
 }
 
 template <int BN, int PLANES>
@@ -301,10 +329,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     char* staging = stages + (size_t)S::kStages * S::kStageBytes;
     Barriers& bars = *reinterpret_cast<Barriers*>(staging + S::kStagingBytes);
     static_assert(sizeof(Barriers) <= 256, "barriers");
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     volatile int* abort = &bars.abort;
+    const Fields f(g);
+    if (threadIdx.x == 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&g.p_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&g.q_map) : "memory");
+        if (f.tma_out) asm volatile("prefetch.tensormap [%0];" ::"l"(&g.out_map) : "memory");
+    }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::kStages; ++i) bar_init(&bars.full[i], 1), bar_init(&bars.empty[i], 1);
+        for (int i = 0; i < S::kStages; ++i) bar_init(&bars.full[i], 2), bar_init(&bars.empty[i], 1);
         for (int i = 0; i < 2; ++i) {
             bar_init(&bars.acc_full[i], 1), bar_init(&bars.acc_empty[i], kDrainWarps);
             bar_init(&bars.corr_full[i], 1), bar_init(&bars.corr_empty[i], kDrainWarps);
@@ -324,30 +358,35 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     fence_after();
     const unsigned tmem = bars.tmem, corr_base = tmem + S::kAccCols;
 
-    if (warp == 0) {
-        if (lane == 0) {
+    if (warp == 0 || warp == kQWarp) {
+        if (elect_one()) {
+            // an operand's copies: K-major, one box of a tile's rows; MN-major, boxes 64 wide, 8 KB each
+            const bool is_p = warp == 0;
+            const CUtensorMap* map = is_p ? &g.p_map : &g.q_map;
+            const int boxes = is_p ? g.p_boxes : g.q_boxes;
+            const bool mn = is_p ? g.p_mn : g.q_mn;
+            const unsigned bytes = PLANES * boxes * (is_p ? g.p_box_bytes : g.q_box_bytes);
+            const unsigned base = smem_u32(stages) + (is_p ? 0 : PLANES * S::kABytes);
+            const unsigned plane = is_p ? S::kABytes : S::kBBytes;
             int stage = 0;
             unsigned phase = 0, issued = 0;
             bool ok = true;
-            const unsigned bytes = PLANES * (g.p_boxes * g.p_box_bytes + g.q_boxes * g.q_box_bytes);
-            for (int u = blockIdx.x; ok && u < g.units; u += gridDim.x) {
-                const Unit t = unit_at<BN>(g, u);
-                for (int kb = t.kb0; kb < t.kb0 + t.kbs; ++kb) {
+            for (int u = blockIdx.x; ok && u < f.units; u += gridDim.x) {
+                const Unit t = unit_at<BN>(f, u);
+                const int row = is_p ? t.r0 : t.c0;
+                for (int k = t.kb0 * kBK; k < (t.kb0 + t.kbs) * kBK; k += kBK) {
                     ok = bar_wait(&bars.empty[stage], phase ^ 1, abort);
                     if (!ok) break;
                     unsigned long long* bar = &bars.full[stage];
                     bar_expect(bar, bytes);
-                    unsigned dst = smem_u32(stages) + stage * S::kStageBytes;
-                    // K-major: one box of a tile's rows. MN-major: boxes 64 wide, 8 KB each.
-                    for (int p = 0; p < PLANES; ++p, dst += S::kABytes) {
-                        for (int b = 0; b < g.p_boxes; ++b)
-                            tma_load(&g.p_map, dst + b * 8192, bar, g.p_mn ? t.r0 + b * 64 : kb * kBK,
-                                     g.p_mn ? kb * kBK : t.r0, p);
-                    }
-                    for (int p = 0; p < PLANES; ++p, dst += S::kBBytes) {
-                        for (int b = 0; b < g.q_boxes; ++b)
-                            tma_load(&g.q_map, dst + b * 8192, bar, g.q_mn ? t.c0 + b * 64 : kb * kBK,
-                                     g.q_mn ? kb * kBK : t.c0, p);
+                    unsigned dst = base + stage * S::kStageBytes;
+#pragma unroll
+                    for (int p = 0; p < PLANES; ++p, dst += plane) {
+                        if (mn) {
+                            for (int b = 0; b < boxes; ++b) tma_load(map, dst + b * 8192, bar, row + b * 64, k, p);
+                        } else {
+                            tma_load(map, dst, bar, k, row, p);
+                        }
                     }
                     ++issued;
                     if (++stage == S::kStages) stage = 0, phase ^= 1;
@@ -362,16 +401,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (elect_one()) {
             int stage = 0, acc = 0, corr = 0;
             unsigned phase = 0, acc_phase = 0, corr_phase = 0;
             bool ok = true;
+            const bool p_mn = g.p_mn, q_mn = g.q_mn;
             // D float32, A and B bfloat16, which of them MN-major, N / 8, M / 16
-            const unsigned idesc = 1u << 4 | 1u << 7 | 1u << 10 | (unsigned)g.p_mn << 15 | (unsigned)g.q_mn << 16 |
+            const unsigned idesc = 1u << 4 | 1u << 7 | 1u << 10 | (unsigned)p_mn << 15 | (unsigned)q_mn << 16 |
                                    (BN / 8) << 17 | (kTileR / 16) << 24;
-            const unsigned a_step = g.p_mn ? 2048 >> 4 : 32 >> 4, b_step = g.q_mn ? 2048 >> 4 : 32 >> 4;
-            for (int u = blockIdx.x; ok && u < g.units; u += gridDim.x) {
-                const Unit t = unit_at<BN>(g, u);
+            const unsigned a_step = p_mn ? 2048 >> 4 : 32 >> 4, b_step = q_mn ? 2048 >> 4 : 32 >> 4;
+            const unsigned long long a_desc = smem_desc(smem_u32(stages), p_mn);
+            const unsigned long long b_desc = smem_desc(smem_u32(stages) + PLANES * S::kABytes, q_mn);
+            for (int u = blockIdx.x; ok && u < f.units; u += gridDim.x) {
+                const Unit t = unit_at<BN>(f, u);
                 if (PLANES == 3) {
                     ok = bar_wait(&bars.corr_empty[corr], corr_phase ^ 1, abort);
                     if (!ok) break;
@@ -385,9 +427,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     ok = bar_wait(&bars.full[stage], phase, abort);
                     if (!ok) break;
                     fence_after();
-                    const unsigned base = smem_u32(stages) + stage * S::kStageBytes;
-                    const unsigned long long da = smem_desc(base, g.p_mn);
-                    const unsigned long long db = smem_desc(base + PLANES * S::kABytes, g.q_mn);
+                    const unsigned long long da = a_desc + stage * (S::kStageBytes >> 4);
+                    const unsigned long long db = b_desc + stage * (S::kStageBytes >> 4);
                     const unsigned d = tmem + acc * BN;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) mma(d, da + k * a_step, db + k * b_step, idesc, !(opens && k == 0));
@@ -426,25 +467,26 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         // a warp reads the 32 lanes of its number mod 4; two warps share them, half of the columns each
         const int quad = warp % 4, half = (warp - 2) / 4;
         const unsigned lanes = (unsigned)(quad * 32) << 16;
-        Store store{staging + (warp - 2) * 2 * kStoreBytes, 0};
+        Store store{staging + (warp - 2) * 2 * kStoreBytes, 0, elect_one()};
         int acc = 0, corr = 0;
         unsigned acc_phase = 0, corr_phase = 0;
         bool ok = true;
-        for (int u = blockIdx.x; ok && u < g.units; u += gridDim.x) {
-            const Unit t = unit_at<BN>(g, u);
+        for (int u = blockIdx.x; ok && u < f.units; u += gridDim.x) {
+            const Unit t = unit_at<BN>(f, u);
             const int c0 = t.c0 + half * (BN / 2);
             const long r0 = t.r0 + quad * 32;
-            const size_t row = (size_t)min(r0 + lane, g.rows - 1L);
+            const size_t row = (size_t)min(r0 + lane, f.rows - 1L);
             if constexpr (PLANES == 1) {
                 constexpr int N = 32;
-                float q[N];
-                if (g.has_residual) load_row<IO, N>(g.residual, row, min(c0, g.cols - 1), g.cols, g.vec, q);
+                float q[N], bias = 0.f;
+                if (f.has_bias) bias = as_float(static_cast<const IO*>(f.bias)[min(c0 + lane, f.cols - 1)]);
+                if (f.has_residual) load_row<IO, N>(f.residual, row, min(c0, f.cols - 1), f.cols, f.vec, q);
                 ok = bar_wait(&bars.acc_full[acc], acc_phase, abort);
                 ok = __all_sync(~0u, ok);
                 if (!ok) break;
                 fence_after();
                 const unsigned from = tmem + lanes + acc * BN + half * (BN / 2);
-                if (g.part) {
+                if (f.part) {
 #pragma unroll 1
                     for (int j = 0; j < BN / 2; j += 16) {
                         float v[16];
@@ -454,28 +496,36 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                             fence_before();
                             if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
                         }
-                        store.operator()<float>(&g.out_map, g.part, g.tma_out, v, r0, c0 + j, t.split, g.rows, g.cols);
+                        store.operator()<float>(&g.out_map, f.part, f.tma_out, v, r0, c0 + j, t.split, f.rows, f.cols);
                     }
                 } else {
 #pragma unroll 1
                     for (int j = 0; j < BN / 2; j += N) {
-                        float v[N], next[N];
+                        float v[N], next[N], next_bias = 0.f;
                         __syncwarp();
                         tmem_load<N>(from + j, v);
                         if (j + N == BN / 2) {
                             fence_before();
                             if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
-                        } else if (g.has_residual) {
-                            load_row<IO, N>(g.residual, row, min(c0 + j + N, g.cols - 1), g.cols, g.vec, next);
+                        } else {
+                            if (f.has_bias) next_bias = as_float(static_cast<const IO*>(f.bias)[min(c0 + j + N + lane, f.cols - 1)]);
+                            if (f.has_residual)
+                                load_row<IO, N>(f.residual, row, min(c0 + j + N, f.cols - 1), f.cols, f.vec, next);
                         }
-                        write_out<IO, N>(g, store, r0, c0 + j, q, v);
+                        write_out<IO, N>(g, f, store, r0, c0 + j, bias, q, v);
+                        bias = next_bias;
 #pragma unroll
                         for (int i = 0; i < N; ++i) q[i] = next[i];
                     }
                 }
                 if (++acc == 2) acc = 0, acc_phase ^= 1;
             } else {
-                float sum[BN / 2];
+                float sum[BN / 2], bias[BN / 32];  // of 16 columns each, in the lower lanes
+#pragma unroll
+                for (int j = 0; j < BN / 32; ++j) {
+                    bias[j] = 0.f;
+                    if (f.has_bias) bias[j] = as_float(static_cast<const IO*>(f.bias)[min(c0 + 16 * j + lane, f.cols - 1)]);
+                }
 #pragma unroll
                 for (int j = 0; j < BN / 2; ++j) sum[j] = 0.f;
                 for (int kb = 0; kb < t.kbs; kb += kChunk) {
@@ -503,7 +553,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
 #pragma unroll
                 for (int j = 0; j < BN / 2; j += 16) {
                     float q[16], v[16];
-                    if (g.has_residual) load_row<IO, 16>(g.residual, row, min(c0 + j, g.cols - 1), g.cols, g.vec, q);
+                    if (f.has_residual) load_row<IO, 16>(f.residual, row, min(c0 + j, f.cols - 1), f.cols, f.vec, q);
                     __syncwarp();
                     tmem_load<16>(corr_base + lanes + corr * BN + half * (BN / 2) + j, v);
                     if (j + 16 == BN / 2) {
@@ -513,16 +563,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) v[i] = isfinite(sum[j + i]) ? sum[j + i] + v[i] : sum[j + i];
-                    if (g.part)
-                        store.operator()<float>(&g.out_map, g.part, g.tma_out, v, r0, c0 + j, t.split, g.rows, g.cols);
+                    if (f.part)
+                        store.operator()<float>(&g.out_map, f.part, f.tma_out, v, r0, c0 + j, t.split, f.rows, f.cols);
                     else
-                        write_out<IO, 16>(g, store, r0, c0 + j, q, v);
+                        write_out<IO, 16>(g, f, store, r0, c0 + j, bias[j / 16], q, v);
                 }
                 if (++corr == 2) corr = 0, corr_phase ^= 1;
             }
         }
         // shared memory is given up once every store has read its piece
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        if (store.leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     }
     __syncwarp();
     fence_before();
