@@ -21,6 +21,24 @@ __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// The kernels of these operators follow one another closely, and each may be set up while the one before it drains
+// (programmatic dependent launch). So each calls after_previous() before it touches anything in global memory, and
+// lets its own successor come as soon as its CTAs are all placed.
+__device__ __forceinline__ void after_previous() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... K, typename... A>
+cudaError_t launch_after(void (*kernel)(K...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A&... args) {
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cfg.attrs = &at, cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // one element of a tensor whose QkDtype is known at run time only
 __device__ __forceinline__ float load_dt(const void* p, size_t i, int dtype) {
     return dtype == QK_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i])

@@ -357,6 +357,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     __syncthreads();
     fence_after();
     const unsigned tmem = bars.tmem, corr_base = tmem + S::kAccCols;
+    after_previous();
 
     if (warp == 0 || warp == kQWarp) {
         if (elect_one()) {
@@ -629,8 +630,7 @@ cudaError_t launch_shape(const GemmProblem& g, cudaStream_t st) {
     cudaError_t e = opt_in_smem(gemm_kernel<BN, PLANES>, &opted, (int)S::kSmem);
     if (e != cudaSuccess) return e;
     const int grid = g.units < kSms ? g.units : kSms;
-    gemm_kernel<BN, PLANES><<<grid, kGemmThreads, S::kSmem, st>>>(g);
-    return cudaPeekAtLastError();
+    return launch_after(gemm_kernel<BN, PLANES>, grid, kGemmThreads, S::kSmem, st, g);
 }
 
 }  // namespace

@@ -65,6 +65,7 @@ __device__ __forceinline__ void load8(const void* p, size_t at, bool vec, int n,
 template <typename IO>
 __global__ void __launch_bounds__(kThreads) prepare_kernel(const PrepArgsL a) {
     __shared__ float sums[kThreads * 8];
+    after_previous();
     int b = blockIdx.x;
     PrepJob j = a.job[0];  // in registers: a reference would be read again behind every store
     if (a.count > 1 && b >= a.job[0].blocks) {
@@ -142,6 +143,7 @@ struct ReduceArgs {
 // One element per thread: the slices of its sum in order, then the epilogue. The blocks behind those add grad_bias'
 // slabs, 32 columns each.
 __global__ void __launch_bounds__(kThreads) reduce_kernel(const ReduceArgs a) {
+    after_previous();
     int b = blockIdx.x;
     ReduceJob j = a.job[0];
     bool sums = a.count > 0 && b < j.blocks;
@@ -338,9 +340,8 @@ cudaError_t launch_prepare(const PrepArgsL& p, int io_dtype, cudaStream_t st) {
     long blocks = 0;
     for (int i = 0; i < p.count; ++i) blocks += p.job[i].blocks;
     if (blocks == 0) return cudaSuccess;
-    if (io_dtype == QK_BF16) prepare_kernel<__nv_bfloat16><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-    else prepare_kernel<float><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-    return cudaPeekAtLastError();
+    return launch_after(io_dtype == QK_BF16 ? prepare_kernel<__nv_bfloat16> : prepare_kernel<float>, (unsigned)blocks,
+                        kThreads, 0, st, p);
 }
 
 cudaError_t launch_reduce(const ReduceArgs& r, cudaStream_t st) {
@@ -349,8 +350,7 @@ cudaError_t launch_reduce(const ReduceArgs& r, cudaStream_t st) {
     if (r.gb) blocks += (r.cols + 31) / 32;
     if (blocks == 0) return cudaSuccess;
     if (blocks > 0x7fffffffl) return cudaErrorInvalidConfiguration;
-    reduce_kernel<<<(unsigned)blocks, kThreads, 0, st>>>(r);
-    return cudaPeekAtLastError();
+    return launch_after(reduce_kernel, (unsigned)blocks, kThreads, 0, st, r);
 }
 
 void add_reduce(ReduceArgs& r, const float* part, int splits, int rows, int cols, const Epilogue& epi) {

@@ -134,6 +134,7 @@ struct GroupSum {
 
 template <typename IO, int VEC, int T>
 __global__ void __launch_bounds__(block_of(T)) norm_forward_kernel(const NormArgs a) {
+    after_previous();
     constexpr int G = block_of(T) / T;
     __shared__ float2 buf[G][2][T / 32];
     const int group = threadIdx.x / T, lane = threadIdx.x % T;
@@ -173,6 +174,7 @@ __global__ void __launch_bounds__(block_of(T)) norm_forward_kernel(const NormArg
 
 template <typename IO, int VEC, int T>
 __global__ void __launch_bounds__(block_of(T)) norm_backward_kernel(const NormArgs a) {
+    after_previous();
     constexpr int G = block_of(T) / T;
     __shared__ float2 buf[G][2][T / 32];
     __shared__ float cols[G > 1 ? G * T * kElems : 1];
@@ -267,6 +269,7 @@ __global__ void __launch_bounds__(block_of(T)) norm_backward_kernel(const NormAr
 // first).
 template <typename IO>
 __global__ void __launch_bounds__(kWideThreads) norm_wide_forward_kernel(const NormArgs a) {
+    after_previous();
     __shared__ float2 buf[2][kWideThreads / 32];
     GroupSum<kWideThreads> sum{&buf[0][0], 0, 0};
     const size_t at = (size_t)blockIdx.x * a.dim;
@@ -290,6 +293,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_wide_forward_kernel(const N
 
 template <typename IO>
 __global__ void __launch_bounds__(kWideThreads) norm_wide_gx_kernel(const NormArgs a) {
+    after_previous();
     __shared__ float2 buf[2][kWideThreads / 32];
     GroupSum<kWideThreads> sum{&buf[0][0], 0, 0};
     const size_t at = (size_t)blockIdx.x * a.dim;
@@ -314,6 +318,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_wide_gx_kernel(const NormAr
 // partial sums of grad_w and grad_b: one thread per column, one slice of rows per blockIdx.y
 template <typename IO>
 __global__ void __launch_bounds__(kWideThreads) norm_wide_param_kernel(const NormArgs a) {
+    after_previous();
     const int c = blockIdx.x * kWideThreads + threadIdx.x;
     if (c >= a.dim) return;
     const IO* x = static_cast<const IO*>(a.x) + c;
@@ -331,6 +336,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_wide_param_kernel(const Nor
 
 // grad_w (blockIdx.y 0) and grad_b (1): adds the slices of 32 columns, each in a fixed order
 __global__ void __launch_bounds__(32 * kFinishSlices) norm_finish_kernel(const NormArgs a, int slices) {
+    after_previous();
     __shared__ float tile[kFinishSlices][33];
     const int c = blockIdx.x * 32 + threadIdx.x;
     void* out = blockIdx.y ? a.gb : a.gw;
@@ -360,41 +366,47 @@ int threads_of(int dim) {
 bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
 template <typename IO, int VEC, int T>
-void run_t(const NormArgs& a, bool backward, cudaStream_t st) {
+cudaError_t run_t(const NormArgs& a, bool backward, cudaStream_t st) {
     constexpr int G = block_of(T) / T;
-    if (backward)
-        norm_backward_kernel<IO, VEC, T><<<norm_slices(a.rows, a.dim), block_of(T), 0, st>>>(a);
-    else
-        norm_forward_kernel<IO, VEC, T><<<(unsigned)((a.rows + G - 1L) / G), block_of(T), 0, st>>>(a);
+    if (backward) return launch_after(norm_backward_kernel<IO, VEC, T>, norm_slices(a.rows, a.dim), block_of(T), 0, st, a);
+    return launch_after(norm_forward_kernel<IO, VEC, T>, (unsigned)((a.rows + G - 1L) / G), block_of(T), 0, st, a);
 }
 
 template <typename IO, int VEC>
-void run_vec(const NormArgs& a, bool backward, cudaStream_t st) {
+cudaError_t run_vec(const NormArgs& a, bool backward, cudaStream_t st) {
     switch (threads_of(a.dim)) {
-        case 32: run_t<IO, VEC, 32>(a, backward, st); break;
-        case 64: run_t<IO, VEC, 64>(a, backward, st); break;
-        case 128: run_t<IO, VEC, 128>(a, backward, st); break;
-        case 256: run_t<IO, VEC, 256>(a, backward, st); break;
-        default: run_t<IO, VEC, 512>(a, backward, st); break;
+        case 32: return run_t<IO, VEC, 32>(a, backward, st);
+        case 64: return run_t<IO, VEC, 64>(a, backward, st);
+        case 128: return run_t<IO, VEC, 128>(a, backward, st);
+        case 256: return run_t<IO, VEC, 256>(a, backward, st);
+        default: return run_t<IO, VEC, 512>(a, backward, st);
     }
 }
 
 template <typename IO>
-void run_rows(const NormArgs& a, bool backward, cudaStream_t st) {
+cudaError_t run_rows(const NormArgs& a, bool backward, cudaStream_t st) {
     constexpr int VEC = 16 / sizeof(IO);
     // 16-byte accesses where every row of every tensor starts on such a boundary
     const bool vec = a.dim % VEC == 0 && aligned16(a.x) && aligned16(a.y) && aligned16(a.gy) && aligned16(a.gx) &&
                      aligned16(a.w) && aligned16(a.b);
-    if (vec) run_vec<IO, VEC>(a, backward, st);
-    else run_vec<IO, 1>(a, backward, st);
+    return vec ? run_vec<IO, VEC>(a, backward, st) : run_vec<IO, 1>(a, backward, st);
 }
 
 template <typename IO>
-void run_wide_backward(const NormArgs& a, cudaStream_t st) {
-    if (a.gx) norm_wide_gx_kernel<IO><<<a.rows, kWideThreads, 0, st>>>(a);
-    if (a.part)
-        norm_wide_param_kernel<IO>
-            <<<dim3((a.dim + kWideThreads - 1) / kWideThreads, norm_slices(a.rows, a.dim)), kWideThreads, 0, st>>>(a);
+cudaError_t run_wide(const NormArgs& a, bool backward, cudaStream_t st) {
+    if (!backward) return launch_after(norm_wide_forward_kernel<IO>, a.rows, kWideThreads, 0, st, a);
+    cudaError_t e = cudaSuccess;
+    if (a.gx) e = launch_after(norm_wide_gx_kernel<IO>, a.rows, kWideThreads, 0, st, a);
+    if (e == cudaSuccess && a.part)
+        e = launch_after(norm_wide_param_kernel<IO>,
+                         dim3((a.dim + kWideThreads - 1) / kWideThreads, norm_slices(a.rows, a.dim)), kWideThreads, 0, st, a);
+    return e;
+}
+
+cudaError_t run(const NormArgs& a, bool backward, cudaStream_t st) {
+    const bool half = a.io_dtype == QK_BF16;
+    if (is_wide(a.dim)) return half ? run_wide<__nv_bfloat16>(a, backward, st) : run_wide<float>(a, backward, st);
+    return half ? run_rows<__nv_bfloat16>(a, backward, st) : run_rows<float>(a, backward, st);
 }
 
 }  // namespace
@@ -407,31 +419,13 @@ int norm_slices(int rows, int dim) {
     return need < most ? need : most;
 }
 
-cudaError_t launch_norm_forward(const NormArgs& a, cudaStream_t st) {
-    if (is_wide(a.dim)) {
-        if (a.io_dtype == QK_BF16) norm_wide_forward_kernel<__nv_bfloat16><<<a.rows, kWideThreads, 0, st>>>(a);
-        else norm_wide_forward_kernel<float><<<a.rows, kWideThreads, 0, st>>>(a);
-    } else if (a.io_dtype == QK_BF16) {
-        run_rows<__nv_bfloat16>(a, false, st);
-    } else {
-        run_rows<float>(a, false, st);
-    }
-    return cudaPeekAtLastError();
-}
+cudaError_t launch_norm_forward(const NormArgs& a, cudaStream_t st) { return run(a, false, st); }
 
 cudaError_t launch_norm_backward(const NormArgs& a, cudaStream_t st) {
-    if (is_wide(a.dim)) {
-        if (a.io_dtype == QK_BF16) run_wide_backward<__nv_bfloat16>(a, st);
-        else run_wide_backward<float>(a, st);
-    } else if (a.io_dtype == QK_BF16) {
-        run_rows<__nv_bfloat16>(a, true, st);
-    } else {
-        run_rows<float>(a, true, st);
-    }
-    cudaError_t e = cudaPeekAtLastError();
+    const cudaError_t e = run(a, true, st);
     if (e != cudaSuccess || !a.part) return e;
-    norm_finish_kernel<<<dim3((a.dim + 31) / 32, 2), dim3(32, kFinishSlices), 0, st>>>(a, norm_slices(a.rows, a.dim));
-    return cudaPeekAtLastError();
+    return launch_after(norm_finish_kernel, dim3((a.dim + 31) / 32, 2), dim3(32, kFinishSlices), 0, st, a,
+                        norm_slices(a.rows, a.dim));
 }
 
 }  // namespace qk
