@@ -39,7 +39,7 @@ int check_aligned(const void* p, int width, int io_dtype, const char* what) {
 }
 
 size_t norm_scratch(const QkNormDesc& d) {
-    return qk::align256((size_t)2 * qk::norm_slices(d.rows, d.dim) * d.dim * sizeof(float));
+    return qk::align256((size_t)2 * qk::norm_slices(d.rows, d.dim, d.io_dtype) * d.dim * sizeof(float));
 }
 
 // a size of 0 says that the descriptor was refused, so "none" is 1

@@ -4,29 +4,34 @@
 //   gx = rstd * (gw - mean(gw) - xh * mean(gw * xh)),  gw = gy * w
 //   grad_w = sum over rows of gy * xh                  grad_b = sum over rows of gy
 //
-// Bound by memory: 2 M D elements forward, 3 M D backward. So each row is read once: T threads hold it in registers
-// (16 elements each), take the mean, then the squares about the mean (no cancellation, whatever the row's offset), and
-// write. The backward walks rows with a fixed set of CTAs, so that the threads' own columns of grad_w and grad_b stay in
-// registers over all their rows; one partial row per CTA goes to scratch, and a second launch adds those in order (no
-// atomics: the same bits every run). The next row's x and gy are fetched before the current one is worked on.
+// Bound by memory: 2 M D elements forward, 3 M D backward. So each row is read once: T threads hold it in registers, E
+// elements each, take the mean, then the squares about the mean (no cancellation, whatever the row's offset), and write.
+// A fixed set of CTAs walks the rows, so that weight and bias, and in the backward the threads' own columns of grad_w and
+// grad_b, stay in registers; one partial row per CTA goes to scratch, and a second launch adds those in order (no
+// atomics: the same bits every run). The next row is fetched before the current one is worked on.
+//
+// A warp takes a whole row where it can: then the sums need no barrier, and their cost is spread over up to 24
+// elements per thread. (With 16 elements per thread and weight and bias read again for every row, bfloat16 rows were bound by
+// instructions, at half of float32's bandwidth.)
 #include <type_traits>
 
 #include "qk_dense.cuh"
+#include "qk_packed.cuh"
 
 namespace qk {
 namespace {
 
-constexpr int kElems = 16;      // of a row, per thread
-constexpr int kMaxT = 512;      // threads of a row: rows up to 8192 stay in registers, wider ones are read again
+constexpr int kMaxT = 512;       // threads of a row, 16 elements each at least: rows up to 8192 stay in registers,
+constexpr int kMaxDim = 8192;    // wider ones are read again
 constexpr int kWideThreads = 256;
 constexpr int kFinishSlices = 32;
 
 __host__ __device__ constexpr int block_of(int t) { return t < 256 ? 256 : t; }
 
 // The part of one row that a thread holds: NV vectors of VEC elements, vector j at column (j * T + lane) * VEC.
-template <typename IO, int VEC, int T>
+template <typename IO, int VEC, int T, int E>
 struct Piece {
-    static constexpr int NV = kElems / VEC;
+    static constexpr int NV = E / VEC;
     using Raw = std::conditional_t<VEC == 1, IO, uint4>;
     Raw v[NV];
     __device__ __forceinline__ void load(const IO* row, int dim, int lane) {
@@ -37,46 +42,54 @@ struct Piece {
             if (c < dim) v[j] = *reinterpret_cast<const Raw*>(row + c);
         }
     }
-    __device__ __forceinline__ void unpack(float (&f)[kElems]) const {
+    __device__ __forceinline__ void unpack(f2 (&f)[E / 2]) const {
         if constexpr (VEC == 1) {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) f[j] = as_float(v[j]);
+            for (int j = 0; j < NV; j += 2) f[j / 2] = make_float2(as_float(v[j]), as_float(v[j + 1]));
         } else if constexpr (VEC == 4) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                f[4 * j] = __uint_as_float(v[j].x);
-                f[4 * j + 1] = __uint_as_float(v[j].y);
-                f[4 * j + 2] = __uint_as_float(v[j].z);
-                f[4 * j + 3] = __uint_as_float(v[j].w);
+                f[2 * j] = make_float2(__uint_as_float(v[j].x), __uint_as_float(v[j].y));
+                f[2 * j + 1] = make_float2(__uint_as_float(v[j].z), __uint_as_float(v[j].w));
             }
         } else {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const unsigned u[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    f[8 * j + 2 * k] = __uint_as_float(u[k] << 16);
-                    f[8 * j + 2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
-                }
+                for (int k = 0; k < 4; ++k)
+                    f[4 * j + k] = make_float2(__uint_as_float(u[k] << 16), __uint_as_float(u[k] & 0xffff0000u));
             }
         }
     }
 };
 
-template <typename IO, int VEC>
-__device__ __forceinline__ void store_vec(IO* at, const float* f) {
-    if constexpr (VEC == 1) {
-        *at = from_float<IO>(f[0]);
-    } else if constexpr (VEC == 4) {
-        *reinterpret_cast<float4*>(at) = make_float4(f[0], f[1], f[2], f[3]);
-    } else {
-        unsigned u[4];
+// element e of a thread's values
+template <int N>
+__device__ __forceinline__ float at(const f2 (&f)[N], int e) {
+    return e % 2 ? f[e / 2].y : f[e / 2].x;
+}
+
+// the thread's values to its columns of a row
+template <typename IO, int VEC, int T, int E>
+__device__ __forceinline__ void store_row(IO* row, int dim, int lane, const f2 (&f)[E / 2]) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
-            u[k] = *reinterpret_cast<const unsigned*>(&h);
+    for (int j = 0; j < E / VEC; ++j) {
+        const int c = (j * T + lane) * VEC;
+        if (c >= dim) continue;
+        if constexpr (VEC == 1) {
+            row[c] = from_float<IO>(at(f, j));
+        } else if constexpr (VEC == 4) {
+            *reinterpret_cast<float4*>(row + c) = make_float4(f[2 * j].x, f[2 * j].y, f[2 * j + 1].x, f[2 * j + 1].y);
+        } else {
+            unsigned u[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(f[4 * j + k].x, f[4 * j + k].y);
+                u[k] = *reinterpret_cast<const unsigned*>(&h);
+            }
+            *reinterpret_cast<uint4*>(row + c) = make_uint4(u[0], u[1], u[2], u[3]);
         }
-        *reinterpret_cast<uint4*>(at) = make_uint4(u[0], u[1], u[2], u[3]);
     }
 }
 
@@ -132,135 +145,159 @@ struct GroupSum {
     }
 };
 
-template <typename IO, int VEC, int T>
-__global__ void __launch_bounds__(block_of(T)) norm_forward_kernel(const NormArgs a) {
-    after_previous();
+// the thread's parameters, columns behind the row's end as `other`
+template <int VEC, int T, int E>
+__device__ __forceinline__ void own_params(const void* p, int dtype, int dim, int lane, float other, f2 (&f)[E / 2]) {
+    float v[E];
+#pragma unroll
+    for (int j = 0; j < E / VEC; ++j) {
+        const int c = (j * T + lane) * VEC;
+        load_params<VEC>(c < dim ? p : nullptr, dtype, c, other, v + j * VEC);
+    }
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) f[i] = make_float2(v[2 * i], v[2 * i + 1]);
+}
+
+// CTAs of 256 threads: two on an SM at least, so 128 registers at most. Arithmetic on pairs: one issue slot for both.
+template <typename IO, int VEC, int T, int E>
+__global__ void __launch_bounds__(block_of(T), 512 / block_of(T)) norm_forward_kernel(const NormArgs a) {
     constexpr int G = block_of(T) / T;
     __shared__ float2 buf[G][2][T / 32];
+    after_previous();
     const int group = threadIdx.x / T, lane = threadIdx.x % T;
-    const long row = (long)blockIdx.x * G + group;
-    if (row >= a.rows) return;  // a whole group leaves together: its barrier counts its own threads only
     GroupSum<T> sum{&buf[group][0][0], group, 0};
-    Piece<IO, VEC, T> p;
-    p.load(static_cast<const IO*>(a.x) + row * a.dim, a.dim, lane);
-    float x[kElems];
-    p.unpack(x);
-    float s = 0.f;
+    const IO* xs = static_cast<const IO*>(a.x);
+    const long step = (long)gridDim.x * G;
+    long row = (long)blockIdx.x * G + group;  // a whole group leaves together: its barrier counts its own threads only
+    Piece<IO, VEC, T, E> p;
+    if (row < a.rows) p.load(xs + row * a.dim, a.dim, lane);
+    f2 w[E / 2], b[E / 2];
+    own_params<VEC, T, E>(a.w, a.param_dtype, a.dim, lane, 1.f, w);
+    own_params<VEC, T, E>(a.b, a.param_dtype, a.dim, lane, 0.f, b);
+    const float inv = 1.f / a.dim;
+    for (; row < a.rows; row += step) {
+        f2 x[E / 2], s = pk(0.f);
+        p.unpack(x);
+        if (row + step < a.rows) p.load(xs + (row + step) * a.dim, a.dim, lane);
 #pragma unroll
-    for (int e = 0; e < kElems; ++e) s += x[e];  // columns past the end hold zeros
-    const float mean = sum(make_float2(s, 0.f)).x / a.dim;
-    float q = 0.f;
+        for (int i = 0; i < E / 2; ++i) s = add2(s, x[i]);  // columns past the end hold zeros
+        const float mean = sum(make_float2(s.x + s.y, 0.f)).x * inv;
+        f2 q = pk(0.f);
 #pragma unroll
-    for (int e = 0; e < kElems; ++e) {
-        const int c = (e / VEC * T + lane) * VEC;
-        x[e] -= mean;
-        if (c < a.dim) q = fmaf(x[e], x[e], q);
-    }
-    const float rstd = 1.f / sqrtf(sum(make_float2(q, 0.f)).x / a.dim + a.eps);
-    if (lane == 0 && a.stats_out) a.stats_out[row] = make_float2(mean, rstd);
-    IO* y = static_cast<IO*>(a.y) + row * a.dim;
+        for (int i = 0; i < E / 2; ++i) {
+            x[i] = add2(x[i], pk(-mean));
+            // and stay zero there: an end falls between the pairs of a vector, but within one of single elements
+            if ((2 * i / VEC * T + lane) * VEC >= a.dim) x[i].x = 0.f;
+            if (((2 * i + 1) / VEC * T + lane) * VEC >= a.dim) x[i].y = 0.f;
+            q = fma2(x[i], x[i], q);
+        }
+        const float rstd = rsqrtf(sum(make_float2(q.x + q.y, 0.f)).x * inv + a.eps);
+        if (lane == 0 && a.stats_out) a.stats_out[row] = make_float2(mean, rstd);
 #pragma unroll
-    for (int j = 0; j < kElems / VEC; ++j) {
-        const int c = (j * T + lane) * VEC;
-        if (c >= a.dim) continue;
-        float w[VEC], b[VEC], o[VEC];
-        load_params<VEC>(a.w, a.param_dtype, c, 1.f, w);
-        load_params<VEC>(a.b, a.param_dtype, c, 0.f, b);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = fmaf(x[j * VEC + i] * rstd, w[i], b[i]);
-        store_vec<IO, VEC>(y + c, o);
+        for (int i = 0; i < E / 2; ++i) x[i] = fma2(mul2(x[i], pk(rstd)), w[i], b[i]);
+        store_row<IO, VEC, T, E>(static_cast<IO*>(a.y) + row * a.dim, a.dim, lane, x);
     }
 }
 
-template <typename IO, int VEC, int T>
-__global__ void __launch_bounds__(block_of(T)) norm_backward_kernel(const NormArgs a) {
-    after_previous();
+template <typename IO, int VEC, int T, int E>
+__global__ void __launch_bounds__(block_of(T), 512 / block_of(T)) norm_backward_kernel(const NormArgs a) {
     constexpr int G = block_of(T) / T;
+    constexpr bool kKeepW = sizeof(IO) == 2;  // float32 rows leave no registers for the weight: from L1 for every row
     __shared__ float2 buf[G][2][T / 32];
-    __shared__ float cols[G > 1 ? G * T * kElems : 1];
+    __shared__ __align__(16) float cols[2][G > 1 ? G * T * E : 1];
+    after_previous();
     const int group = threadIdx.x / T, lane = threadIdx.x % T;
     GroupSum<T> sum{&buf[group][0][0], group, 0};
-    float dw[kElems], db[kElems];
+    f2 dw[E / 2], db[E / 2], w[kKeepW ? E / 2 : 1];
 #pragma unroll
-    for (int e = 0; e < kElems; ++e) dw[e] = db[e] = 0.f;
+    for (int i = 0; i < E / 2; ++i) dw[i] = db[i] = pk(0.f);
     const IO* xs = static_cast<const IO*>(a.x);
     const IO* gys = static_cast<const IO*>(a.gy);
+    const float inv = 1.f / a.dim;
     const long step = (long)gridDim.x * G;
     long row = (long)blockIdx.x * G + group;
-    Piece<IO, VEC, T> px, pg;
+    Piece<IO, VEC, T, E> px, pg;
     float2 st{};
     if (row < a.rows) {
         px.load(xs + row * a.dim, a.dim, lane);
         pg.load(gys + row * a.dim, a.dim, lane);
         st = a.stats[row];
     }
+    if constexpr (kKeepW) own_params<VEC, T, E>(a.w, a.param_dtype, a.dim, lane, 1.f, w);
     for (; row < a.rows; row += step) {
-        float xh[kElems], g[kElems];
+        f2 xh[E / 2], g[E / 2], s1 = pk(0.f), s2 = pk(0.f);
         px.unpack(xh);
         pg.unpack(g);
-        const float mean = st.x, rstd = st.y;
+        const f2 rstd = pk(st.y), shift = pk(-st.x * st.y);
         if (row + step < a.rows) {
             px.load(xs + (row + step) * a.dim, a.dim, lane);
             pg.load(gys + (row + step) * a.dim, a.dim, lane);
             st = a.stats[row + step];
         }
-        float2 s = make_float2(0.f, 0.f);
+        // past the end gy is zero, and so is all that it is a factor of
+        auto pair = [&](int i, f2 weight) {
+            xh[i] = fma2(xh[i], rstd, shift);
+            dw[i] = fma2(g[i], xh[i], dw[i]);
+            db[i] = add2(db[i], g[i]);
+            g[i] = mul2(g[i], weight);
+            s1 = add2(s1, g[i]);
+            s2 = fma2(g[i], xh[i], s2);
+        };
+        if constexpr (kKeepW) {
 #pragma unroll
-        for (int j = 0; j < kElems / VEC; ++j) {
-            const int c = (j * T + lane) * VEC;
-            if (c >= a.dim) continue;
-            float w[VEC];
-            load_params<VEC>(a.w, a.param_dtype, c, 1.f, w);
+            for (int i = 0; i < E / 2; ++i) pair(i, w[i]);
+        } else {
+            constexpr int W = VEC == 1 ? 2 : VEC;  // elements at a time
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int e = j * VEC + i;
-                xh[e] = (xh[e] - mean) * rstd;
-                dw[e] = fmaf(g[e], xh[e], dw[e]);
-                db[e] += g[e];
-                g[e] *= w[i];
-                s.x += g[e];
-                s.y = fmaf(g[e], xh[e], s.y);
+            for (int j = 0; j < E / W; ++j) {
+                float v[W];
+#pragma unroll
+                for (int k = 0; k < W / VEC; ++k) {
+                    const int c = ((j * (W / VEC) + k) * T + lane) * VEC;
+                    load_params<VEC>(c < a.dim ? a.w : nullptr, a.param_dtype, c, 1.f, v + k * VEC);
+                }
+#pragma unroll
+                for (int k = 0; k < W / 2; ++k) pair(j * (W / 2) + k, make_float2(v[2 * k], v[2 * k + 1]));
             }
         }
         if (!a.gx) continue;
-        s = sum(s);
-        const float m1 = s.x / a.dim, m2 = s.y / a.dim;
-        IO* gx = static_cast<IO*>(a.gx) + row * a.dim;
+        const float2 s = sum(make_float2(s1.x + s1.y, s2.x + s2.y));
+        const f2 m1 = pk(-s.x * inv * rstd.x), m2 = pk(-s.y * inv * rstd.x);
 #pragma unroll
-        for (int j = 0; j < kElems / VEC; ++j) {
-            const int c = (j * T + lane) * VEC;
-            if (c >= a.dim) continue;
-            float o[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int e = j * VEC + i;
-                o[i] = (g[e] - m1 - xh[e] * m2) * rstd;
-            }
-            store_vec<IO, VEC>(gx + c, o);
-        }
+        for (int i = 0; i < E / 2; ++i) g[i] = fma2(g[i], rstd, fma2(xh[i], m2, m1));
+        store_row<IO, VEC, T, E>(static_cast<IO*>(a.gx) + row * a.dim, a.dim, lane, g);
     }
     if (!a.part) return;
+    // this CTA's sums: straight to scratch, or over its groups first
+    auto put = [&](float* out, const f2(&v)[E / 2], int end) {
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        float* out = a.part + ((size_t)which * gridDim.x + blockIdx.x) * a.dim;
-        if constexpr (G == 1) {
+        for (int j = 0; j < E / VEC; ++j) {
+            const int c = (j * T + lane) * VEC;
+            if (c >= end) continue;
+            if constexpr (VEC == 1) {
+                out[c] = at(v, j);
+            } else {
 #pragma unroll
-            for (int e = 0; e < kElems; ++e) {
-                const int c = (e / VEC * T + lane) * VEC + e % VEC;
-                if (c < a.dim) out[c] = which ? db[e] : dw[e];
+                for (int i = j * VEC / 2; i < (j + 1) * VEC / 2; i += 2)
+                    *reinterpret_cast<float4*>(out + c + 2 * i - j * VEC) = make_float4(v[i].x, v[i].y, v[i + 1].x, v[i + 1].y);
             }
-        } else {
-            __syncthreads();
+        }
+    };
+    float* out = a.part + (size_t)blockIdx.x * a.dim;
+    const size_t bias = (size_t)gridDim.x * a.dim;
+    if constexpr (G == 1) {
+        put(out, dw, a.dim);
+        put(out + bias, db, a.dim);
+    } else {
+        put(cols[0] + group * T * E, dw, T * E);
+        put(cols[1] + group * T * E, db, T * E);
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.dim; c += block_of(T)) {
+            float u = cols[0][c], v = cols[1][c];
 #pragma unroll
-            for (int e = 0; e < kElems; ++e)
-                cols[group * T * kElems + (e / VEC * T + lane) * VEC + e % VEC] = which ? db[e] : dw[e];
-            __syncthreads();
-            for (int c = threadIdx.x; c < a.dim; c += block_of(T)) {
-                float s = cols[c];
-#pragma unroll
-                for (int k = 1; k < G; ++k) s += cols[k * T * kElems + c];
-                out[c] = s;
-            }
+            for (int k = 1; k < G; ++k) u += cols[0][k * T * E + c], v += cols[1][k * T * E + c];
+            out[c] = u;
+            out[bias + c] = v;
         }
     }
 }
@@ -334,7 +371,8 @@ __global__ void __launch_bounds__(kWideThreads) norm_wide_param_kernel(const Nor
     a.part[((size_t)gridDim.y + blockIdx.y) * a.dim + c] = db;
 }
 
-// grad_w (blockIdx.y 0) and grad_b (1): adds the slices of 32 columns, each in a fixed order
+// grad_w (blockIdx.y 0) and grad_b (1): adds the slices of 32 columns, each in a fixed order, 32 of them at a time
+// (256 threads of four columns each took 0.7 us longer over 296 slices)
 __global__ void __launch_bounds__(32 * kFinishSlices) norm_finish_kernel(const NormArgs a, int slices) {
     after_previous();
     __shared__ float tile[kFinishSlices][33];
@@ -343,8 +381,10 @@ __global__ void __launch_bounds__(32 * kFinishSlices) norm_finish_kernel(const N
     if (!out) return;
     const float* part = a.part + (size_t)blockIdx.y * slices * a.dim;
     float s = 0.f;
-    if (c < a.dim)
+    if (c < a.dim) {
+#pragma unroll 10
         for (int k = threadIdx.y; k < slices; k += kFinishSlices) s += part[(size_t)k * a.dim + c];
+    }
     tile[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y == 0 && c < a.dim) {
@@ -354,27 +394,55 @@ __global__ void __launch_bounds__(32 * kFinishSlices) norm_finish_kernel(const N
     }
 }
 
-bool is_wide(int dim) { return dim > kMaxT * kElems; }
+bool is_wide(int dim) { return dim > kMaxDim; }
 
-// threads of a row: the smallest power of two whose registers hold it
-int threads_of(int dim) {
+// Elements of a row that a thread can hold without spilling its 128 registers (bfloat16 at 24 spills 45 of them in the
+// backward: 12.6 against 8.4 us at 8192 x 768; single elements at 16 spill up to 127)
+int most_of(int io_dtype, int dim, bool backward) {
+    const bool vec = dim % (io_dtype == QK_BF16 ? 8 : 4) == 0;
+    if (backward) return vec ? 16 : 8;
+    return vec && io_dtype == QK_BF16 ? 24 : 16;
+}
+// Threads of a row: a warp while they hold it, doubled until they do. Few rows get more threads each, down to eight
+// elements per thread, until there are some 512 threads per SM: a row then takes less time.
+int threads_of(int rows, int dim, int io_dtype, bool backward) {
+    const int most = most_of(io_dtype, dim, backward);
     int t = 32;
-    while (t < kMaxT && t * kElems < dim) t *= 2;
+    while (t < kMaxT && (t * most < dim || (t * 8 < dim && (long)rows * t < 512l * kSms))) t *= 2;
     return t;
 }
 
 bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
+// CTAs for groups of `each` rows at least
+int ctas_of(int rows, int t, int each) {
+    const int g = block_of(t) / t * each, most = kSms * (512 / block_of(t));
+    const int need = (int)((rows + (long)g - 1) / g);
+    return need < most ? need : most;
+}
+// A CTA of the backward leaves a row of partial sums, which the second launch reads again: not for a single row each.
+constexpr int kBackwardEach = 2;
+
+template <typename IO, int VEC, int T, int E>
+cudaError_t run_e(const NormArgs& a, bool backward, cudaStream_t st) {
+    const dim3 grid(ctas_of(a.rows, T, backward ? kBackwardEach : 1)), block(block_of(T));
+    if constexpr (E <= 16)
+        if (backward) return launch_after(norm_backward_kernel<IO, VEC, T, E>, grid, block, 0, st, a);
+    return launch_after(norm_forward_kernel<IO, VEC, T, E>, grid, block, 0, st, a);
+}
+
 template <typename IO, int VEC, int T>
 cudaError_t run_t(const NormArgs& a, bool backward, cudaStream_t st) {
-    constexpr int G = block_of(T) / T;
-    if (backward) return launch_after(norm_backward_kernel<IO, VEC, T>, norm_slices(a.rows, a.dim), block_of(T), 0, st, a);
-    return launch_after(norm_forward_kernel<IO, VEC, T>, (unsigned)((a.rows + G - 1L) / G), block_of(T), 0, st, a);
+    const int need = (a.dim + T - 1) / T;  // elements per thread
+    if (need <= 8) return run_e<IO, VEC, T, 8>(a, backward, st);
+    if constexpr (sizeof(IO) == 2)  // rows of whole 16-byte words that do not start on one: by element, as many of them
+        if (need > 16 && !backward) return run_e<IO, VEC, T, 24>(a, backward, st);
+    return run_e<IO, VEC, T, 16>(a, backward, st);
 }
 
 template <typename IO, int VEC>
 cudaError_t run_vec(const NormArgs& a, bool backward, cudaStream_t st) {
-    switch (threads_of(a.dim)) {
+    switch (threads_of(a.rows, a.dim, a.io_dtype, backward)) {
         case 32: return run_t<IO, VEC, 32>(a, backward, st);
         case 64: return run_t<IO, VEC, 64>(a, backward, st);
         case 128: return run_t<IO, VEC, 128>(a, backward, st);
@@ -399,7 +467,7 @@ cudaError_t run_wide(const NormArgs& a, bool backward, cudaStream_t st) {
     if (a.gx) e = launch_after(norm_wide_gx_kernel<IO>, a.rows, kWideThreads, 0, st, a);
     if (e == cudaSuccess && a.part)
         e = launch_after(norm_wide_param_kernel<IO>,
-                         dim3((a.dim + kWideThreads - 1) / kWideThreads, norm_slices(a.rows, a.dim)), kWideThreads, 0, st, a);
+                         dim3((a.dim + kWideThreads - 1) / kWideThreads, norm_slices(a.rows, a.dim, a.io_dtype)), kWideThreads, 0, st, a);
     return e;
 }
 
@@ -411,12 +479,9 @@ cudaError_t run(const NormArgs& a, bool backward, cudaStream_t st) {
 
 }  // namespace
 
-int norm_slices(int rows, int dim) {
+int norm_slices(int rows, int dim, int io_dtype) {
     if (is_wide(dim)) return rows < 64 ? rows : 64;
-    const int t = threads_of(dim), g = block_of(t) / t;
-    const int most = kSms * (block_of(t) == 256 ? 2 : 1);
-    const int need = (int)((rows + (long)g - 1) / g);
-    return need < most ? need : most;
+    return ctas_of(rows, threads_of(rows, dim, io_dtype, true), kBackwardEach);
 }
 
 cudaError_t launch_norm_forward(const NormArgs& a, cudaStream_t st) { return run(a, false, st); }
@@ -424,8 +489,9 @@ cudaError_t launch_norm_forward(const NormArgs& a, cudaStream_t st) { return run
 cudaError_t launch_norm_backward(const NormArgs& a, cudaStream_t st) {
     const cudaError_t e = run(a, true, st);
     if (e != cudaSuccess || !a.part) return e;
-    return launch_after(norm_finish_kernel, dim3((a.dim + 31) / 32, 2), dim3(32, kFinishSlices), 0, st, a,
-                        norm_slices(a.rows, a.dim));
+    const dim3 grid((a.dim + 31) / 32, 2);
+    const int slices = norm_slices(a.rows, a.dim, a.io_dtype);
+    return launch_after(norm_finish_kernel, grid, dim3(32, kFinishSlices), 0, st, a, slices);
 }
 
 }  // namespace qk
