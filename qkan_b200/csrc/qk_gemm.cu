@@ -1,588 +1,17 @@
-// Matrix products of the linear map on the tensor cores (tcgen05): C[r,c] = sum_k P[r,k] Q[c,k] with the epilogue
-// act(C + bias[c]) + residual[r,c].
-//
-// One CTA per SM walks units of work (a tile of 128 rows and BN columns, a slice of the depth). Two warps copy 64-deep
-// blocks of the operands, one each, into a ring of stages (TMA, 128-byte swizzle; one thread for both, at 140 clocks a
-// copy, was slower than the MMAs of narrow tiles), warp 1 issues the MMAs, eight warps drain the sums from one of two
-// accumulators in tensor memory while the other one is filled. An operand is read as it lies in
-// memory: "K-major" when the summed axis is contiguous (forward: x and W), "MN-major" when it is the other axis (W in
-// grad_x, x and gz in grad_weight).
-//
-// A lane of tensor memory is a row of C, so a thread of the epilogue has one row and reads the residual along it. Results
-// go through 64-byte rows in shared memory, from where TMA stores them (rows of whole 16-byte words) or the warp does,
-// row by row. Stored straight from the registers, two bytes per lane and row, a 64 x 128 tile took 1.4 us; that was the
-// whole time of a product with a short depth.
-//
-// float32 (PLANES == 3): x = h + m + l exactly, each part a bfloat16 (8 significant bits, float32's exponents). Six of
-// the nine products are kept: hh | hm mh hl lh mm; what is dropped is below 2^-22 of |x||w|. hh goes to one accumulator
-// and the five small ones to another. The tensor core truncates where it adds to its accumulator, which over a long
-// sum would drift by more than float32 rounding does: so hh is drained every kChunk blocks and added in registers, with
-// rounding. Where hh's sum is not finite the small products are left out: float32's own infinities come out.
-#include <cuda.h>
-
+// Host side of the products (qk_gemm.cuh): their tensor maps, and the launch for each type.
 #include "qk_linear.cuh"
 
 namespace qk {
+
+cudaError_t launch_gemm_bf16(const GemmProblem& g, int bn, cudaStream_t st);
+cudaError_t launch_gemm_f32(const GemmProblem& g, int bn, cudaStream_t st);
+cudaError_t gave_up_bf16(unsigned* total, cudaStream_t st);
+cudaError_t gave_up_f32(unsigned* total, cudaStream_t st);
+
 namespace {
 
-constexpr int kBK = 64;             // depth of a stage: 128 bytes of bfloat16, one swizzle row
-constexpr int kTileR = 128;         // the MMA's M
-constexpr int kChunk = 2;           // stages between two drains of hh (float32)
-constexpr int kGemmThreads = 352;   // copies of P, MMAs, 8 epilogue warps, copies of Q
-constexpr int kDrainWarps = 8;
-constexpr int kQWarp = 10;
-constexpr unsigned long long kGiveUpNs = 10ull * 1000 * 1000 * 1000;  // the longest that a wait may take
-
-constexpr int kStoreBytes = 2048;   // 32 rows of 64 bytes: what a warp stages for one store; two of them per warp
-
-template <int BN, int PLANES>
-struct Shape {
-    static constexpr int kABytes = kTileR * 128;
-    static constexpr int kBBytes = BN * 128;
-    static constexpr int kStageBytes = PLANES * (kABytes + kBBytes);
-    static constexpr int kStagingBytes = kDrainWarps * 2 * kStoreBytes;
-    static constexpr int kStagesFit = (225 * 1024 - kStagingBytes) / kStageBytes;
-    static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
-    static constexpr int kAccCols = 2 * BN;
-    static constexpr int kTmemCols = PLANES == 3 ? 2 * kAccCols : kAccCols;
-    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kStagingBytes + 1024 + 256;
-    static_assert(kStages >= 2 && kTmemCols <= 512 && kSmem <= 227 * 1024, "does not fit an SM");
-};
-
-struct Barriers {
-    unsigned long long full[8], empty[8];
-    unsigned long long acc_full[2], acc_empty[2];    // the accumulator (of hh)
-    unsigned long long corr_full[2], corr_empty[2];  // the accumulator of the small products
-    unsigned long long drain;
-    unsigned tmem;
-    int abort;
-};
-
-__device__ unsigned g_gave_up;  // waits that ran out
-
-__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void bar_init(unsigned long long* b, int count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(unsigned long long* b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
-}
-__device__ __forceinline__ void bar_expect(unsigned long long* b, unsigned bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool bar_try(unsigned long long* b, unsigned parity) {
-    unsigned done;
-    asm volatile(
-        "{\n.reg .pred p;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(done)
-        : "r"(smem_u32(b)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-// One lane of a whole warp. The compiler knows what this instruction chooses: what stands behind it is issued once, its
-// operands in uniform registers. Behind "lane == 0" a copy took 150 clocks to issue and an MMA 72.
-__device__ __forceinline__ bool elect_one() {
-    unsigned chosen;
-    asm volatile(
-        "{\n.reg .pred p;\n"
-        "elect.sync _|p, 0xffffffff;\n"
-        "selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(chosen));
-    return chosen != 0;
-}
-__device__ __forceinline__ unsigned long long now_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-// Waits for the phase of `parity` to end. Every wait ends: after kGiveUpNs, or once another warp has given up, the
-// answer is false, and the caller leaves its loop.
-__device__ __noinline__ bool bar_wait_long(unsigned long long* b, unsigned parity, volatile int* abort) {
-    const unsigned long long start = now_ns();
-    while (now_ns() - start < kGiveUpNs) {
-        for (int i = 0; i < 64; ++i)
-            if (bar_try(b, parity)) return true;
-        if (*abort) return false;
-    }
-    *abort = 1;
-    atomicAdd(&g_gave_up, 1u);
-    return false;
-}
-__device__ __forceinline__ bool bar_wait(unsigned long long* b, unsigned parity, volatile int* abort) {
-    for (int i = 0; i < 16; ++i)
-        if (bar_try(b, parity)) return true;
-    return bar_wait_long(b, parity, abort);
-}
-__device__ __forceinline__ void tma_load(const CUtensorMap* map, unsigned dst, unsigned long long* bar, int x, int y,
-                                         int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
-        : "memory");
-}
-__device__ __forceinline__ void tma_store(const CUtensorMap* map, unsigned src, int x, int y, int z) {
-    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(src),
-                 "r"(x), "r"(y), "r"(z)
-                 : "memory");
-}
-__device__ __forceinline__ void mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, bool add) {
-    asm volatile(
-        "{\n.reg .pred p;\n"
-        "setp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((unsigned)add)
-        : "memory");
-}
-__device__ __forceinline__ void mma_commit(unsigned long long* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// 16 columns of the warp's 32 lanes
-__device__ __forceinline__ void tmem_load16(unsigned addr, float (&v)[16]) {
-    unsigned u[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-        "[%16];\n"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
-          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
-        : "r"(addr)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(u[i]);
-}
-
-template <int N>
-__device__ __forceinline__ void tmem_load(unsigned addr, float (&v)[N]) {
-#pragma unroll
-    for (int j = 0; j < N; j += 16) {
-        float u[16];
-        tmem_load16(addr + j, u);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[j + i] = u[i];
-    }
-}
-
-// Shared-memory matrix descriptor, 128-byte swizzle. K-major: rows of 128 bytes, 8-row groups 1024 bytes apart, a
-// 16-deep step is 32 bytes on. MN-major: 64-wide boxes (8 KB each) of 64 rows of the depth, 8-row groups 1024 bytes
-// apart, a 16-deep step is 16 rows on.
-__device__ __forceinline__ unsigned long long smem_desc(unsigned addr, bool mn) {
-    const unsigned long long lead = mn ? 8192 >> 4 : 1, stride = 1024 >> 4;
-    return (unsigned long long)((addr & 0x3ffff) >> 4) | lead << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
-}
-
-// The fields of the problem that the loops use, in registers. Read from the parameter itself they are fetched again after
-// every asm statement, since its address is taken for the tensor maps: the producer's loop took 320 ns per block that way.
-struct Fields {
-    int rows, cols, tiles, tiles_c, kper, kblocks, units, act;
-    bool has_bias, has_residual, vec, tma_out;
-    const void* bias;
-    const void* residual;
-    void* out;
-    void* tape;
-    float* part;
-    __device__ __forceinline__ explicit Fields(const GemmProblem& g)
-        : rows(g.rows), cols(g.cols), tiles(g.tiles_r * g.tiles_c), tiles_c(g.tiles_c), kper(g.kper), kblocks(g.kblocks),
-          units(g.units), act(g.act), has_bias(g.has_bias), has_residual(g.has_residual), vec(g.vec), tma_out(g.tma_out),
-          bias(g.bias), residual(g.residual), out(g.out), tape(g.tape), part(g.part) {}
-};
-
-// One unit of work: a tile of C and a slice of the depth.
-struct Unit {
-    int r0, c0, kb0, kbs, split;  // first row and column, first block and number of blocks of the slice
-};
-template <int BN>
-__device__ __forceinline__ Unit unit_at(const Fields& f, int u) {
-    Unit t;
-    t.split = u / f.tiles;
-    u -= t.split * f.tiles;
-    t.r0 = u / f.tiles_c;  // columns run fastest, so that neighbouring CTAs share P
-    t.c0 = (u - t.r0 * f.tiles_c) * BN;
-    t.r0 *= kTileR;
-    t.kb0 = t.split * f.kper;
-    t.kbs = min(f.kper, f.kblocks - t.kb0);
-    return t;
-}
-
-// N values of a row of IO elements from column c on. Row and column are held inside the matrix, so that every load is good
-// by itself, whether or not its value is wanted; what lies behind the edge is never stored.
-template <typename IO, int N>
-__device__ __forceinline__ void load_row(const void* base, size_t row, int c, int cols, bool vec, float (&v)[N]) {
-    const IO* p = static_cast<const IO*>(base) + row * cols;
-    if (vec && c + N <= cols) {
-        const uint4* q = reinterpret_cast<const uint4*>(p + c);
-#pragma unroll
-        for (int i = 0; i < N * (int)sizeof(IO) / 16; ++i) {
-            const uint4 w = q[i];
-            const unsigned u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if constexpr (sizeof(IO) == 4) {
-                    v[4 * i + k] = __uint_as_float(u[k]);
-                } else {
-                    v[8 * i + 2 * k] = __uint_as_float(u[k] << 16);
-                    v[8 * i + 2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
-                }
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = as_float(p[min(c + i, cols - 1)]);
-    }
-}
-
-// 64 bytes of this lane's row as words; T: float, __nv_bfloat16, or __half for the tape
-template <typename T, int N>
-__device__ __forceinline__ void pack_row(const float (&v)[N], unsigned (&u)[16]) {
-    static_assert(N * sizeof(T) == 64, "a staged row");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        if constexpr (sizeof(T) == 4) {
-            u[i] = __float_as_uint(v[i]);
-        } else if constexpr (std::is_same_v<T, __half>) {
-            u[i] = (unsigned)__half_as_ushort(tape_half(v[2 * i])) | (unsigned)__half_as_ushort(tape_half(v[2 * i + 1])) << 16;
-        } else {
-            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-        }
-    }
-}
-
-// A warp's way from its registers to 32 rows of a matrix in global memory: two 2 KB pieces of shared memory in turn, rows
-// of 64 bytes, 16-byte words swizzled by the row (the 64-byte swizzle of a tensor map), so that lanes meet no bank twice.
-struct Store {
-    char* buf;
-    unsigned flip;
-    bool leader;  // the lane that issues the copies and waits for them
-    __device__ __forceinline__ char* next() {
-        // all but the latest store have been read out of shared memory: the piece of the one before that is free
-        if (leader) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-        __syncwarp();
-        char* b = buf + flip * kStoreBytes;
-        flip ^= 1;
-        return b;
-    }
-    // N elements per lane, rows r .. r + 31, columns c .. c + N - 1 of slice z; `size` rows by `cols`
-    template <typename T, int N>
-    __device__ __forceinline__ void operator()(const CUtensorMap* map, void* out, bool tma, const float (&v)[N], long r,
-                                               int c, int z, int rows, int cols) {
-        const int lane = threadIdx.x % 32;
-        char* b = next();
-        unsigned u[16];
-        pack_row<T>(v, u);
-        uint4* row = reinterpret_cast<uint4*>(b + lane * 64);
-        const int x = lane >> 1 & 3;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) row[i ^ x] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
-        if (tma) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (leader) {
-                if (r < rows && c < cols) tma_store(map, smem_u32(b), c, (int)r, z);
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            }
-        } else {
-            __syncwarp();
-            T* at = static_cast<T*>(out) + (size_t)z * rows * cols;
-            constexpr int kRows = 32 / N;  // rows of one pass of the warp
-            const int j = lane % N;
-#pragma unroll 8
-            for (int i = lane / N; i < 32; i += kRows) {
-                const T e = *reinterpret_cast<const T*>(b + i * 64 + ((j * (int)sizeof(T) / 16) ^ (i >> 1 & 3)) * 16 +
-                                                        j * (int)sizeof(T) % 16);
-                if (r + i < rows && c + j < cols) at[(size_t)(r + i) * cols + c + j] = e;
-            }
-            __syncwarp();
-        }
-    }
-};
-
-// The epilogue of one piece: N sums per lane, which has row r + lane, from column c on. bias: lane i has that of column
-// c + i; q: the residual.
-template <typename IO, int N>
-__device__ __forceinline__ void write_out(const GemmProblem& g, const Fields& f, Store& store, long r, int c, float bias,
-                                          const float (&q)[N], float (&v)[N]) {
-    if (f.has_bias) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += __shfl_sync(~0u, bias, i);
-    }
-    if (f.tape) {
-        using T = std::conditional_t<sizeof(IO) == 2, __half, float>;
-        store.operator()<T>(&g.tape_map, f.tape, f.tma_out, v, r, c, 0, f.rows, f.cols);
-    }
-    if (f.act) activate_all<sizeof(IO) == 2>(v, f.act);
-    if (f.has_residual) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += q[i];
-    }
-    store.operator()<IO>(&g.out_map, f.out, f.tma_out, v, r, c, 0, f.rows, f.cols);
-}
-
-template <int BN, int PLANES>
-__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmProblem g) {
-    using S = Shape<BN, PLANES>;
-    using IO = std::conditional_t<PLANES == 3, float, __nv_bfloat16>;
-    extern __shared__ char raw[];
-    char* stages = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
-    char* staging = stages + (size_t)S::kStages * S::kStageBytes;
-    Barriers& bars = *reinterpret_cast<Barriers*>(staging + S::kStagingBytes);
-    static_assert(sizeof(Barriers) <= 256, "barriers");
-    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
-    volatile int* abort = &bars.abort;
-    const Fields f(g);
-    if (threadIdx.x == 32) {
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&g.p_map) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&g.q_map) : "memory");
-        if (f.tma_out) asm volatile("prefetch.tensormap [%0];" ::"l"(&g.out_map) : "memory");
-    }
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < S::kStages; ++i) bar_init(&bars.full[i], 2), bar_init(&bars.empty[i], 1);
-        for (int i = 0; i < 2; ++i) {
-            bar_init(&bars.acc_full[i], 1), bar_init(&bars.acc_empty[i], kDrainWarps);
-            bar_init(&bars.corr_full[i], 1), bar_init(&bars.corr_empty[i], kDrainWarps);
-        }
-        bar_init(&bars.drain, 1);
-        bars.abort = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)),
-                     "n"(S::kTmemCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    fence_before();
-    __syncthreads();
-    fence_after();
-    const unsigned tmem = bars.tmem, corr_base = tmem + S::kAccCols;
-    after_previous();
-
-    if (warp == 0 || warp == kQWarp) {
-        if (elect_one()) {
-            // an operand's copies: K-major, one box of a tile's rows; MN-major, boxes 64 wide, 8 KB each
-            const bool is_p = warp == 0;
-            const CUtensorMap* map = is_p ? &g.p_map : &g.q_map;
-            const int boxes = is_p ? g.p_boxes : g.q_boxes;
-            const bool mn = is_p ? g.p_mn : g.q_mn;
-            const unsigned bytes = PLANES * boxes * (is_p ? g.p_box_bytes : g.q_box_bytes);
-            const unsigned base = smem_u32(stages) + (is_p ? 0 : PLANES * S::kABytes);
-            const unsigned plane = is_p ? S::kABytes : S::kBBytes;
-            int stage = 0;
-            unsigned phase = 0, issued = 0;
-            bool ok = true;
-            for (int u = blockIdx.x; ok && u < f.units; u += gridDim.x) {
-                const Unit t = unit_at<BN>(f, u);
-                const int row = is_p ? t.r0 : t.c0;
-                for (int k = t.kb0 * kBK; k < (t.kb0 + t.kbs) * kBK; k += kBK) {
-                    ok = bar_wait(&bars.empty[stage], phase ^ 1, abort);
-                    if (!ok) break;
-                    unsigned long long* bar = &bars.full[stage];
-                    bar_expect(bar, bytes);
-                    unsigned dst = base + stage * S::kStageBytes;
-#pragma unroll
-                    for (int p = 0; p < PLANES; ++p, dst += plane) {
-                        if (mn) {
-                            for (int b = 0; b < boxes; ++b) tma_load(map, dst + b * 8192, bar, row + b * 64, k, p);
-                        } else {
-                            tma_load(map, dst, bar, k, row, p);
-                        }
-                    }
-                    ++issued;
-                    if (++stage == S::kStages) stage = 0, phase ^= 1;
-                }
-            }
-            if (!ok) {  // the copies still in flight write to this CTA's shared memory: see them land before it is given up
-                for (unsigned n = 0; n < S::kStages && n < issued; ++n) {
-                    if (--stage < 0) stage = S::kStages - 1, phase ^= 1;
-                    for (int i = 0; i < (1 << 20) && !bar_try(&bars.full[stage], phase); ++i) {
-                    }
-                }
-            }
-        }
-    } else if (warp == 1) {
-        if (elect_one()) {
-            int stage = 0, acc = 0, corr = 0;
-            unsigned phase = 0, acc_phase = 0, corr_phase = 0;
-            bool ok = true;
-            const bool p_mn = g.p_mn, q_mn = g.q_mn;
-            // D float32, A and B bfloat16, which of them MN-major, N / 8, M / 16
-            const unsigned idesc = 1u << 4 | 1u << 7 | 1u << 10 | (unsigned)p_mn << 15 | (unsigned)q_mn << 16 |
-                                   (BN / 8) << 17 | (kTileR / 16) << 24;
-            const unsigned a_step = p_mn ? 2048 >> 4 : 32 >> 4, b_step = q_mn ? 2048 >> 4 : 32 >> 4;
-            const unsigned long long a_desc = smem_desc(smem_u32(stages), p_mn);
-            const unsigned long long b_desc = smem_desc(smem_u32(stages) + PLANES * S::kABytes, q_mn);
-            for (int u = blockIdx.x; ok && u < f.units; u += gridDim.x) {
-                const Unit t = unit_at<BN>(f, u);
-                if (PLANES == 3) {
-                    ok = bar_wait(&bars.corr_empty[corr], corr_phase ^ 1, abort);
-                    if (!ok) break;
-                }
-                for (int kb = 0; kb < t.kbs; ++kb) {
-                    const bool opens = PLANES == 3 ? kb % kChunk == 0 : kb == 0;
-                    if (opens) {
-                        ok = bar_wait(&bars.acc_empty[acc], acc_phase ^ 1, abort);
-                        if (!ok) break;
-                    }
-                    ok = bar_wait(&bars.full[stage], phase, abort);
-                    if (!ok) break;
-                    fence_after();
-                    const unsigned long long da = a_desc + stage * (S::kStageBytes >> 4);
-                    const unsigned long long db = b_desc + stage * (S::kStageBytes >> 4);
-                    const unsigned d = tmem + acc * BN;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) mma(d, da + k * a_step, db + k * b_step, idesc, !(opens && k == 0));
-                    if constexpr (PLANES == 3) {
-                        const unsigned dc = corr_base + corr * BN;
-                        constexpr int kA = S::kABytes >> 4, kB = S::kBBytes >> 4;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const unsigned long long ak = da + k * a_step, bk = db + k * b_step;
-                            mma(dc, ak + 2 * kA, bk, idesc, !(kb == 0 && k == 0));
-                            mma(dc, ak, bk + 2 * kB, idesc, true);
-                            mma(dc, ak + kA, bk + kB, idesc, true);
-                            mma(dc, ak + kA, bk, idesc, true);
-                            mma(dc, ak, bk + kB, idesc, true);
-                        }
-                    }
-                    mma_commit(&bars.empty[stage]);
-                    if (++stage == S::kStages) stage = 0, phase ^= 1;
-                    if (PLANES == 3 ? (kb % kChunk == kChunk - 1 || kb == t.kbs - 1) : kb == t.kbs - 1) {
-                        mma_commit(&bars.acc_full[acc]);
-                        if (++acc == 2) acc = 0, acc_phase ^= 1;
-                    }
-                }
-                if (ok && PLANES == 3) {
-                    mma_commit(&bars.corr_full[corr]);
-                    if (++corr == 2) corr = 0, corr_phase ^= 1;
-                }
-            }
-            if (!ok) {  // products still running write to the tensor memory that is freed below
-                mma_commit(&bars.drain);
-                for (int i = 0; i < (1 << 20) && !bar_try(&bars.drain, 0); ++i) {
-                }
-            }
-        }
-    } else {
-        // a warp reads the 32 lanes of its number mod 4; two warps share them, half of the columns each
-        const int quad = warp % 4, half = (warp - 2) / 4;
-        const unsigned lanes = (unsigned)(quad * 32) << 16;
-        Store store{staging + (warp - 2) * 2 * kStoreBytes, 0, elect_one()};
-        int acc = 0, corr = 0;
-        unsigned acc_phase = 0, corr_phase = 0;
-        bool ok = true;
-        for (int u = blockIdx.x; ok && u < f.units; u += gridDim.x) {
-            const Unit t = unit_at<BN>(f, u);
-            const int c0 = t.c0 + half * (BN / 2);
-            const long r0 = t.r0 + quad * 32;
-            const size_t row = (size_t)min(r0 + lane, f.rows - 1L);
-            if constexpr (PLANES == 1) {
-                constexpr int N = 32;
-                float q[N], bias = 0.f;
-                if (f.has_bias) bias = as_float(static_cast<const IO*>(f.bias)[min(c0 + lane, f.cols - 1)]);
-                if (f.has_residual) load_row<IO, N>(f.residual, row, min(c0, f.cols - 1), f.cols, f.vec, q);
-                ok = bar_wait(&bars.acc_full[acc], acc_phase, abort);
-                ok = __all_sync(~0u, ok);
-                if (!ok) break;
-                fence_after();
-                const unsigned from = tmem + lanes + acc * BN + half * (BN / 2);
-                if (f.part) {
-#pragma unroll 1
-                    for (int j = 0; j < BN / 2; j += 16) {
-                        float v[16];
-                        __syncwarp();
-                        tmem_load<16>(from + j, v);
-                        if (j + 16 == BN / 2) {
-                            fence_before();
-                            if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
-                        }
-                        store.operator()<float>(&g.out_map, f.part, f.tma_out, v, r0, c0 + j, t.split, f.rows, f.cols);
-                    }
-                } else {
-#pragma unroll 1
-                    for (int j = 0; j < BN / 2; j += N) {
-                        float v[N], next[N], next_bias = 0.f;
-                        __syncwarp();
-                        tmem_load<N>(from + j, v);
-                        if (j + N == BN / 2) {
-                            fence_before();
-                            if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
-                        } else {
-                            if (f.has_bias) next_bias = as_float(static_cast<const IO*>(f.bias)[min(c0 + j + N + lane, f.cols - 1)]);
-                            if (f.has_residual)
-                                load_row<IO, N>(f.residual, row, min(c0 + j + N, f.cols - 1), f.cols, f.vec, next);
-                        }
-                        write_out<IO, N>(g, f, store, r0, c0 + j, bias, q, v);
-                        bias = next_bias;
-#pragma unroll
-                        for (int i = 0; i < N; ++i) q[i] = next[i];
-                    }
-                }
-                if (++acc == 2) acc = 0, acc_phase ^= 1;
-            } else {
-                float sum[BN / 2], bias[BN / 32];  // of 16 columns each, in the lower lanes
-#pragma unroll
-                for (int j = 0; j < BN / 32; ++j) {
-                    bias[j] = 0.f;
-                    if (f.has_bias) bias[j] = as_float(static_cast<const IO*>(f.bias)[min(c0 + 16 * j + lane, f.cols - 1)]);
-                }
-#pragma unroll
-                for (int j = 0; j < BN / 2; ++j) sum[j] = 0.f;
-                for (int kb = 0; kb < t.kbs; kb += kChunk) {
-                    ok = bar_wait(&bars.acc_full[acc], acc_phase, abort);
-                    ok = __all_sync(~0u, ok);
-                    if (!ok) break;
-                    fence_after();
-#pragma unroll
-                    for (int j = 0; j < BN / 2; j += 16) {
-                        float v[16];
-                        tmem_load<16>(tmem + lanes + acc * BN + half * (BN / 2) + j, v);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) sum[j + i] += v[i];
-                    }
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
-                    if (++acc == 2) acc = 0, acc_phase ^= 1;
-                }
-                if (!ok) break;
-                ok = bar_wait(&bars.corr_full[corr], corr_phase, abort);
-                ok = __all_sync(~0u, ok);
-                if (!ok) break;
-                fence_after();
-#pragma unroll
-                for (int j = 0; j < BN / 2; j += 16) {
-                    float q[16], v[16];
-                    if (f.has_residual) load_row<IO, 16>(f.residual, row, min(c0 + j, f.cols - 1), f.cols, f.vec, q);
-                    __syncwarp();
-                    tmem_load<16>(corr_base + lanes + corr * BN + half * (BN / 2) + j, v);
-                    if (j + 16 == BN / 2) {
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(&bars.corr_empty[corr]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = isfinite(sum[j + i]) ? sum[j + i] + v[i] : sum[j + i];
-                    if (f.part)
-                        store.operator()<float>(&g.out_map, f.part, f.tma_out, v, r0, c0 + j, t.split, f.rows, f.cols);
-                    else
-                        write_out<IO, 16>(g, f, store, r0, c0 + j, bias[j / 16], q, v);
-                }
-                if (++corr == 2) corr = 0, corr_phase ^= 1;
-            }
-        }
-        // shared memory is given up once every store has read its piece
-        if (store.leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-    }
-    __syncwarp();
-    fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::kTmemCols) : "memory");
-    }
-}
+constexpr int kDepth = 64;     // of a stage
+constexpr int kTileRows = 128;
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -618,19 +47,9 @@ bool make_map(CUtensorMap* map, const void* base, int el, long inner, long outer
 bool bind_operand(CUtensorMap* map, const Operand& o, int planes, int tile, int rows, int* boxes, int* box_bytes) {
     const int need = rows < tile ? (rows + 7) / 8 * 8 : tile;
     *boxes = o.mn_major ? (need + 63) / 64 : 1;
-    const int outer = o.mn_major ? kBK : need;
+    const int outer = o.mn_major ? kDepth : need;
     *box_bytes = outer * 128;
     return make_map(map, o.base, 2, o.inner, o.outer, o.ld, planes, 64, outer, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
-template <int BN, int PLANES>
-cudaError_t launch_shape(const GemmProblem& g, cudaStream_t st) {
-    using S = Shape<BN, PLANES>;
-    static unsigned long long opted = 0;
-    cudaError_t e = opt_in_smem(gemm_kernel<BN, PLANES>, &opted, (int)S::kSmem);
-    if (e != cudaSuccess) return e;
-    const int grid = g.units < kSms ? g.units : kSms;
-    return launch_after(gemm_kernel<BN, PLANES>, grid, kGemmThreads, S::kSmem, st, g);
 }
 
 }  // namespace
@@ -638,7 +57,7 @@ cudaError_t launch_shape(const GemmProblem& g, cudaStream_t st) {
 bool gemm_bind(GemmProblem& g, const Operand& p, const Operand& q, int planes, int bn) {
     g.p_mn = p.mn_major;
     g.q_mn = q.mn_major;
-    if (!bind_operand(&g.p_map, p, planes, kTileR, g.rows, &g.p_boxes, &g.p_box_bytes) ||
+    if (!bind_operand(&g.p_map, p, planes, kTileRows, g.rows, &g.p_boxes, &g.p_box_bytes) ||
         !bind_operand(&g.q_map, q, planes, bn, g.cols, &g.q_boxes, &g.q_box_bytes))
         return false;
     const int el = planes == 3 ? 4 : 2, out_el = g.part ? 4 : el;
@@ -654,18 +73,13 @@ bool gemm_bind(GemmProblem& g, const Operand& p, const Operand& q, int planes, i
 }
 
 cudaError_t launch_gemm(const GemmProblem& g, int planes, int bn, cudaStream_t st) {
-    if (planes == 3) return bn == 128 ? launch_shape<128, 3>(g, st) : launch_shape<64, 3>(g, st);
-    if (bn == 256) return launch_shape<256, 1>(g, st);
-    return bn == 128 ? launch_shape<128, 1>(g, st) : launch_shape<64, 1>(g, st);
+    return planes == 3 ? launch_gemm_f32(g, bn, st) : launch_gemm_bf16(g, bn, st);
 }
 
 cudaError_t gemm_gave_up(unsigned* count, cudaStream_t st) {
-    const unsigned zero = 0;
-    cudaError_t e = cudaMemcpyFromSymbolAsync(count, g_gave_up, sizeof(unsigned), 0, cudaMemcpyDeviceToHost, st);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-    if (e == cudaSuccess && *count) e = cudaMemcpyToSymbolAsync(g_gave_up, &zero, sizeof(unsigned), 0, cudaMemcpyHostToDevice, st);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-    return e;
+    *count = 0;
+    const cudaError_t e = gave_up_bf16(count, st), e2 = gave_up_f32(count, st);
+    return e != cudaSuccess ? e : e2;
 }
 
 }  // namespace qk
