@@ -499,9 +499,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             const Unit t = unit_at<BN>(f, u);
             const int c0 = t.c0 + half * (BN / 2);
             const long r0 = t.r0 + quad * 32;
-            unsigned q[16], next_q[16];
+            unsigned q[2][16];  // residual of this piece and of the next
             float bias = bias_of(c0), next_bias = 0.f;
-            if (f.has_residual) out.fetch<IO>(f, r0, c0, q);
+            if (f.has_residual) out.fetch<IO>(f, r0, c0, q[0]);
             if constexpr (PLANES == 1) {
                 ok = bar_wait(&bars.acc_full[acc], acc_phase, abort);
                 ok = __all_sync(~0u, ok);
@@ -521,22 +521,26 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                         out.store<float>(&g.out_map, f.part, f, v, r0, c0 + j, t.split);
                     }
                 } else {
+                    // two pieces a turn, so that the residuals change places without being moved
+                    constexpr int kTurn = BN / 2 < 2 * N ? 1 : 2;
 #pragma unroll 1
-                    for (int j = 0; j < BN / 2; j += N) {
-                        float v[N];
-                        __syncwarp();
-                        tmem_load<N>(from + j, v);
-                        if (j + N == BN / 2) {
-                            fence_before();
-                            if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
-                        } else {
-                            next_bias = bias_of(c0 + j + N);
-                            if (f.has_residual) out.fetch<IO>(f, r0, c0 + j + N, next_q);
-                        }
-                        write_out<IO, FULL, N>(g, f, out, r0, c0 + j, bias, q, v);
-                        bias = next_bias;
+                    for (int j = 0; j < BN / 2; j += kTurn * N) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) q[i] = next_q[i];
+                        for (int h = 0; h < kTurn; ++h) {
+                            const int at = j + h * N;
+                            float v[N];
+                            __syncwarp();
+                            tmem_load<N>(from + at, v);
+                            if (at + N == BN / 2) {
+                                fence_before();
+                                if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
+                            } else {
+                                next_bias = bias_of(c0 + at + N);
+                                if (f.has_residual) out.fetch<IO>(f, r0, c0 + at + N, q[(h + 1) % 2]);
+                            }
+                            write_out<IO, FULL, N>(g, f, out, r0, c0 + at, bias, q[h], v);
+                            bias = next_bias;
+                        }
                     }
                 }
                 if (++acc == 2) acc = 0, acc_phase ^= 1;
@@ -580,24 +584,26 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 if (++corr == 2) corr = 0, corr_phase ^= 1;
                 // the sums leave sixteen at a time, the others moving up: one copy of the epilogue's code
 #pragma unroll 1
-                for (int j = 0; j < BN / 2; j += 16) {
-                    float v[16];
+                for (int j = 0; j < BN / 2; j += 32) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = sum[i];
+                    for (int h = 0; h < 2; ++h) {
+                        const int at = j + h * 16;
+                        float v[16];
 #pragma unroll
-                    for (int i = 0; i + 16 < BN / 2; ++i) sum[i] = sum[i + 16];
-                    if (f.part) {
-                        out.store<float>(&g.out_map, f.part, f, v, r0, c0 + j, t.split);
-                        continue;
+                        for (int i = 0; i < 16; ++i) v[i] = sum[h * 16 + i];
+                        if (f.part) {
+                            out.store<float>(&g.out_map, f.part, f, v, r0, c0 + at, t.split);
+                            continue;
+                        }
+                        if (at + N < BN / 2) {
+                            next_bias = bias_of(c0 + at + N);
+                            if (f.has_residual) out.fetch<IO>(f, r0, c0 + at + N, q[(h + 1) % 2]);
+                        }
+                        write_out<IO, FULL, 16>(g, f, out, r0, c0 + at, bias, q[h], v);
+                        bias = next_bias;
                     }
-                    if (j + N < BN / 2) {
-                        next_bias = bias_of(c0 + j + N);
-                        if (f.has_residual) out.fetch<IO>(f, r0, c0 + j + N, next_q);
-                    }
-                    write_out<IO, FULL, 16>(g, f, out, r0, c0 + j, bias, q, v);
-                    bias = next_bias;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) q[i] = next_q[i];
+                    for (int i = 0; i + 32 < BN / 2; ++i) sum[i] = sum[i + 32];
                 }
             }
         }

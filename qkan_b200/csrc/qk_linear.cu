@@ -82,16 +82,17 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const PrepArgsL a) {
     const size_t plane = (size_t)j.rows * j.ld;
     float sum[8] = {};
     if (c < j.ld) {
-        const int n = min(8, j.cols - c);
+        const int n = min(8, j.cols - c);  // none in the padding
+        const bool vec = j.vec && n > 0;
 #pragma unroll 2
         for (long r = (long)slab * j.slab_rows + ty; r < end; r += ny) {
             const size_t at = (size_t)r * j.cols + c;
             float v[8];
-            load8<IO>(j.src, at, j.vec, n, v);
+            load8<IO>(j.src, at, vec, n, v);
             if (j.tape) {
                 float z[8];
-                if constexpr (sizeof(IO) == 4) load8<float>(j.tape, at, j.vec, n, z);
-                else load8<__half>(j.tape, at, j.vec, n, z);
+                if constexpr (sizeof(IO) == 4) load8<float>(j.tape, at, vec, n, z);
+                else load8<__half>(j.tape, at, vec, n, z);
                 times_slope<sizeof(IO) == 2>(v, z, j.act);  // columns past the end: 0 times a slope at 0
             }
 #pragma unroll
@@ -234,7 +235,9 @@ Plan plan_for(const Size& s, int planes) {
 
 // ---- scratch -------------------------------------------------------------------
 int planes_of(int io_dtype) { return io_dtype == QK_F32 ? 3 : 1; }
-long padded(long n) { return (n + 7) / 8 * 8; }
+// Packed rows: whole 16-byte words, and 128 bytes at least, which is what a copy takes of them (rows of 32 bytes came
+// 1 to 2 us later)
+long padded(long n) { return n < 64 ? 64 : (n + 7) / 8 * 8; }
 size_t packed_bytes(long rows, long cols, int planes) { return align256((size_t)planes * rows * padded(cols) * 2); }
 int blocks_of(long depth) { return (int)((depth + 63) / 64); }
 
