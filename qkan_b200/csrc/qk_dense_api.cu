@@ -14,6 +14,10 @@ int check_linear(const QkLinearDesc* d) {
     if (d->rows < 0 || d->in_features < 0 || d->out_features < 0)
         return fail(QK_ERR_BAD_ARGUMENT, "negative dimension (rows=%d in=%d out=%d)", d->rows, d->in_features,
                     d->out_features);
+    const int most = 0x7fffff00;  // indices are rounded up to whole tiles in 32 bits
+    if (d->rows > most || d->in_features > most || d->out_features > most)
+        return fail(QK_ERR_UNSUPPORTED, "a dimension exceeds %d (rows=%d in=%d out=%d)", most, d->rows, d->in_features,
+                    d->out_features);
     if (!is_dtype(d->io_dtype)) return fail(QK_ERR_BAD_ARGUMENT, "io_dtype %d is neither QK_F32 nor QK_BF16", d->io_dtype);
     if (d->activation < QK_ACT_NONE || d->activation > QK_ACT_SIGMOID)
         return fail(QK_ERR_BAD_ARGUMENT, "activation %d is not a QkActivation value", d->activation);

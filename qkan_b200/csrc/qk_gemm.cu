@@ -3,8 +3,8 @@
 
 namespace qk {
 
-cudaError_t launch_gemm_bf16(const GemmProblem& g, int bn, cudaStream_t st);
-cudaError_t launch_gemm_f32(const GemmProblem& g, int bn, cudaStream_t st);
+cudaError_t launch_gemm_bf16(const GemmArgs& a, int bn, cudaStream_t st);
+cudaError_t launch_gemm_f32(const GemmArgs& a, int bn, cudaStream_t st);
 cudaError_t gave_up_bf16(unsigned* total, cudaStream_t st);
 cudaError_t gave_up_f32(unsigned* total, cudaStream_t st);
 
@@ -72,8 +72,8 @@ bool gemm_bind(GemmProblem& g, const Operand& p, const Operand& q, int planes, i
     return !g.tape || make_map(&g.tape_map, g.tape, el, g.cols, g.rows, g.cols, 1, 64 / el, 32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-cudaError_t launch_gemm(const GemmProblem& g, int planes, int bn, cudaStream_t st) {
-    return planes == 3 ? launch_gemm_f32(g, bn, st) : launch_gemm_bf16(g, bn, st);
+cudaError_t launch_gemm(const GemmArgs& a, int planes, int bn, cudaStream_t st) {
+    return planes == 3 ? launch_gemm_f32(a, bn, st) : launch_gemm_bf16(a, bn, st);
 }
 
 cudaError_t gemm_gave_up(unsigned* count, cudaStream_t st) {

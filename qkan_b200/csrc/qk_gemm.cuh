@@ -342,7 +342,10 @@ __device__ __forceinline__ void write_out(const GemmProblem& g, const Fields& f,
 }
 
 template <int BN, int PLANES, bool FULL>
-__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmProblem g) {
+__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs a) {
+    const bool second = (int)blockIdx.x >= a.first;
+    const GemmProblem& g = second ? a.g[1] : a.g[0];
+    const int cta = blockIdx.x - (second ? a.first : 0), ctas = second ? a.ctas - a.first : a.first;
     using S = Shape<BN, PLANES>;
     using IO = std::conditional_t<PLANES == 3, float, __nv_bfloat16>;
     extern __shared__ char raw[];
@@ -393,7 +396,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             int stage = 0;
             unsigned phase = 0, issued = 0;
             bool ok = true;
-            for (int u = blockIdx.x; ok && u < f.units; u += gridDim.x) {
+            for (int u = cta; ok && u < f.units; u += ctas) {
                 const Unit t = unit_at<BN>(f, u);
                 const int row = is_p ? t.r0 : t.c0;
                 for (int k = t.kb0 * kBK; k < (t.kb0 + t.kbs) * kBK; k += kBK) {
@@ -434,7 +437,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             const unsigned a_step = p_mn ? 2048 >> 4 : 32 >> 4, b_step = q_mn ? 2048 >> 4 : 32 >> 4;
             const unsigned long long a_desc = smem_desc(smem_u32(stages), p_mn);
             const unsigned long long b_desc = smem_desc(smem_u32(stages) + PLANES * S::kABytes, q_mn);
-            for (int u = blockIdx.x; ok && u < f.units; u += gridDim.x) {
+            for (int u = cta; ok && u < f.units; u += ctas) {
                 const Unit t = unit_at<BN>(f, u);
                 if (PLANES == 3) {
                     ok = bar_wait(&bars.corr_empty[corr], corr_phase ^ 1, abort);
@@ -495,7 +498,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         int acc = 0, corr = 0;
         unsigned acc_phase = 0, corr_phase = 0;
         bool ok = true;
-        for (int u = blockIdx.x; ok && u < f.units; u += gridDim.x) {
+        for (int u = cta; ok && u < f.units; u += ctas) {
             const Unit t = unit_at<BN>(f, u);
             const int c0 = t.c0 + half * (BN / 2);
             const long r0 = t.r0 + quad * 32;
@@ -620,19 +623,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
 }
 
 template <int BN, int PLANES, bool FULL>
-cudaError_t launch_shape(const GemmProblem& g, cudaStream_t st) {
+cudaError_t launch_shape(const GemmArgs& a, cudaStream_t st) {
     using S = Shape<BN, PLANES>;
     static unsigned long long opted = 0;
     cudaError_t e = opt_in_smem(gemm_kernel<BN, PLANES, FULL>, &opted, (int)S::kSmem);
     if (e != cudaSuccess) return e;
-    const int grid = g.units < kSms ? g.units : kSms;
-    return launch_after(gemm_kernel<BN, PLANES, FULL>, grid, kGemmThreads, S::kSmem, st, g);
+    return launch_after(gemm_kernel<BN, PLANES, FULL>, a.ctas, kGemmThreads, S::kSmem, st, a);
 }
 
 template <int BN, int PLANES>
-cudaError_t launch_tile(const GemmProblem& g, cudaStream_t st) {
+cudaError_t launch_tile(const GemmArgs& a, cudaStream_t st) {
+    const GemmProblem& g = a.g[0];  // two problems: gradients, neither has an activation
     const bool full = !g.part && (g.tape || g.act != QK_ACT_NONE);
-    return full ? launch_shape<BN, PLANES, true>(g, st) : launch_shape<BN, PLANES, false>(g, st);
+    return full ? launch_shape<BN, PLANES, true>(a, st) : launch_shape<BN, PLANES, false>(a, st);
 }
 
 // adds this unit's count of waits that ran out, and clears it; synchronises the stream

@@ -4,7 +4,8 @@
 //   prepare   operands that the products cannot read where they lie: float32 is split into three bfloat16 parts, rows
 //             that are no multiple of 16 bytes are padded, and in the backward gz = gy * act'(tape) is formed, with
 //             its column sums for grad_bias on the way
-//   products  forward: one; backward: grad_weight and grad_x
+//   products  forward: one (a few rows: qk_gemv.cu, nothing else); backward: grad_weight and grad_x, in one launch where
+//             both fit the GPU side by side
 //   reduce    adds the slices of a depth that was cut for want of tiles, then the epilogue; adds grad_bias' slabs
 #include "qk_linear.cuh"
 
@@ -220,17 +221,40 @@ double cost_of(const Size& s, int bn, int planes, const Cut& c) {
     return t;
 }
 
-Plan plan_for(const Size& s, int planes) {
+// the cheapest plan, of at most `most_units` units where that is not 0, with tiles of `only_bn` columns where that is not
+Plan plan_for(const Size& s, int planes, double* cost = nullptr, long most_units = 0, int only_bn = 0) {
     Plan best{};
     double least = 1e300;
-    for (int bn = planes == 3 ? 128 : 256; bn >= 64; bn /= 2)
+    for (int bn = planes == 3 ? 128 : 256; bn >= 64; bn /= 2) {
+        if (only_bn && bn != only_bn) continue;
         for (int k : kCuts) {
             if (k > 1 && (k > s.kblocks || s.tiles(bn) * k > 4l * kSms || (double)k * s.rows * s.cols > kMostPart)) break;
             const Cut c = cut_into(s.kblocks, k);
+            if (most_units && s.tiles(bn) * c.splits > most_units) break;
             const double t = cost_of(s, bn, planes, c);
             if (t < least) least = t, best = {bn, c};
         }
+    }
+    if (cost) *cost = least;
     return best;
+}
+
+// Two products in one launch: where both fit the SMs side by side, that costs the longer of the two, not the sum.
+// False: one after the other is cheaper.
+bool plan_pair(const Size& a, const Size& b, int planes, Plan* pa, Plan* pb) {
+    double ca, cb;
+    *pa = plan_for(a, planes, &ca);
+    *pb = plan_for(b, planes, &cb);
+    double least = ca + cb;
+    bool together = false;
+    for (int bn = planes == 3 ? 128 : 256; bn >= 64; bn /= 2)
+        for (int first = kSms / 8; first < kSms; first += kSms / 8) {
+            double ta, tb;
+            const Plan qa = plan_for(a, planes, &ta, first, bn), qb = plan_for(b, planes, &tb, kSms - first, bn);
+            const double t = ta > tb ? ta : tb;
+            if (t < least) least = t, *pa = qa, *pb = qb, together = true;
+        }
+    return together;
 }
 
 // ---- scratch -------------------------------------------------------------------
@@ -281,6 +305,7 @@ ForwardScratch plan_forward(const QkLinearDesc& d) {
 // The layout is that of all gradients, whatever is asked for.
 struct BackwardScratch {
     Plan plan_w, plan_x;
+    bool together;  // both products in one launch
     Slabs slabs;
     size_t gz, x, w, colpart, part_w, part_x, total;
 };
@@ -290,8 +315,7 @@ BackwardScratch plan_backward(const QkLinearDesc& d) {
     const long M = d.rows, K = d.in_features, N = d.out_features;
     const bool pack_gz = d.activation != QK_ACT_NONE || !reads_in_place(N, d.io_dtype);
     const bool pack = !reads_in_place(K, d.io_dtype);
-    s.plan_w = plan_for({N, K, blocks_of(M)}, planes);
-    s.plan_x = plan_for({M, K, blocks_of(N)}, planes);
+    s.together = K > 0 && plan_pair({N, K, blocks_of(M)}, {M, K, blocks_of(N)}, planes, &s.plan_w, &s.plan_x);
     s.slabs = slabs_of(M, N);
     s.gz = 0;
     s.x = pack_gz ? packed_bytes(M, N, planes) : 0;
@@ -369,10 +393,8 @@ Operand operand(const void* base, int rows, int cols, bool packed, bool mn_major
 }
 
 // C (rows, cols) = P Q^T over `depth`, with its epilogue; where the depth is cut, the sums wait in `part` for `red`
-cudaError_t run_product(int rows, int cols, int depth, const Plan& plan, const Operand& p, const Operand& q, float* part,
-                        const Epilogue& epi, ReduceArgs& red, cudaStream_t st) {
-    const int planes = planes_of(epi.io_dtype);
-    GemmProblem g{};
+cudaError_t set_product(GemmProblem& g, int rows, int cols, int depth, const Plan& plan, const Operand& p, const Operand& q,
+                        float* part, const Epilogue& epi, ReduceArgs& red) {
     g.rows = rows, g.cols = cols;
     g.kblocks = blocks_of(depth), g.kper = plan.cut.kper, g.splits = plan.cut.splits;
     g.tiles_r = (rows + 127) / 128, g.tiles_c = (cols + plan.bn - 1) / plan.bn;
@@ -383,15 +405,22 @@ cudaError_t run_product(int rows, int cols, int depth, const Plan& plan, const O
     g.has_bias = epi.bias && !g.part, g.has_residual = epi.residual && !g.part;
     g.bias = g.has_bias ? epi.bias : epi.out, g.residual = g.has_residual ? epi.residual : epi.out;
     g.out = epi.out, g.tape = epi.tape, g.act = epi.act;
-    if (!gemm_bind(g, p, q, planes, plan.bn)) return cudaErrorInvalidValue;
+    if (!gemm_bind(g, p, q, planes_of(epi.io_dtype), plan.bn)) return cudaErrorInvalidValue;
     if (g.splits > 1) add_reduce(red, part, g.splits, rows, cols, epi);
-    return launch_gemm(g, planes, plan.bn, st);
+    return cudaSuccess;
+}
+
+// one of the problems of `a` by itself
+cudaError_t run_alone(GemmArgs& a, int which, int planes, int bn, cudaStream_t st) {
+    if (which) a.g[0] = a.g[1];
+    a.first = a.ctas = a.g[0].units < kSms ? a.g[0].units : kSms;
+    return launch_gemm(a, planes, bn, st);
 }
 
 }  // namespace
 
 size_t linear_forward_scratch(const QkLinearDesc& d) {
-    if (d.rows == 0 || d.out_features == 0 || d.in_features == 0) return 0;
+    if (d.rows <= kGemvRows || d.out_features == 0 || d.in_features == 0) return 0;
     return forward_scratch(d).total;
 }
 
@@ -408,6 +437,7 @@ cudaError_t launch_linear_forward(const LinearArgs& a, cudaStream_t st) {
         add_reduce(red, nullptr, 0, M, N, epi);
         return launch_reduce(red, st);
     }
+    if (M <= kGemvRows) return launch_gemv({M, N, K, a.x, a.w, epi, 0, 0}, st);
     const QkLinearDesc d{M, K, N, a.io_dtype, a.act, 0};
     const ForwardScratch& s = forward_scratch(d);
     char* ws = static_cast<char*>(a.scratch);
@@ -422,8 +452,10 @@ cudaError_t launch_linear_forward(const LinearArgs& a, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         x = ws + s.x, w = ws + s.w;
     }
-    e = run_product(M, N, K, s.plan, operand(x, M, K, pack, false), operand(w, N, K, pack, false),
-                    reinterpret_cast<float*>(ws + s.part), epi, red, st);
+    GemmArgs g{};
+    e = set_product(g.g[0], M, N, K, s.plan, operand(x, M, K, pack, false), operand(w, N, K, pack, false),
+                    reinterpret_cast<float*>(ws + s.part), epi, red);
+    if (e == cudaSuccess) e = run_alone(g, 0, planes_of(a.io_dtype), s.plan.bn, st);
     return e == cudaSuccess ? launch_reduce(red, st) : e;
 }
 
@@ -445,14 +477,21 @@ cudaError_t launch_linear_backward(const LinearArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     const void* gz = pack_gz ? ws + s.gz : a.gy;
     ReduceArgs red{};
+    GemmArgs g{};
+    const int planes = planes_of(a.io_dtype);
     if (a.gw)
-        e = run_product(N, K, M, s.plan_w, operand(gz, M, N, pack_gz, true), operand(pack ? ws + s.x : a.x, M, K, pack, true),
-                        reinterpret_cast<float*>(ws + s.part_w), {nullptr, nullptr, a.gw, nullptr, QK_ACT_NONE, a.io_dtype},
-                        red, st);
+        e = set_product(g.g[0], N, K, M, s.plan_w, operand(gz, M, N, pack_gz, true), operand(pack ? ws + s.x : a.x, M, K, pack, true),
+                        reinterpret_cast<float*>(ws + s.part_w), {nullptr, nullptr, a.gw, nullptr, QK_ACT_NONE, a.io_dtype}, red);
     if (e == cudaSuccess && a.gx)
-        e = run_product(M, K, N, s.plan_x, operand(gz, M, N, pack_gz, false), operand(pack ? ws + s.w : a.w, N, K, pack, true),
-                        reinterpret_cast<float*>(ws + s.part_x), {nullptr, nullptr, a.gx, nullptr, QK_ACT_NONE, a.io_dtype},
-                        red, st);
+        e = set_product(g.g[1], M, K, N, s.plan_x, operand(gz, M, N, pack_gz, false), operand(pack ? ws + s.w : a.w, N, K, pack, true),
+                        reinterpret_cast<float*>(ws + s.part_x), {nullptr, nullptr, a.gx, nullptr, QK_ACT_NONE, a.io_dtype}, red);
+    if (e == cudaSuccess && a.gw && a.gx && s.together) {
+        g.first = g.g[0].units, g.ctas = g.first + g.g[1].units;
+        e = launch_gemm(g, planes, s.plan_w.bn, st);
+    } else {
+        if (e == cudaSuccess && a.gw) e = run_alone(g, 0, planes, s.plan_w.bn, st);
+        if (e == cudaSuccess && a.gx) e = run_alone(g, 1, planes, s.plan_x.bn, st);
+    }
     if (e != cudaSuccess) return e;
     red.colpart = colpart, red.gb = a.gb, red.slabs = s.slabs.count, red.cols = N, red.io_dtype = a.io_dtype;
     return launch_reduce(red, st);

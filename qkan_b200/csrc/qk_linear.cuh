@@ -37,11 +37,28 @@ struct alignas(64) GemmProblem {
     int act;
 };
 
+// One launch: one problem, or two that share the SMs, the first `first` CTAs with g[0].
+struct GemmArgs {
+    GemmProblem g[2];
+    int first, ctas;
+};
+
 // fills in the tensor maps and what goes with them; false: the driver refused one
 bool gemm_bind(GemmProblem& g, const Operand& p, const Operand& q, int planes, int bn);
-cudaError_t launch_gemm(const GemmProblem& g, int planes, int bn, cudaStream_t st);
+cudaError_t launch_gemm(const GemmArgs& a, int planes, int bn, cudaStream_t st);
 // waits that ran out on the current device since the last call; synchronises the stream
 cudaError_t gemm_gave_up(unsigned* count, cudaStream_t st);
+
+// ---- few rows (qk_gemv.cu) -------------------------------------------------------
+constexpr int kGemvRows = 8;
+struct GemvArgs {
+    int rows, cols, depth;
+    const void* x;
+    const void* w;
+    Epilogue epi;
+    int cuts, per;  // filled by the launcher: warps that share the depth, elements of it for each
+};
+cudaError_t launch_gemv(const GemvArgs& a, cudaStream_t st);
 
 // ---- the map (qk_linear.cu) ----------------------------------------------------
 struct LinearArgs {

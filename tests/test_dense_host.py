@@ -35,6 +35,16 @@ def test_linear_descriptors_that_are_refused(fields, text):
     assert lib.qk_linear_backward(dp, one, one, one, one, one, one, one, one, 1 << 30, None) == _abi.QK_ERR_BAD_ARGUMENT
 
 
+def test_dimensions_beyond_the_index_range_are_refused():
+    lib = _lib()
+    for fields in ((2 ** 31 - 1, 1, 1), (1, 2 ** 31 - 1, 1), (1, 1, 2 ** 31 - 1)):
+        dp = _abi.desc_pointer(_abi.QkLinearDesc(*fields, 0, 0, 0))
+        one = ctypes.c_void_p(256)
+        assert lib.qk_linear_forward_workspace_bytes(dp) == 0 and b"exceeds" in lib.qk_last_error()
+        assert lib.qk_linear_forward(dp, one, one, None, None, one, None, one, 1 << 30, None) == _abi.QK_ERR_UNSUPPORTED
+        assert lib.qk_linear_backward(dp, one, one, one, one, one, one, one, one, 1 << 30, None) == _abi.QK_ERR_UNSUPPORTED
+
+
 def test_linear_pointers_and_workspaces_that_are_refused():
     lib = _lib()
     dp = _abi.desc_pointer(_abi.QkLinearDesc(64, 64, 64, _abi.QK_F32, _abi.QK_ACT_SILU, 0))
