@@ -251,8 +251,8 @@ typedef struct QkLinearDesc {
  * y (M,N) = act(x (M,K) weight (N,K)^T + bias (N)) + residual (M,N); bias and residual may be NULL.
  * tape (M,N), NULL when no backward follows or the activation is QK_ACT_NONE: the argument of the activation, for
  * qk_linear_backward. It is float32 for QK_F32 and IEEE half for QK_BF16: three more bits than bfloat16 where the
- * activations bend. A finite value beyond half's range is held at its largest, and one below its smallest at plus or
- * minus that, so that no sign is lost. Products and sums: float32, for QK_F32 to float32 accuracy.
+ * activations bend; beyond half's range it is infinite, where every derivative has its limit, and relu's keeps the sign
+ * of what is below it. Products and sums: float32, for QK_F32 to float32 accuracy.
  * y may not overlap an input. in_features == 0 gives act(bias) + residual.
  */
 size_t qk_linear_forward_workspace_bytes(const QkLinearDesc* desc);

@@ -72,30 +72,38 @@ cudaError_t launch_norm_backward(const NormArgs& a, cudaStream_t st);
 
 // ---- linear map --------------------------------------------------------------
 // act(z) and its derivative in float32, by CUDA's own functions. FAST, for values that are rounded to bfloat16 next: exp
-// and division by the special-function unit (off by some 2^-20 where bfloat16 is off by 2^-9). tanh and erf are the full
-// ones throughout: near zero theirs is a relative error.
+// and the reciprocal by the special-function unit (off by some 2^-20 where bfloat16 is off by 2^-9). tanh and erf are the
+// full ones throughout: near zero theirs is a relative error.
 template <bool FAST>
-__device__ __forceinline__ float over_one_plus_exp(float num, float z) {  // num / (1 + exp(-z))
-    if constexpr (FAST) return __fdividef(num, 1.f + __expf(-z));
-    else return num / (1.f + expf(-z));
+__device__ __forceinline__ float sigmoid_of(float z) {
+    if constexpr (FAST) {
+        float r;
+        asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-z)));
+        return r;
+    } else {
+        return 1.f / (1.f + expf(-z));
+    }
 }
 template <bool FAST>
 __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {
-        case QK_ACT_SILU: return over_one_plus_exp<FAST>(z, z);
+        case QK_ACT_SILU: return FAST ? z * sigmoid_of<FAST>(z) : z / (1.f + expf(-z));
         case QK_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
         case QK_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(0.79788456080286536f * fmaf(0.044715f * z * z, z, z)));
         case QK_ACT_RELU: return z < 0.f ? 0.f : z;  // a NaN stays one
         case QK_ACT_TANH: return tanhf(z);
-        case QK_ACT_SIGMOID: return over_one_plus_exp<FAST>(1.f, z);
+        case QK_ACT_SIGMOID: return sigmoid_of<FAST>(z);
         default: return z;
     }
 }
+// Beyond +-10^4 every derivative has reached its limit, which is what an infinite z (and one that the tape holds as such)
+// gets; a NaN passes.
 template <bool FAST>
 __device__ __forceinline__ float act_slope(float z, int act) {
+    asm("{max.NaN.f32 %0, %0, %1;\n min.NaN.f32 %0, %0, %2;}" : "+f"(z) : "f"(-1e4f), "f"(1e4f));
     switch (act) {
         case QK_ACT_SILU: {
-            const float s = over_one_plus_exp<FAST>(1.f, z);
+            const float s = sigmoid_of<FAST>(z);
             return s * fmaf(z, 1.f - s, 1.f);
         }
         case QK_ACT_GELU: {
@@ -113,7 +121,7 @@ __device__ __forceinline__ float act_slope(float z, int act) {
             return 1.f - t * t;
         }
         case QK_ACT_SIGMOID: {
-            const float s = over_one_plus_exp<FAST>(1.f, z);
+            const float s = sigmoid_of<FAST>(z);
             return s * (1.f - s);
         }
         default: return 1.f;
@@ -156,19 +164,15 @@ __device__ __forceinline__ void times_slope(float (&v)[N], const float (&z)[N], 
 }
 
 // The tape: float32, or half for bfloat16 activations. Rounding an argument of the activation to half moves it by at
-// most 2^-12 of itself (2^-9 in bfloat16). What half cannot hold keeps its sign: beyond +-65504 every derivative here
-// has reached its limit, and below half's smallest number the value is stored as that (relu asks for z > 0 only).
-__device__ __forceinline__ __half tape_half(float z) {
-    if (fabsf(z) <= 65504.f || z != z) {
-        const __half h = __float2half_rn(z);
-        if (z != 0.f && __half2float(h) == 0.f) return __ushort_as_half(z < 0.f ? 0x8001 : 0x0001);
-        return h;
-    }
-    if (isinf(z)) return __float2half_rn(z);
-    return __float2half_rn(copysignf(65504.f, z));
+// most 2^-12 of itself (2^-9 in bfloat16). What is beyond half's range becomes infinite, where the derivatives have their
+// limits; what is below it becomes zero, which matters to relu alone: its tape keeps the sign as half's smallest number.
+__device__ __forceinline__ __half tape_half(float z, int act) {
+    const __half h = __float2half_rn(z);
+    if (act == QK_ACT_RELU && z != 0.f && __half2float(h) == 0.f) return __ushort_as_half(z < 0.f ? 0x8001 : 0x0001);
+    return h;
 }
-__device__ __forceinline__ void store_tape(void* tape, size_t i, int io_dtype, float z) {
-    if (io_dtype == QK_BF16) static_cast<__half*>(tape)[i] = tape_half(z);
+__device__ __forceinline__ void store_tape(void* tape, size_t i, int io_dtype, float z, int act) {
+    if (io_dtype == QK_BF16) static_cast<__half*>(tape)[i] = tape_half(z, act);
     else static_cast<float*>(tape)[i] = z;
 }
 __device__ __forceinline__ float load_tape(const void* tape, size_t i, int io_dtype) {
@@ -186,7 +190,7 @@ struct Epilogue {
 __device__ __forceinline__ void finish_element(const Epilogue& e, size_t at, int c, float acc) {
     float z = acc;
     if (e.bias) z += load_dt(e.bias, c, e.io_dtype);
-    if (e.tape) store_tape(e.tape, at, e.io_dtype, z);
+    if (e.tape) store_tape(e.tape, at, e.io_dtype, z, e.act);
     float y = e.io_dtype == QK_BF16 ? activate<true>(z, e.act) : activate<false>(z, e.act);
     if (e.residual) y += load_dt(e.residual, at, e.io_dtype);
     store_dt(e.out, at, e.io_dtype, y);

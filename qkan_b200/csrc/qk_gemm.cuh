@@ -240,7 +240,7 @@ __device__ __forceinline__ void pack_row(const float (&v)[N], unsigned (&u)[16])
         if constexpr (sizeof(T) == 4) {
             u[i] = __float_as_uint(v[i]);
         } else if constexpr (std::is_same_v<T, __half>) {
-            u[i] = (unsigned)__half_as_ushort(tape_half(v[2 * i])) | (unsigned)__half_as_ushort(tape_half(v[2 * i + 1])) << 16;
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
         } else {
             asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
         }
@@ -260,14 +260,18 @@ struct Stage {
         flip ^= 1;
         return b;
     }
-    // N elements per lane to rows r .. r + 31, columns c .. c + N - 1, of slice z
+    // N elements per lane, by way of piece b, to rows r .. r + 31, columns c .. c + N - 1, of slice z
     template <typename T, int N>
-    __device__ __forceinline__ void store(const CUtensorMap* map, void* out, const Fields& f, const float (&v)[N], long r,
-                                          int c, int z) {
-        const int lane = threadIdx.x % 32;
-        char* b = next();
+    __device__ __forceinline__ void store(char* b, const CUtensorMap* map, void* out, const Fields& f, const float (&v)[N],
+                                          long r, int c, int z) {
         unsigned u[16];
         pack_row<T>(v, u);
+        store_words<T>(b, map, out, f, u, r, c, z);
+    }
+    template <typename T>
+    __device__ __forceinline__ void store_words(char* b, const CUtensorMap* map, void* out, const Fields& f,
+                                                const unsigned (&u)[16], long r, int c, int z) {
+        const int lane = threadIdx.x % 32;
         uint4* row = reinterpret_cast<uint4*>(b + lane * 64);
         const int x = lane >> 1 & 3;
 #pragma unroll
@@ -285,29 +289,53 @@ struct Stage {
             __syncwarp();
         }
     }
-    // 64 bytes of the residual from column c on for each lane, which has row r + lane; behind the matrix' edge anything
+};
+
+// 32 rows of 64 bytes of the residual on their way: four lanes to a row, so that a load meets 8 lines and not 32 (with a
+// row per lane the loads of a 128 x 128 tile took 2000 clocks). Rows are held inside the matrix, whole pieces only: what
+// a ragged edge cuts is fetched when it is needed.
+struct Ahead {
+    uint4 w[4];
     template <typename T>
-    __device__ __forceinline__ void fetch(const Fields& f, long r, int c, unsigned (&u)[16]) {
+    __device__ __forceinline__ void fetch(const Fields& f, long r, int c) {
         const int lane = threadIdx.x % 32;
-        const T* from = static_cast<const T*>(f.residual);
-        uint4 w[4];
-        if (f.vec && c + 64 / (int)sizeof(T) <= f.cols) {
-            const uint4* row = reinterpret_cast<const uint4*>(from + (size_t)min(r + lane, f.rows - 1L) * f.cols + c);
+        if (!f.vec || c + 64 / (int)sizeof(T) > f.cols) return;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = row[i];
-        } else {
-            char* b = next();
-            copy_in<T>(b, from, r, c, f.rows, f.cols);
-            __syncwarp();
-            const uint4* row = reinterpret_cast<const uint4*>(b + lane * 64);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = row[i ^ (lane >> 1 & 3)];
-            __syncwarp();
-            // an empty group in this piece's turn: next() counts groups, one for each piece that was taken
-            if (leader) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        for (int i = 0; i < 4; ++i) {
+            const long row = min(r + 8 * i + lane / 4, f.rows - 1L);
+            w[i] = reinterpret_cast<const uint4*>(static_cast<const T*>(f.residual) + (size_t)row * f.cols + c)[lane % 4];
         }
+    }
+    // adds them to v, lane by lane a row, by way of piece b
+    template <typename T, int N>
+    __device__ __forceinline__ void add(char* b, const Fields& f, long r, int c, float (&v)[N]) {
+        const int lane = threadIdx.x % 32;
+        if (!f.vec || c + N > f.cols) {
+            copy_in<T>(b, static_cast<const T*>(f.residual), r, c, f.rows, f.cols);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[4 * i] = w[i].x, u[4 * i + 1] = w[i].y, u[4 * i + 2] = w[i].z, u[4 * i + 3] = w[i].w;
+            for (int i = 0; i < 4; ++i) {
+                const int row = 8 * i + lane / 4;
+                reinterpret_cast<uint4*>(b + row * 64)[lane % 4 ^ (row >> 1 & 3)] = w[i];
+            }
+        }
+        __syncwarp();
+        const uint4* own = reinterpret_cast<const uint4*>(b + lane * 64);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 q = own[i ^ (lane >> 1 & 3)];
+            const unsigned u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (sizeof(T) == 4) {
+                    v[4 * i + k] += __uint_as_float(u[k]);
+                } else {
+                    v[8 * i + 2 * k] += __uint_as_float(u[k] << 16);
+                    v[8 * i + 2 * k + 1] += __uint_as_float(u[k] & 0xffff0000u);
+                }
+            }
+        }
+        // a lane writes its own row of the piece next, and no other one's: no barrier
     }
 };
 
@@ -315,30 +343,30 @@ struct Stage {
 // c + i; q: the residual. FULL: with activation and tape.
 template <typename IO, bool FULL, int N>
 __device__ __forceinline__ void write_out(const GemmProblem& g, const Fields& f, Stage& stage, long r, int c, float bias,
-                                          const unsigned (&q)[16], float (&v)[N]) {
+                                          Ahead& q, float (&v)[N]) {
     if (f.has_bias) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] += __shfl_sync(~0u, bias, i);
     }
     if constexpr (FULL) {
         if (f.tape) {
-            using T = std::conditional_t<sizeof(IO) == 2, __half, float>;
-            stage.store<T>(&g.tape_map, f.tape, f, v, r, c, 0);
+            char* b = stage.next();
+            if (sizeof(IO) == 2 && f.act == QK_ACT_RELU) {
+                unsigned u[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    u[i] = (unsigned)__half_as_ushort(tape_half(v[2 * i % N], f.act)) |
+                           (unsigned)__half_as_ushort(tape_half(v[(2 * i + 1) % N], f.act)) << 16;
+                stage.store_words<__half>(b, &g.tape_map, f.tape, f, u, r, c, 0);
+            } else {
+                stage.store<std::conditional_t<sizeof(IO) == 2, __half, float>>(b, &g.tape_map, f.tape, f, v, r, c, 0);
+            }
         }
         activate_all<sizeof(IO) == 2>(v, f.act);
     }
-    if (f.has_residual) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if constexpr (sizeof(IO) == 4) {
-                v[i] += __uint_as_float(q[i]);
-            } else {
-                v[2 * i] += __uint_as_float(q[i] << 16);
-                v[2 * i + 1] += __uint_as_float(q[i] & 0xffff0000u);
-            }
-        }
-    }
-    stage.store<IO>(&g.out_map, f.out, f, v, r, c, 0);
+    char* b = stage.next();
+    if (f.has_residual) q.add<IO>(b, f, r, c, v);
+    stage.store<IO>(b, &g.out_map, f.out, f, v, r, c, 0);
 }
 
 template <int BN, int PLANES, bool FULL>
@@ -502,9 +530,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             const Unit t = unit_at<BN>(f, u);
             const int c0 = t.c0 + half * (BN / 2);
             const long r0 = t.r0 + quad * 32;
-            unsigned q[2][16];  // residual of this piece and of the next
+            Ahead q[2];  // residual of this piece and of the next
             float bias = bias_of(c0), next_bias = 0.f;
-            if (f.has_residual) out.fetch<IO>(f, r0, c0, q[0]);
+            if (f.has_residual) q[0].fetch<IO>(f, r0, c0);
             if constexpr (PLANES == 1) {
                 ok = bar_wait(&bars.acc_full[acc], acc_phase, abort);
                 ok = __all_sync(~0u, ok);
@@ -521,7 +549,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                             fence_before();
                             if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
                         }
-                        out.store<float>(&g.out_map, f.part, f, v, r0, c0 + j, t.split);
+                        out.store<float>(out.next(), &g.out_map, f.part, f, v, r0, c0 + j, t.split);
                     }
                 } else {
                     // two pieces a turn, so that the residuals change places without being moved
@@ -539,7 +567,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                                 if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
                             } else {
                                 next_bias = bias_of(c0 + at + N);
-                                if (f.has_residual) out.fetch<IO>(f, r0, c0 + at + N, q[(h + 1) % 2]);
+                                if (f.has_residual) q[(h + 1) % 2].fetch<IO>(f, r0, c0 + at + N);
                             }
                             write_out<IO, FULL, N>(g, f, out, r0, c0 + at, bias, q[h], v);
                             bias = next_bias;
@@ -595,12 +623,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[i] = sum[h * 16 + i];
                         if (f.part) {
-                            out.store<float>(&g.out_map, f.part, f, v, r0, c0 + at, t.split);
+                            out.store<float>(out.next(), &g.out_map, f.part, f, v, r0, c0 + at, t.split);
                             continue;
                         }
                         if (at + N < BN / 2) {
                             next_bias = bias_of(c0 + at + N);
-                            if (f.has_residual) out.fetch<IO>(f, r0, c0 + at + N, q[(h + 1) % 2]);
+                            if (f.has_residual) q[(h + 1) % 2].fetch<IO>(f, r0, c0 + at + N);
                         }
                         write_out<IO, FULL, 16>(g, f, out, r0, c0 + at, bias, q[h], v);
                         bias = next_bias;

@@ -1,7 +1,7 @@
-// The linear map for a few rows (single tokens): y[m,n] = act(sum_k x[m,k] W[n,k] + b[n]) + r[m,n], at most kGemvRows rows.
+// The linear map for a few rows (single tokens): y[m,n] = act(sum_k x[m,k] W[n,k] + b[n]) + r[m,n], a few rows only.
 //
-// Bound by reading W once. A warp takes C rows of W at a time, 16 bytes per lane and row, the next ones already under way,
-// and keeps C x R sums; x comes from L1, each piece of it used for C rows of W. Where there are too few rows of W to
+// Bound by reading W once. A warp takes C rows of W at a time, 16 bytes per lane and row, the next kAhead such loads
+// under way, and keeps C x R sums; x comes from L1, each piece of it used for C rows of W. Where there are too few rows of W to
 // occupy the GPU, the warps of a CTA share them and cut the depth. float32 is multiplied as it is: the three-part form of
 // the tensor-core products would write W out again, six bytes for four.
 #include <type_traits>
@@ -12,6 +12,7 @@ namespace qk {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kAhead = 4;
 
 template <typename IO, int VEC>
 __device__ __forceinline__ void widen(const uint4& u, float (&f)[VEC]) {
@@ -50,30 +51,35 @@ __global__ void __launch_bounds__(kWarps * 32) gemv_kernel(const GemvArgs a) {
             if (k < end) v[c] = *reinterpret_cast<const Raw*>(w[c] + k);
         }
     };
-    Raw next[C];
+    constexpr int kStep = 32 * VEC;
+    const int row0 = blockIdx.y * R;
+    Raw ahead[kAhead][C];
     long k = begin + lane * VEC;
-    load(k, next);
-    for (; k < end; k += 32 * VEC) {
-        Raw now[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) now[c] = next[c];
-        load(k + 32 * VEC, next);
-        float wf[C][VEC];
+    for (int i = 0; i < kAhead; ++i) load(k + i * kStep, ahead[i]);
+    for (; k < end; k += kAhead * kStep) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if constexpr (VEC == 1) wf[c][0] = as_float(now[c]);
-            else widen<IO, VEC>(now[c], wf[c]);
-        }
+        for (int i = 0; i < kAhead; ++i) {
+            const long at = k + i * kStep;
+            float wf[C][VEC];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const IO* row = x + (size_t)min(r, a.rows - 1) * a.depth + k;
-            float xf[VEC];
-            if constexpr (VEC == 1) xf[0] = as_float(*row);
-            else widen<IO, VEC>(*reinterpret_cast<const uint4*>(row), xf);
+            for (int c = 0; c < C; ++c) {
+                if constexpr (VEC == 1) wf[c][0] = as_float(ahead[i][c]);
+                else widen<IO, VEC>(ahead[i][c], wf[c]);
+            }
+            load(at + kAhead * kStep, ahead[i]);
+            if (at >= end) continue;
 #pragma unroll
-            for (int c = 0; c < C; ++c)
+            for (int r = 0; r < R; ++r) {
+                const IO* row = x + (size_t)min(row0 + r, a.rows - 1) * a.depth + at;
+                float xf[VEC];
+                if constexpr (VEC == 1) xf[0] = as_float(*row);
+                else widen<IO, VEC>(*reinterpret_cast<const uint4*>(row), xf);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) acc[c][r] = fmaf(xf[i], wf[c][i], acc[c][r]);
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) acc[c][r] = fmaf(xf[e], wf[c][e], acc[c][r]);
+            }
         }
     }
 #pragma unroll
@@ -88,7 +94,7 @@ __global__ void __launch_bounds__(kWarps * 32) gemv_kernel(const GemvArgs a) {
     __syncthreads();
     // the sums of this CTA's groups, their parts in order
     for (int t = threadIdx.x; t < groups * R * C; t += kWarps * 32) {
-        const int g = t / (R * C), e = t % (R * C), r = e % R;
+        const int g = t / (R * C), e = t % (R * C), r = row0 + e % R;
         const long n = ((long)blockIdx.x * groups + g) * C + e / R;
         if (r >= a.rows || n >= a.cols) continue;
         float s = sums[g * a.cuts][e];
@@ -105,18 +111,22 @@ cudaError_t launch_rows(GemvArgs& a, cudaStream_t st) {
     const bool vec = a.depth % VEC == 0 && (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.w % 16 == 0;
     const int step = 32 * (vec ? VEC : 1);
     a.cuts = 1;
-    while (a.cuts < kWarps && groups * a.cuts < 8 * kSms && a.depth > a.cuts * step) a.cuts *= 2;
+    while (a.cuts < kWarps && groups * a.cuts < 8 * kSms && a.depth > (long)a.cuts * step) a.cuts *= 2;
     a.per = (int)(((long)a.depth + a.cuts * step - 1) / (a.cuts * step) * step);
     const long grid = (groups + kWarps / a.cuts - 1) / (kWarps / a.cuts);
-    return launch_after(vec ? gemv_kernel<IO, R, C, VEC> : gemv_kernel<IO, R, C, 1>, (unsigned)grid, kWarps * 32, 0, st, a);
+    return launch_after(vec ? gemv_kernel<IO, R, C, VEC> : gemv_kernel<IO, R, C, 1>,
+                        dim3((unsigned)grid, (a.rows + R - 1) / R), kWarps * 32, 0, st, a);
 }
 
 template <typename IO>
 cudaError_t launch_typed(GemvArgs& a, cudaStream_t st) {
-    if (a.rows == 1) return launch_rows<IO, 1, 4>(a, st);
-    if (a.rows == 2) return launch_rows<IO, 2, 4>(a, st);
-    if (a.rows <= 4) return launch_rows<IO, 4, 4>(a, st);
-    return launch_rows<IO, 8, 4>(a, st);
+    if (a.rows == 1) return launch_rows<IO, 1, 2>(a, st);
+    if (a.rows == 2) return launch_rows<IO, 2, 2>(a, st);
+    if constexpr (sizeof(IO) == 4) {
+        if (a.rows <= 4) return launch_rows<IO, 4, 2>(a, st);
+        return launch_rows<IO, 8, 2>(a, st);  // groups of eight, the later ones with W from L2
+    }
+    return cudaErrorInvalidValue;  // few_rows() lets none through
 }
 
 }  // namespace

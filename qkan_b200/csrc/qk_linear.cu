@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const PrepArgsL a) {
     if (c < j.ld) {
         const int n = min(8, j.cols - c);  // none in the padding
         const bool vec = j.vec && n > 0;
-#pragma unroll 2
+#pragma unroll 4
         for (long r = (long)slab * j.slab_rows + ty; r < end; r += ny) {
             const size_t at = (size_t)r * j.cols + c;
             float v[8];
@@ -268,16 +268,16 @@ int blocks_of(long depth) { return (int)((depth + 63) / 64); }
 struct Slabs {
     int rows, count, cblocks, tx_log2;
 };
-// 256 threads as 2^tx_log2 groups of eight columns by the rest in rows; enough slabs of rows for eight CTAs per SM, each
-// of two rows per thread at least
+// 256 threads as 2^tx_log2 groups of eight columns by the rest in rows; enough slabs of rows for four CTAs per SM, each
+// of four rows per thread at least
 Slabs slabs_of(long rows, long cols) {
     const long groups = padded(cols) / 8;
     Slabs s{};
     while (s.tx_log2 < 5 && (1 << s.tx_log2) < groups) ++s.tx_log2;
     s.cblocks = (int)((groups + (1 << s.tx_log2) - 1) >> s.tx_log2);
     const long ny = kThreads >> s.tx_log2;
-    long want = (8l * kSms + s.cblocks - 1) / s.cblocks;
-    const long most = (rows + 2 * ny - 1) / (2 * ny);
+    long want = (4l * kSms + s.cblocks - 1) / s.cblocks;
+    const long most = (rows + 4 * ny - 1) / (4 * ny);
     if (want > most) want = most;
     if (want < 1) want = 1;
     s.rows = (int)((rows + want - 1) / want);
@@ -420,7 +420,7 @@ cudaError_t run_alone(GemmArgs& a, int which, int planes, int bn, cudaStream_t s
 }  // namespace
 
 size_t linear_forward_scratch(const QkLinearDesc& d) {
-    if (d.rows <= kGemvRows || d.out_features == 0 || d.in_features == 0) return 0;
+    if (few_rows(d.rows, d.io_dtype) || d.out_features == 0 || d.in_features == 0) return 0;
     return forward_scratch(d).total;
 }
 
@@ -437,7 +437,7 @@ cudaError_t launch_linear_forward(const LinearArgs& a, cudaStream_t st) {
         add_reduce(red, nullptr, 0, M, N, epi);
         return launch_reduce(red, st);
     }
-    if (M <= kGemvRows) return launch_gemv({M, N, K, a.x, a.w, epi, 0, 0}, st);
+    if (few_rows(M, a.io_dtype)) return launch_gemv({M, N, K, a.x, a.w, epi, 0, 0}, st);
     const QkLinearDesc d{M, K, N, a.io_dtype, a.act, 0};
     const ForwardScratch& s = forward_scratch(d);
     char* ws = static_cast<char*>(a.scratch);

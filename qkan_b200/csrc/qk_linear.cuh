@@ -50,7 +50,9 @@ cudaError_t launch_gemm(const GemmArgs& a, int planes, int bn, cudaStream_t st);
 cudaError_t gemm_gave_up(unsigned* count, cudaStream_t st);
 
 // ---- few rows (qk_gemv.cu) -------------------------------------------------------
-constexpr int kGemvRows = 8;
+// Rows up to which it is taken. bfloat16: 2 (at 4096 x 4096, 4 rows took 14 us here and 9 us as a tensor-core product);
+// float32, whose products split W first: 16 (8 rows 20 us, as a product 64).
+inline bool few_rows(int rows, int io_dtype) { return rows <= (io_dtype == QK_BF16 ? 2 : 16); }
 struct GemvArgs {
     int rows, cols, depth;
     const void* x;

@@ -143,15 +143,23 @@ def test_float32_extremes_survive_the_split():
         within(tiny, x[:, 1:].double() @ w[:, 1:].double().t(), torch.full_like(want, 1e-40), "subnormal")
 
 
-def test_bfloat16_tape_keeps_signs_and_saturates():
-    x = torch.tensor([[1e-30], [-1e-30], [3e38], [-3e38], [0.0], [float("nan")]], dtype=torch.bfloat16, device="cuda")
+def test_far_arguments_of_the_activation():
+    """What half precision cannot hold: relu's tape keeps the sign of tiny values, and beyond the range every derivative
+    has its limit. A NaN stays one (relu's derivative asks for z > 0, as torch's does, and is 0 there)."""
+    z = torch.tensor([[1e-30], [-1e-30], [3e38], [-3e38], [0.0], [float("inf")], [float("-inf")], [float("nan")]],
+                     dtype=torch.bfloat16, device="cuda")
     w = torch.ones(1, 1, dtype=torch.bfloat16, device="cuda")
-    for x in (x, x.repeat(50, 1)):
-        _, tape = F.linear_forward(x, w, activation="relu", return_tape=True)
-        t = tape[:6, 0].tolist()
-        assert t[0] > 0 > t[1] and t[2] == 65504 and t[3] == -65504 and t[4] == 0 and t[5] != t[5]
-        g = F.linear_backward(x, w, torch.ones_like(x), tape=tape, activation="relu", want=("x",))["x"]
-        assert g[:5, 0].tolist() == [1, 0, 1, 0, 0]
+    limits = {"relu": (1, 0), "silu": (1, 0), "gelu": (1, 0), "gelu_tanh": (1, 0), "tanh": (0, 0), "sigmoid": (0, 0)}
+    for x in (z[:2], z, z.repeat(40, 1), z.float(), z.float().repeat(40, 1)):
+        for act, (up, down) in limits.items():
+            _, tape = F.linear_forward(x, w.to(x.dtype), activation=act, return_tape=True)
+            g = F.linear_backward(x, w.to(x.dtype), torch.ones_like(x), tape=tape, activation=act, want=("x",))["x"]
+            g = g[:8, 0].tolist()
+            if act == "relu":
+                assert g[:2] == [1, 0], (act, g)
+            if len(g) > 2:
+                assert g[2:4] == [up, down] and g[5:7] == [up, down], (act, g)
+                assert g[7] == 0 if act == "relu" else g[7] != g[7], (act, g)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16"])
