@@ -13,6 +13,9 @@
 // row by row. Stored straight from the registers, two bytes per lane and row, a 64 x 128 tile took 1.4 us; that was the
 // whole time of a product with a short depth.
 //
+// The sums of P's rows (grad_bias, where P is gz transposed) come from the tensor core as well: one more column group,
+// against a tile of ones.
+//
 // float32 (PLANES == 3): x = h + m + l exactly, each part a bfloat16 (8 significant bits, float32's exponents). Six of
 // the nine products are kept: hh | hm mh hl lh mm; what is dropped is below 2^-22 of |x||w|. hh goes to one accumulator
 // and the five small ones to another. The tensor core truncates where it adds to its accumulator, which over a long
@@ -35,17 +38,25 @@ constexpr unsigned long long kGiveUpNs = 10ull * 1000 * 1000 * 1000;  // the lon
 
 constexpr int kStoreBytes = 2048;   // 32 rows of 64 bytes: what a warp stages for one store; two of them per warp
 
-template <int BN, int PLANES>
+// Three kernels of each shape: without and with activation and tape, and one that sums P's rows as well (bfloat16, where
+// tensor memory has the room; float32 sums them where it splits them, with rounding). The sums are a few instructions in
+// the MMA loop, but products that do not want them took up to a quarter longer with those inside.
+enum Kind { kPlain, kFull, kSumRows };
+constexpr int kOnesBytes = 512;  // 16 rows of 16, without swizzle: four 8 x 16-byte pieces; every 16 of the depth reads them again
+
+template <int BN, int PLANES, Kind KIND>
 struct Shape {
     static constexpr int kABytes = kTileR * 128;
     static constexpr int kBBytes = BN * 128;
     static constexpr int kStageBytes = PLANES * (kABytes + kBBytes);
     static constexpr int kStagingBytes = kDrainWarps * 2 * kStoreBytes;
-    static constexpr int kStagesFit = (225 * 1024 - kStagingBytes) / kStageBytes;
+    static constexpr bool kSums = KIND == kSumRows;
+    static constexpr int kExtraBytes = kStagingBytes + (kSums ? kOnesBytes : 0);
+    static constexpr int kStagesFit = (225 * 1024 - kExtraBytes) / kStageBytes;
     static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
     static constexpr int kAccCols = 2 * BN;
-    static constexpr int kTmemCols = PLANES == 3 ? 2 * kAccCols : kAccCols;
-    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kStagingBytes + 1024 + 256;
+    static constexpr int kTmemCols = PLANES == 3 || kSums ? 2 * kAccCols : kAccCols;  // a power of two
+    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kExtraBytes + 1024 + 256;
     static_assert(kStages >= 2 && kTmemCols <= 512 && kSmem <= 227 * 1024, "does not fit an SM");
 };
 
@@ -184,10 +195,12 @@ struct Fields {
     void* out;
     void* tape;
     float* part;
+    float* row_sums;
     __device__ __forceinline__ explicit Fields(const GemmProblem& g)
         : rows(g.rows), cols(g.cols), tiles(g.tiles_r * g.tiles_c), tiles_c(g.tiles_c), kper(g.kper), kblocks(g.kblocks),
           units(g.units), act(g.act), has_bias(g.has_bias), has_residual(g.has_residual), vec(g.vec), tma_out(g.tma_out),
-          bias(g.bias), residual(g.residual), out(g.out), tape(g.tape), part(g.part) {}
+          bias(g.bias), residual(g.residual), out(g.out), tape(g.tape), part(g.part),
+          row_sums(g.row_sums) {}
 };
 
 // One unit of work: a tile of C and a slice of the depth.
@@ -369,17 +382,19 @@ __device__ __forceinline__ void write_out(const GemmProblem& g, const Fields& f,
     stage.store<IO>(b, &g.out_map, f.out, f, v, r, c, 0);
 }
 
-template <int BN, int PLANES, bool FULL>
+template <int BN, int PLANES, Kind KIND>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs a) {
     const bool second = (int)blockIdx.x >= a.first;
     const GemmProblem& g = second ? a.g[1] : a.g[0];
     const int cta = blockIdx.x - (second ? a.first : 0), ctas = second ? a.ctas - a.first : a.first;
-    using S = Shape<BN, PLANES>;
+    using S = Shape<BN, PLANES, KIND>;
+    constexpr bool FULL = KIND == kFull;
     using IO = std::conditional_t<PLANES == 3, float, __nv_bfloat16>;
     extern __shared__ char raw[];
     char* stages = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
     char* staging = stages + (size_t)S::kStages * S::kStageBytes;
-    Barriers& bars = *reinterpret_cast<Barriers*>(staging + S::kStagingBytes);
+    char* ones = staging + S::kStagingBytes;
+    Barriers& bars = *reinterpret_cast<Barriers*>(staging + S::kExtraBytes);
     static_assert(sizeof(Barriers) <= 256, "barriers");
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     volatile int* abort = &bars.abort;
@@ -398,6 +413,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         bar_init(&bars.drain, 1);
         bars.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if constexpr (S::kSums) {
+        if (threadIdx.x < kOnesBytes / 16)
+            reinterpret_cast<uint4*>(ones)[threadIdx.x] = make_uint4(0x3f803f80, 0x3f803f80, 0x3f803f80, 0x3f803f80);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)),
@@ -465,6 +485,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             const unsigned a_step = p_mn ? 2048 >> 4 : 32 >> 4, b_step = q_mn ? 2048 >> 4 : 32 >> 4;
             const unsigned long long a_desc = smem_desc(smem_u32(stages), p_mn);
             const unsigned long long b_desc = smem_desc(smem_u32(stages) + PLANES * S::kABytes, q_mn);
+            const unsigned long long ones_desc = (unsigned long long)((smem_u32(ones) & 0x3ffff) >> 4) | (128ull >> 4) << 16 |
+                                                 (256ull >> 4) << 32 | 1ull << 46;
+            const unsigned ones_idesc = (idesc & ~(1u << 16 | 0x3fu << 17)) | (16 / 8) << 17;  // K-major, 16 columns
             for (int u = cta; ok && u < f.units; u += ctas) {
                 const Unit t = unit_at<BN>(f, u);
                 if (PLANES == 3) {
@@ -485,6 +508,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     const unsigned d = tmem + acc * BN;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) mma(d, da + k * a_step, db + k * b_step, idesc, !(opens && k == 0));
+                    if constexpr (S::kSums) {
+                        if (f.row_sums && t.c0 == 0) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                mma(tmem + S::kAccCols + acc * 16, da + k * a_step, ones_desc, ones_idesc, !(opens && k == 0));
+                        }
+                    }
                     if constexpr (PLANES == 3) {
                         const unsigned dc = corr_base + corr * BN;
                         constexpr int kA = S::kABytes >> 4, kB = S::kBBytes >> 4;
@@ -539,6 +569,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 if (!ok) break;
                 fence_after();
                 const unsigned from = tmem + lanes + acc * BN + half * (BN / 2);
+                if constexpr (S::kSums) {
+                    if (f.row_sums && t.c0 == 0 && half == 0) {
+                        unsigned sum;
+                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\ntcgen05.wait::ld.sync.aligned;"
+                                     : "=r"(sum)
+                                     : "r"(tmem + S::kAccCols + lanes + acc * 16)
+                                     : "memory");
+                        if (r0 + lane < f.rows) f.row_sums[(size_t)t.split * f.rows + r0 + lane] = __uint_as_float(sum);
+                        __syncwarp();
+                    }
+                }
                 if (f.part) {
 #pragma unroll 1
                     for (int j = 0; j < BN / 2; j += 16) {
@@ -650,20 +691,22 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     }
 }
 
-template <int BN, int PLANES, bool FULL>
+template <int BN, int PLANES, Kind KIND>
 cudaError_t launch_shape(const GemmArgs& a, cudaStream_t st) {
-    using S = Shape<BN, PLANES>;
+    using S = Shape<BN, PLANES, KIND>;
     static unsigned long long opted = 0;
-    cudaError_t e = opt_in_smem(gemm_kernel<BN, PLANES, FULL>, &opted, (int)S::kSmem);
+    cudaError_t e = opt_in_smem(gemm_kernel<BN, PLANES, KIND>, &opted, (int)S::kSmem);
     if (e != cudaSuccess) return e;
-    return launch_after(gemm_kernel<BN, PLANES, FULL>, a.ctas, kGemmThreads, S::kSmem, st, a);
+    return launch_after(gemm_kernel<BN, PLANES, KIND>, a.ctas, kGemmThreads, S::kSmem, st, a);
 }
 
 template <int BN, int PLANES>
 cudaError_t launch_tile(const GemmArgs& a, cudaStream_t st) {
     const GemmProblem& g = a.g[0];  // two problems: gradients, neither has an activation
-    const bool full = !g.part && (g.tape || g.act != QK_ACT_NONE);
-    return full ? launch_shape<BN, PLANES, true>(a, st) : launch_shape<BN, PLANES, false>(a, st);
+    if (!g.part && (g.tape || g.act != QK_ACT_NONE)) return launch_shape<BN, PLANES, kFull>(a, st);
+    if constexpr (PLANES == 1 && BN <= 128)
+        if (g.row_sums) return launch_shape<BN, PLANES, kSumRows>(a, st);
+    return g.row_sums ? cudaErrorInvalidValue : launch_shape<BN, PLANES, kPlain>(a, st);
 }
 
 // adds this unit's count of waits that ran out, and clears it; synchronises the stream

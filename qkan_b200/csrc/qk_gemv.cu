@@ -12,7 +12,7 @@ namespace qk {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kAhead = 4;
+constexpr int kAhead = 2;
 
 template <typename IO, int VEC>
 __device__ __forceinline__ void widen(const uint4& u, float (&f)[VEC]) {
@@ -120,11 +120,11 @@ cudaError_t launch_rows(GemvArgs& a, cudaStream_t st) {
 
 template <typename IO>
 cudaError_t launch_typed(GemvArgs& a, cudaStream_t st) {
-    if (a.rows == 1) return launch_rows<IO, 1, 2>(a, st);
-    if (a.rows == 2) return launch_rows<IO, 2, 2>(a, st);
+    if (a.rows == 1) return launch_rows<IO, 1, 4>(a, st);
+    if (a.rows == 2) return launch_rows<IO, 2, 4>(a, st);
     if constexpr (sizeof(IO) == 4) {
-        if (a.rows <= 4) return launch_rows<IO, 4, 2>(a, st);
-        return launch_rows<IO, 8, 2>(a, st);  // groups of eight, the later ones with W from L2
+        if (a.rows <= 4) return launch_rows<IO, 4, 4>(a, st);
+        return launch_rows<IO, 8, 4>(a, st);  // groups of eight, the later ones with W from L2
     }
     return cudaErrorInvalidValue;  // few_rows() lets none through
 }

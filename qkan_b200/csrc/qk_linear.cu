@@ -222,11 +222,11 @@ double cost_of(const Size& s, int bn, int planes, const Cut& c) {
 }
 
 // the cheapest plan, of at most `most_units` units where that is not 0, with tiles of `only_bn` columns where that is not
-Plan plan_for(const Size& s, int planes, double* cost = nullptr, long most_units = 0, int only_bn = 0) {
+Plan plan_for(const Size& s, int planes, double* cost = nullptr, long most_units = 0, int only_bn = 0, int most_bn = 256) {
     Plan best{};
     double least = 1e300;
     for (int bn = planes == 3 ? 128 : 256; bn >= 64; bn /= 2) {
-        if (only_bn && bn != only_bn) continue;
+        if ((only_bn && bn != only_bn) || bn > most_bn) continue;
         for (int k : kCuts) {
             if (k > 1 && (k > s.kblocks || s.tiles(bn) * k > 4l * kSms || (double)k * s.rows * s.cols > kMostPart)) break;
             const Cut c = cut_into(s.kblocks, k);
@@ -302,10 +302,12 @@ ForwardScratch plan_forward(const QkLinearDesc& d) {
     return s;
 }
 
-// The layout is that of all gradients, whatever is asked for.
+// The layout is that of all gradients, whatever is asked for. grad_bias: the sums of gz's columns come from the products
+// (the tensor core sums gz as it makes grad_weight) where nothing else needs to go over gz, else from prepare.
 struct BackwardScratch {
     Plan plan_w, plan_x;
     bool together;  // both products in one launch
+    bool sums;      // grad_weight's product can sum gz's columns
     Slabs slabs;
     size_t gz, x, w, colpart, part_w, part_x, total;
 };
@@ -316,12 +318,21 @@ BackwardScratch plan_backward(const QkLinearDesc& d) {
     const bool pack_gz = d.activation != QK_ACT_NONE || !reads_in_place(N, d.io_dtype);
     const bool pack = !reads_in_place(K, d.io_dtype);
     s.together = K > 0 && plan_pair({N, K, blocks_of(M)}, {M, K, blocks_of(N)}, planes, &s.plan_w, &s.plan_x);
+    if (!pack_gz && s.plan_w.bn > 128) {
+        // narrower tiles, whose product can sum gz, against another pass over gz
+        double wide, narrow;
+        plan_for({N, K, blocks_of(M)}, planes, &wide);
+        const Plan p = plan_for({N, K, blocks_of(M)}, planes, &narrow, 0, 0, 128);
+        if (narrow < wide + 5000 + 2.0 * M * N / (kSms * 16)) s.plan_w = p, s.together = false;
+    }
     s.slabs = slabs_of(M, N);
+    s.sums = K > 0 && !pack_gz && s.plan_w.bn <= 128;
     s.gz = 0;
     s.x = pack_gz ? packed_bytes(M, N, planes) : 0;
     s.w = s.x + (pack ? packed_bytes(M, K, planes) : 0);
     s.colpart = s.w + (pack ? packed_bytes(N, K, planes) : 0);
-    s.part_w = s.colpart + align256((size_t)s.slabs.count * N * 4);
+    const int parts = s.sums && s.plan_w.cut.splits > s.slabs.count ? s.plan_w.cut.splits : s.slabs.count;
+    s.part_w = s.colpart + align256((size_t)parts * N * 4);
     s.part_x = s.part_w + (s.plan_w.cut.splits > 1 ? align256((size_t)s.plan_w.cut.splits * N * K * 4) : 0);
     s.total = s.part_x + (s.plan_x.cut.splits > 1 ? align256((size_t)s.plan_x.cut.splits * M * K * 4) : 0);
     return s;
@@ -467,8 +478,9 @@ cudaError_t launch_linear_backward(const LinearArgs& a, cudaStream_t st) {
     const bool pack = !reads_in_place(K, a.io_dtype);
     const bool pack_gz = (a.gx || a.gw) && (a.act != QK_ACT_NONE || !reads_in_place(N, a.io_dtype));
     float* colpart = a.gb ? reinterpret_cast<float*>(ws + s.colpart) : nullptr;
+    const bool sums = a.gb && a.gw && s.sums;
     PrepArgsL p{};
-    if (pack_gz || a.gb)
+    if (pack_gz || (a.gb && !sums))
         p.job[p.count++] = prep_job(a.gy, a.act == QK_ACT_NONE ? nullptr : a.tape, pack_gz ? ws + s.gz : nullptr, colpart, M,
                                     N, a.act, a.io_dtype);
     if (pack && a.gw) p.job[p.count++] = prep_job(a.x, nullptr, ws + s.x, nullptr, M, K, 0, a.io_dtype);
@@ -482,6 +494,7 @@ cudaError_t launch_linear_backward(const LinearArgs& a, cudaStream_t st) {
     if (a.gw)
         e = set_product(g.g[0], N, K, M, s.plan_w, operand(gz, M, N, pack_gz, true), operand(pack ? ws + s.x : a.x, M, K, pack, true),
                         reinterpret_cast<float*>(ws + s.part_w), {nullptr, nullptr, a.gw, nullptr, QK_ACT_NONE, a.io_dtype}, red);
+    if (sums) g.g[0].row_sums = colpart;
     if (e == cudaSuccess && a.gx)
         e = set_product(g.g[1], M, K, N, s.plan_x, operand(gz, M, N, pack_gz, false), operand(pack ? ws + s.w : a.w, N, K, pack, true),
                         reinterpret_cast<float*>(ws + s.part_x), {nullptr, nullptr, a.gx, nullptr, QK_ACT_NONE, a.io_dtype}, red);
@@ -493,7 +506,7 @@ cudaError_t launch_linear_backward(const LinearArgs& a, cudaStream_t st) {
         if (e == cudaSuccess && a.gx) e = run_alone(g, 1, planes, s.plan_x.bn, st);
     }
     if (e != cudaSuccess) return e;
-    red.colpart = colpart, red.gb = a.gb, red.slabs = s.slabs.count, red.cols = N, red.io_dtype = a.io_dtype;
+    red.colpart = colpart, red.gb = a.gb, red.slabs = sums ? s.plan_w.cut.splits : s.slabs.count, red.cols = N, red.io_dtype = a.io_dtype;
     return launch_reduce(red, st);
 }
 

@@ -27,6 +27,7 @@ struct alignas(64) GemmProblem {
     bool vec;      // bias and residual can be read in 16-byte words
     bool tma_out;  // out (part) and tape can be written by TMA
     float* part;  // splits > 1: [splits][rows][cols] sums, no epilogue; nullptr otherwise
+    float* row_sums;  // [splits][rows] sums of P's rows over the depth; nullptr: not wanted (bfloat16, no activation)
     // The epilogue, as in Epilogue. What it lacks points to `out`, so that a load of either is good whether or not it is
     // wanted: where a null pointer stood behind a test, hoisting the load over the test made it a fault.
     bool has_bias, has_residual;
