@@ -75,10 +75,20 @@ cudaError_t launch_norm_backward(const NormArgs& a, cudaStream_t st);
 // and the reciprocal by the special-function unit (off by some 2^-20 where bfloat16 is off by 2^-9). tanh and erf are the
 // full ones throughout: near zero theirs is a relative error.
 template <bool FAST>
+__device__ __forceinline__ float exp_of(float z) {
+    if constexpr (FAST) {  // without the steps that keep results below float32's normal numbers
+        float r;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(z * 1.44269504088896341f));
+        return r;
+    } else {
+        return expf(z);
+    }
+}
+template <bool FAST>
 __device__ __forceinline__ float sigmoid_of(float z) {
     if constexpr (FAST) {
         float r;
-        asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-z)));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + exp_of<FAST>(-z)));
         return r;
     } else {
         return __fdividef(1.f, 1.f + expf(-z));  // off by 2 steps at most; the exact quotient took twice as long
@@ -107,7 +117,7 @@ __device__ __forceinline__ float act_slope(float z, int act) {
             return s * fmaf(z, 1.f - s, 1.f);
         }
         case QK_ACT_GELU: {
-            const float e = FAST ? __expf(-0.5f * z * z) : expf(-0.5f * z * z);
+            const float e = exp_of<FAST>(-0.5f * z * z);
             return fmaf(z * 0.39894228040143268f, e, 0.5f * (1.f + erff(z * 0.70710678118654752f)));
         }
         case QK_ACT_GELU_TANH: {
