@@ -57,7 +57,8 @@ bool bind_operand(CUtensorMap* map, const Operand& o, int planes, int tile, int 
 bool gemm_bind(GemmProblem& g, const Operand& p, const Operand& q, int planes, int bn) {
     g.p_mn = p.mn_major;
     g.q_mn = q.mn_major;
-    if (!bind_operand(&g.p_map, p, planes, kTileRows, g.rows, &g.p_boxes, &g.p_box_bytes) ||
+    if (!bind_operand(&g.p_map, p, planes == 1 && g.wrap < g.kblocks ? 2 : planes, kTileRows, g.rows, &g.p_boxes,
+                      &g.p_box_bytes) ||
         !bind_operand(&g.q_map, q, planes, bn, g.cols, &g.q_boxes, &g.q_box_bytes))
         return false;
     const int el = planes == 3 ? 4 : 2, out_el = g.part ? 4 : el;

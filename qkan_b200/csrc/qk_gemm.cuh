@@ -13,6 +13,9 @@
 // row by row. Stored straight from the registers, two bytes per lane and row, a 64 x 128 tile took 1.4 us; that was the
 // whole time of a product with a short depth.
 //
+// A product of bfloat16 operands can take P in two parts, h + m, with 16 significant bits: gz of a backward, where
+// rounding it to eight would show beside the rounding of the result. The depth is walked twice, Q being read again.
+//
 // The sums of P's rows (grad_bias, where P is gz transposed) come from the tensor core as well: one more column group,
 // against a tile of ones.
 //
@@ -441,13 +444,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             const unsigned bytes = PLANES * boxes * (is_p ? g.p_box_bytes : g.q_box_bytes);
             const unsigned base = smem_u32(stages) + (is_p ? 0 : PLANES * S::kABytes);
             const unsigned plane = is_p ? S::kABytes : S::kBBytes;
+            const int wrap = g.wrap;
             int stage = 0;
             unsigned phase = 0, issued = 0;
             bool ok = true;
             for (int u = cta; ok && u < f.units; u += ctas) {
                 const Unit t = unit_at<BN>(f, u);
                 const int row = is_p ? t.r0 : t.c0;
-                for (int k = t.kb0 * kBK; k < (t.kb0 + t.kbs) * kBK; k += kBK) {
+                for (int kb = t.kb0; kb < t.kb0 + t.kbs; ++kb) {
+                    const bool again = kb >= wrap;  // P's second part, Q once more
+                    const int k = (again ? kb - wrap : kb) * kBK, z = again && is_p ? 1 : 0;
                     ok = bar_wait(&bars.empty[stage], phase ^ 1, abort);
                     if (!ok) break;
                     unsigned long long* bar = &bars.full[stage];
@@ -456,9 +462,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
 #pragma unroll
                     for (int p = 0; p < PLANES; ++p, dst += plane) {
                         if (mn) {
-                            for (int b = 0; b < boxes; ++b) tma_load(map, dst + b * 8192, bar, row + b * 64, k, p);
+                            for (int b = 0; b < boxes; ++b) tma_load(map, dst + b * 8192, bar, row + b * 64, k, z + p);
                         } else {
-                            tma_load(map, dst, bar, k, row, p);
+                            tma_load(map, dst, bar, k, row, z + p);
                         }
                     }
                     ++issued;

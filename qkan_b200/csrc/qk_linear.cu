@@ -4,7 +4,7 @@
 //   prepare   operands that the products cannot read where they lie: float32 is split into three bfloat16 parts, rows
 //             that are no multiple of 16 bytes are padded, and in the backward gz = gy * act'(tape) is formed, with
 //             its column sums for grad_bias on the way
-//   products  forward: one (a few rows: qk_gemv.cu, nothing else); backward: grad_weight and grad_x, in one launch where
+//   products  forward: one (a few rows: qk_gemv.cu, as in the backward); backward: grad_weight and grad_x, in one launch where
 //             both fit the GPU side by side
 //   reduce    adds the slices of a depth that was cut for want of tiles, then the epilogue; adds grad_bias' slabs
 #include "qk_linear.cuh"
@@ -18,6 +18,7 @@ struct PrepJob {
     const void* src;
     const void* tape;      // nullptr: the source as it is
     __nv_bfloat16* dst;    // [parts][rows][ld]; nullptr: column sums only
+    bool two;              // bfloat16: two parts, h + m (float32 has three)
     float* colpart;        // [slabs][cols]; nullptr: not wanted
     int rows, cols, ld, act;
     int slab_rows, cblocks, tx_log2, blocks;
@@ -110,6 +111,16 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const PrepArgsL a) {
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(h[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+                if (j.two) {
+                    unsigned m[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        // of an infinity or a NaN nothing is left
+                        const float x = v[2 * i] - __uint_as_float(h[i] << 16), y = v[2 * i + 1] - __uint_as_float(h[i] & 0xffff0000u);
+                        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(m[i]) : "f"(isfinite(y) ? y : 0.f), "f"(isfinite(x) ? x : 0.f));
+                    }
+                    out[plane / 8] = make_uint4(m[0], m[1], m[2], m[3]);
+                }
             }
             out[0] = make_uint4(h[0], h[1], h[2], h[3]);
         }
@@ -131,6 +142,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const PrepArgsL a) {
 struct ReduceJob {
     const float* part;  // [splits][rows][cols]; splits 0: sums of nothing
     int splits, cols, blocks;
+    bool tall;          // many slices of few sums: eight threads share a sum
     size_t n;
     Epilogue epi;
 };
@@ -142,10 +154,28 @@ struct ReduceArgs {
     int slabs, cols, io_dtype;
 };
 
-// One element per thread: the slices of its sum in order, then the epilogue. The blocks behind those add grad_bias'
-// slabs, 32 columns each.
+// The sum over `count` slices, n apart, of 32 neighbouring elements, by 256 threads; valid in the first 32 of them.
+__device__ __forceinline__ float tall_sum(const float* part, size_t n, size_t at, int count, float (&tile)[8][33]) {
+    const int x = threadIdx.x % 32, y = threadIdx.x / 32;
+    float s = 0.f;
+    if (at < n) {
+#pragma unroll 8
+        for (int k = y; k < count; k += 8) s += part[(size_t)k * n + at];
+    }
+    tile[y][x] = s;
+    __syncthreads();
+    if (y == 0) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) s += tile[k][x];
+    }
+    return s;
+}
+
+// The slices of each sum in a fixed order, then the epilogue: an element per thread, or (tall) 32 per CTA. The blocks
+// behind those add grad_bias' slabs, 32 columns each.
 __global__ void __launch_bounds__(kThreads) reduce_kernel(const ReduceArgs a) {
     after_previous();
+    __shared__ float tile[8][33];
     int b = blockIdx.x;
     ReduceJob j = a.job[0];
     bool sums = a.count > 0 && b < j.blocks;
@@ -155,26 +185,21 @@ __global__ void __launch_bounds__(kThreads) reduce_kernel(const ReduceArgs a) {
         sums = a.count > 1 && b < j.blocks;
         if (a.count > 1 && !sums) b -= j.blocks;
     }
-    if (sums) {
+    if (sums && !j.tall) {
         const size_t i = (size_t)b * kThreads + threadIdx.x;
         if (i >= j.n) return;
         float s = 0.f;
-#pragma unroll 4
+#pragma unroll 8
         for (int k = 0; k < j.splits; ++k) s += j.part[(size_t)k * j.n + i];
         finish_element(j.epi, i, (int)(i % j.cols), s);
-        return;
-    }
-    __shared__ float tile[8][33];
-    const int x = threadIdx.x % 32, y = threadIdx.x / 32, c = b * 32 + x;
-    float s = 0.f;
-    if (c < a.cols)
-        for (int k = y; k < a.slabs; k += 8) s += a.colpart[(size_t)k * a.cols + c];
-    tile[y][x] = s;
-    __syncthreads();
-    if (y == 0 && c < a.cols) {
-#pragma unroll
-        for (int k = 1; k < 8; ++k) s += tile[k][x];
-        store_dt(a.gb, c, a.io_dtype, s);
+    } else if (sums) {
+        const size_t i = (size_t)b * 32 + threadIdx.x % 32;
+        const float s = tall_sum(j.part, j.n, i, j.splits, tile);
+        if (threadIdx.x < 32 && i < j.n) finish_element(j.epi, i, (int)(i % j.cols), s);
+    } else {
+        const size_t c = (size_t)b * 32 + threadIdx.x % 32;
+        const float s = tall_sum(a.colpart, a.cols, c, a.slabs, tile);
+        if (threadIdx.x < 32 && c < a.cols) store_dt(a.gb, c, a.io_dtype, s);
     }
 }
 
@@ -304,8 +329,16 @@ ForwardScratch plan_forward(const QkLinearDesc& d) {
 
 // The layout is that of all gradients, whatever is asked for. grad_bias: the sums of gz's columns come from the products
 // (the tensor core sums gz as it makes grad_weight) where nothing else needs to go over gz, else from prepare.
+//
+// gz in bfloat16: where it is not gy itself it has to be rounded. To bfloat16 where there is much of it, as a framework
+// that stores gz has it: over many values that error is as large as the one of rounding the gradients, so theirs is sqrt 2
+// of what it would be. Over few values it can be up to twice: those are taken in two parts, products of twice the depth
+// (1501 x 517 -> 333: 40 against 33 us for the training step). Few rows have gz in float32.
+constexpr long kTwoPartsMost = 1 << 18;  // values of gz
 struct BackwardScratch {
     Plan plan_w, plan_x;
+    bool two;       // gz in two parts
+    FewPlan few;    // slab 0: not a matter of few rows
     bool together;  // both products in one launch
     bool sums;      // grad_weight's product can sum gz's columns
     Slabs slabs;
@@ -317,7 +350,14 @@ BackwardScratch plan_backward(const QkLinearDesc& d) {
     const long M = d.rows, K = d.in_features, N = d.out_features;
     const bool pack_gz = d.activation != QK_ACT_NONE || !reads_in_place(N, d.io_dtype);
     const bool pack = !reads_in_place(K, d.io_dtype);
-    s.together = K > 0 && plan_pair({N, K, blocks_of(M)}, {M, K, blocks_of(N)}, planes, &s.plan_w, &s.plan_x);
+    if (few_rows_backward(d.rows, d.io_dtype)) {
+        s.few = few_plan((int)K, (int)N);
+        s.total = align256((size_t)s.few.slabs * M * K * 4);  // partial sums of grad_x
+        return s;
+    }
+    s.two = d.activation != QK_ACT_NONE && planes == 1 && M * N <= kTwoPartsMost;
+    const int times = s.two ? 2 : 1;
+    s.together = K > 0 && plan_pair({N, K, times * blocks_of(M)}, {M, K, times * blocks_of(N)}, planes, &s.plan_w, &s.plan_x);
     if (!pack_gz && s.plan_w.bn > 128) {
         // narrower tiles, whose product can sum gz, against another pass over gz
         double wide, narrow;
@@ -328,7 +368,7 @@ BackwardScratch plan_backward(const QkLinearDesc& d) {
     s.slabs = slabs_of(M, N);
     s.sums = K > 0 && !pack_gz && s.plan_w.bn <= 128;
     s.gz = 0;
-    s.x = pack_gz ? packed_bytes(M, N, planes) : 0;
+    s.x = pack_gz ? packed_bytes(M, N, s.two ? 2 : planes) : 0;
     s.w = s.x + (pack ? packed_bytes(M, K, planes) : 0);
     s.colpart = s.w + (pack ? packed_bytes(N, K, planes) : 0);
     const int parts = s.sums && s.plan_w.cut.splits > s.slabs.count ? s.plan_w.cut.splits : s.slabs.count;
@@ -395,7 +435,8 @@ void add_reduce(ReduceArgs& r, const float* part, int splits, int rows, int cols
     ReduceJob& j = r.job[r.count++];
     j.part = part, j.splits = splits, j.cols = cols, j.epi = epi;
     j.n = (size_t)rows * cols;
-    j.blocks = (int)((j.n + kThreads - 1) / kThreads);
+    j.tall = splits > 8 && j.n < 64l * kThreads * kSms;
+    j.blocks = (int)(j.tall ? (j.n + 31) / 32 : (j.n + kThreads - 1) / kThreads);
 }
 
 // an operand of `rows` x `cols`, packed or as it is
@@ -404,10 +445,10 @@ Operand operand(const void* base, int rows, int cols, bool packed, bool mn_major
 }
 
 // C (rows, cols) = P Q^T over `depth`, with its epilogue; where the depth is cut, the sums wait in `part` for `red`
-cudaError_t set_product(GemmProblem& g, int rows, int cols, int depth, const Plan& plan, const Operand& p, const Operand& q,
+cudaError_t set_product(GemmProblem& g, int rows, int cols, int depth, bool two, const Plan& plan, const Operand& p, const Operand& q,
                         float* part, const Epilogue& epi, ReduceArgs& red) {
     g.rows = rows, g.cols = cols;
-    g.kblocks = blocks_of(depth), g.kper = plan.cut.kper, g.splits = plan.cut.splits;
+    g.wrap = blocks_of(depth), g.kblocks = (two ? 2 : 1) * g.wrap, g.kper = plan.cut.kper, g.splits = plan.cut.splits;
     g.tiles_r = (rows + 127) / 128, g.tiles_c = (cols + plan.bn - 1) / plan.bn;
     const long units = (long)g.tiles_r * g.tiles_c * g.splits;
     if (units > 0x3fffffff) return cudaErrorInvalidConfiguration;
@@ -464,7 +505,7 @@ cudaError_t launch_linear_forward(const LinearArgs& a, cudaStream_t st) {
         x = ws + s.x, w = ws + s.w;
     }
     GemmArgs g{};
-    e = set_product(g.g[0], M, N, K, s.plan, operand(x, M, K, pack, false), operand(w, N, K, pack, false),
+    e = set_product(g.g[0], M, N, K, false, s.plan, operand(x, M, K, pack, false), operand(w, N, K, pack, false),
                     reinterpret_cast<float*>(ws + s.part), epi, red);
     if (e == cudaSuccess) e = run_alone(g, 0, planes_of(a.io_dtype), s.plan.bn, st);
     return e == cudaSuccess ? launch_reduce(red, st) : e;
@@ -475,6 +516,15 @@ cudaError_t launch_linear_backward(const LinearArgs& a, cudaStream_t st) {
     const QkLinearDesc d{M, K, N, a.io_dtype, a.act, 0};
     const BackwardScratch& s = backward_scratch(d);
     char* ws = static_cast<char*>(a.scratch);
+    ReduceArgs red{};
+    if (s.few.slab) {
+        float* part = a.gx ? reinterpret_cast<float*>(ws) : nullptr;
+        cudaError_t e = launch_few_backward({M, K, N, a.act, a.io_dtype, a.x, a.w, a.gy, a.act == QK_ACT_NONE ? nullptr : a.tape,
+                                             part, a.gw, a.gb, s.few.blocks, s.few.slab}, st);
+        if (e != cudaSuccess) return e;
+        if (a.gx) add_reduce(red, part, s.few.slabs, M, K, {nullptr, nullptr, a.gx, nullptr, QK_ACT_NONE, a.io_dtype});
+        return launch_reduce(red, st);
+    }
     const bool pack = !reads_in_place(K, a.io_dtype);
     const bool pack_gz = (a.gx || a.gw) && (a.act != QK_ACT_NONE || !reads_in_place(N, a.io_dtype));
     float* colpart = a.gb ? reinterpret_cast<float*>(ws + s.colpart) : nullptr;
@@ -483,20 +533,20 @@ cudaError_t launch_linear_backward(const LinearArgs& a, cudaStream_t st) {
     if (pack_gz || (a.gb && !sums))
         p.job[p.count++] = prep_job(a.gy, a.act == QK_ACT_NONE ? nullptr : a.tape, pack_gz ? ws + s.gz : nullptr, colpart, M,
                                     N, a.act, a.io_dtype);
+    if (p.count) p.job[0].two = s.two;
     if (pack && a.gw) p.job[p.count++] = prep_job(a.x, nullptr, ws + s.x, nullptr, M, K, 0, a.io_dtype);
     if (pack && a.gx) p.job[p.count++] = prep_job(a.w, nullptr, ws + s.w, nullptr, N, K, 0, a.io_dtype);
     cudaError_t e = launch_prepare(p, a.io_dtype, st);
     if (e != cudaSuccess) return e;
     const void* gz = pack_gz ? ws + s.gz : a.gy;
-    ReduceArgs red{};
     GemmArgs g{};
     const int planes = planes_of(a.io_dtype);
     if (a.gw)
-        e = set_product(g.g[0], N, K, M, s.plan_w, operand(gz, M, N, pack_gz, true), operand(pack ? ws + s.x : a.x, M, K, pack, true),
+        e = set_product(g.g[0], N, K, M, s.two, s.plan_w, operand(gz, M, N, pack_gz, true), operand(pack ? ws + s.x : a.x, M, K, pack, true),
                         reinterpret_cast<float*>(ws + s.part_w), {nullptr, nullptr, a.gw, nullptr, QK_ACT_NONE, a.io_dtype}, red);
     if (sums) g.g[0].row_sums = colpart;
     if (e == cudaSuccess && a.gx)
-        e = set_product(g.g[1], M, K, N, s.plan_x, operand(gz, M, N, pack_gz, false), operand(pack ? ws + s.w : a.w, N, K, pack, true),
+        e = set_product(g.g[1], M, K, N, s.two, s.plan_x, operand(gz, M, N, pack_gz, false), operand(pack ? ws + s.w : a.w, N, K, pack, true),
                         reinterpret_cast<float*>(ws + s.part_x), {nullptr, nullptr, a.gx, nullptr, QK_ACT_NONE, a.io_dtype}, red);
     if (e == cudaSuccess && a.gw && a.gx && s.together) {
         g.first = g.g[0].units, g.ctas = g.first + g.g[1].units;

@@ -21,6 +21,7 @@ struct alignas(64) GemmProblem {
     CUtensorMap p_map, q_map, out_map, tape_map;  // out_map: of `part` where there is one
     int rows, cols;
     int kblocks, kper, splits;  // 64-deep blocks in all, per slice of the depth, slices
+    int wrap;                   // blocks of one part of P where P has two (Q again for the second); kblocks otherwise
     int tiles_r, tiles_c, units;
     bool p_mn, q_mn;
     int p_boxes, q_boxes, p_box_bytes, q_box_bytes;  // what one stage takes of each operand (and part)
@@ -62,6 +63,25 @@ struct GemvArgs {
     int cuts, per;  // filled by the launcher: warps that share the depth, elements of it for each
 };
 cudaError_t launch_gemv(const GemvArgs& a, cudaStream_t st);
+
+// The backward of a few rows, all gradients in one pass over W.
+inline bool few_rows_backward(int rows, int io_dtype) { return rows <= (io_dtype == QK_BF16 ? 4 : 16); }
+struct FewArgs {
+    int rows, in, out, act, io_dtype;
+    const void* x;
+    const void* w;
+    const void* gy;
+    const void* tape;
+    float* gx_part;  // [slabs][rows][in] sums; nullptr: grad_x not wanted
+    void* gw;
+    void* gb;
+    int blocks, slab;  // CTAs side by side, rows of W for each
+};
+struct FewPlan {
+    int blocks, slab, slabs;
+};
+FewPlan few_plan(int in, int out);
+cudaError_t launch_few_backward(const FewArgs& a, cudaStream_t st);
 
 // ---- the map (qk_linear.cu) ----------------------------------------------------
 struct LinearArgs {
