@@ -65,12 +65,13 @@ bool gemm_bind(GemmProblem& g, const Operand& p, const Operand& q, int planes, i
     auto words = [](const void* p) { return (uintptr_t)p % 16 == 0; };
     g.vec = (long)g.cols * el % 16 == 0 && words(g.bias) && words(g.residual);
     void* out = g.part ? static_cast<void*>(g.part) : g.out;
-    g.tma_out = (long)g.cols * out_el % 16 == 0 && words(out) && (!g.tape || words(g.tape));
+    const bool tape = g.tape && !g.part;  // partial sums leave the tape to the reduction
+    g.tma_out = (long)g.cols * out_el % 16 == 0 && words(out) && (!tape || words(g.tape));
     if (!g.tma_out) return true;
     if (!make_map(&g.out_map, out, out_el, g.cols, g.rows, g.cols, g.part ? g.splits : 1, 64 / out_el, 32,
                   CU_TENSOR_MAP_SWIZZLE_64B))
         return false;
-    return !g.tape || make_map(&g.tape_map, g.tape, el, g.cols, g.rows, g.cols, 1, 64 / el, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+    return !tape || make_map(&g.tape_map, g.tape, el, g.cols, g.rows, g.cols, 1, 64 / el, 32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 cudaError_t launch_gemm(const GemmArgs& a, int planes, int bn, cudaStream_t st) {

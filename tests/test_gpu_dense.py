@@ -33,7 +33,9 @@ def _problem(M, K, N, dtype, seed=0):
 SIZES = [(1, 1, 1), (1, 768, 10), (1, 10, 768), (1, 515, 1030), (2, 2048, 64), (3, 17, 5), (4, 4096, 33), (7, 264, 520),
          (8, 1000, 40), (9, 64, 128), (16, 130, 257), (17, 8, 8), (33, 64, 300), (48, 512, 256), (64, 784, 128),
          (100, 65, 127), (130, 10, 768), (129, 768, 10), (257, 100, 129), (300, 256, 256), (512, 520, 1000),
-         (1025, 24, 72), (2000, 72, 40), (4100, 40, 24), (5000, 16, 16), (260, 1032, 136), (700, 333, 260)]
+         (1025, 24, 72), (2000, 72, 40), (4100, 40, 24), (5000, 16, 16), (260, 1032, 136), (700, 333, 260),
+         # partial sums whose float32 rows are whole 16-byte words and whose bfloat16 rows are not
+         (300, 1000, 700)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16"])
