@@ -385,13 +385,144 @@ __device__ __forceinline__ void write_out(const GemmProblem& g, const Fields& f,
     stage.store<IO>(b, &g.out_map, f.out, f, v, r, c, 0);
 }
 
+// Where a warp of the epilogue stands: the next accumulator of each kind and its phase.
+struct Drain {
+    int acc = 0, corr = 0;
+    unsigned acc_phase = 0, corr_phase = 0;
+
+    // One unit: rows r0 .. r0 + 31, W columns of the tile from `offset` on. main, small: the accumulators of BN columns;
+    // lanes: the warp's part of tensor memory. False: a wait was given up.
+    template <typename IO, Kind KIND, int PLANES, int BN, int W>
+    __device__ __forceinline__ bool unit(const GemmProblem& g, const Fields& f, Stage& out, Barriers& bars, const Unit& t,
+                                         long r0, int offset, unsigned main, unsigned small, unsigned lanes) {
+        constexpr int N = 64 / sizeof(IO);  // columns of a piece
+        constexpr bool FULL = KIND == kFull;
+        volatile int* abort = &bars.abort;
+        const int lane = threadIdx.x % 32, c0 = t.c0 + offset;
+        auto bias_of = [&](int c) { return f.has_bias ? as_float(static_cast<const IO*>(f.bias)[min(c + lane, f.cols - 1)]) : 0.f; };
+        bool ok;
+        Ahead q[PLANES == 1 ? 2 : 1];  // residual of this piece and of the next (float32 has no registers for two)
+        float bias = bias_of(c0), next_bias = 0.f;
+        if (f.has_residual) q[0].template fetch<IO>(f, r0, c0);
+        if constexpr (PLANES == 1) {
+            ok = bar_wait(&bars.acc_full[acc], acc_phase, abort);
+            if (!__all_sync(~0u, ok)) return false;
+            fence_after();
+            const unsigned from = main + lanes + acc * BN + offset;
+            if constexpr (KIND == kSumRows) {
+                if (f.row_sums && t.c0 == 0 && offset == 0) {
+                    unsigned sum;
+                    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\ntcgen05.wait::ld.sync.aligned;"
+                                 : "=r"(sum)
+                                 : "r"(main + 2 * BN + lanes + acc * 16)
+                                 : "memory");
+                    if (r0 + lane < f.rows) f.row_sums[(size_t)t.split * f.rows + r0 + lane] = __uint_as_float(sum);
+                    __syncwarp();
+                }
+            }
+            if (f.part) {
+#pragma unroll 1
+                for (int j = 0; j < W; j += 16) {
+                    float v[16];
+                    __syncwarp();
+                    tmem_load<16>(from + j, v);
+                    if (j + 16 == W) {
+                        fence_before();
+                        if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
+                    }
+                    out.store<float>(out.next(), &g.out_map, f.part, f, v, r0, c0 + j, t.split);
+                }
+            } else {
+                // two pieces a turn, so that the residuals change places without being moved
+                constexpr int kTurn = W < 2 * N ? 1 : 2;
+#pragma unroll 1
+                for (int j = 0; j < W; j += kTurn * N) {
+#pragma unroll
+                    for (int h = 0; h < kTurn; ++h) {
+                        const int at = j + h * N;
+                        float v[N];
+                        __syncwarp();
+                        tmem_load<N>(from + at, v);
+                        if (at + N == W) {
+                            fence_before();
+                            if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
+                        } else {
+                            next_bias = bias_of(c0 + at + N);
+                            if (f.has_residual) q[(h + 1) % 2].template fetch<IO>(f, r0, c0 + at + N);
+                        }
+                        write_out<IO, FULL, N>(g, f, out, r0, c0 + at, bias, q[h], v);
+                        bias = next_bias;
+                    }
+                }
+            }
+            if (++acc == 2) acc = 0, acc_phase ^= 1;
+        } else {
+            float sum[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) sum[j] = 0.f;
+            for (int kb = 0; kb < t.kbs; kb += kChunk) {
+                ok = bar_wait(&bars.acc_full[acc], acc_phase, abort);
+                if (!__all_sync(~0u, ok)) return false;
+                fence_after();
+#pragma unroll
+                for (int j = 0; j < W; j += 16) {
+                    float v[16];
+                    tmem_load<16>(main + lanes + acc * BN + offset + j, v);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum[j + i] += v[i];
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
+                if (++acc == 2) acc = 0, acc_phase ^= 1;
+            }
+            ok = bar_wait(&bars.corr_full[corr], corr_phase, abort);
+            if (!__all_sync(~0u, ok)) return false;
+            fence_after();
+#pragma unroll
+            for (int j = 0; j < W; j += 16) {
+                float v[16];
+                __syncwarp();
+                tmem_load<16>(small + lanes + corr * BN + offset + j, v);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum[j + i] = isfinite(sum[j + i]) ? sum[j + i] + v[i] : sum[j + i];
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars.corr_empty[corr]);
+            if (++corr == 2) corr = 0, corr_phase ^= 1;
+            // the sums leave sixteen at a time, the others moving up: one copy of the epilogue's code
+#pragma unroll 1
+            for (int j = 0; j < W; j += 32) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int at = j + h * 16;
+                    float v[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = sum[h * 16 + i];
+                    if (f.part) {
+                        out.store<float>(out.next(), &g.out_map, f.part, f, v, r0, c0 + at, t.split);
+                        continue;
+                    }
+                    if (at + N < W) next_bias = bias_of(c0 + at + N);
+                    write_out<IO, FULL, 16>(g, f, out, r0, c0 + at, bias, q[0], v);
+                    bias = next_bias;
+                    if (f.has_residual && at + N < W) q[0].template fetch<IO>(f, r0, c0 + at + N);
+                }
+#pragma unroll
+                for (int i = 0; i + 32 < W; ++i) sum[i] = sum[i + 32];
+            }
+        }
+        return true;
+    }
+};
+
 template <int BN, int PLANES, Kind KIND>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs a) {
     const bool second = (int)blockIdx.x >= a.first;
     const GemmProblem& g = second ? a.g[1] : a.g[0];
     const int cta = blockIdx.x - (second ? a.first : 0), ctas = second ? a.ctas - a.first : a.first;
     using S = Shape<BN, PLANES, KIND>;
-    constexpr bool FULL = KIND == kFull;
     using IO = std::conditional_t<PLANES == 3, float, __nv_bfloat16>;
     extern __shared__ char raw[];
     char* stages = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
@@ -557,133 +688,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         const int quad = warp % 4, half = (warp - 2) / 4;
         const unsigned lanes = (unsigned)(quad * 32) << 16;
         Stage out{staging + (warp - 2) * 2 * kStoreBytes, 0, elect_one()};
-        constexpr int N = 64 / sizeof(IO);  // columns of a piece
-        auto bias_of = [&](int c) { return f.has_bias ? as_float(static_cast<const IO*>(f.bias)[min(c + lane, f.cols - 1)]) : 0.f; };
-        int acc = 0, corr = 0;
-        unsigned acc_phase = 0, corr_phase = 0;
+        Drain d;
         bool ok = true;
         for (int u = cta; ok && u < f.units; u += ctas) {
             const Unit t = unit_at<BN>(f, u);
-            const int c0 = t.c0 + half * (BN / 2);
-            const long r0 = t.r0 + quad * 32;
-            Ahead q[2];  // residual of this piece and of the next
-            float bias = bias_of(c0), next_bias = 0.f;
-            if (f.has_residual) q[0].fetch<IO>(f, r0, c0);
-            if constexpr (PLANES == 1) {
-                ok = bar_wait(&bars.acc_full[acc], acc_phase, abort);
-                ok = __all_sync(~0u, ok);
-                if (!ok) break;
-                fence_after();
-                const unsigned from = tmem + lanes + acc * BN + half * (BN / 2);
-                if constexpr (S::kSums) {
-                    if (f.row_sums && t.c0 == 0 && half == 0) {
-                        unsigned sum;
-                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\ntcgen05.wait::ld.sync.aligned;"
-                                     : "=r"(sum)
-                                     : "r"(tmem + S::kAccCols + lanes + acc * 16)
-                                     : "memory");
-                        if (r0 + lane < f.rows) f.row_sums[(size_t)t.split * f.rows + r0 + lane] = __uint_as_float(sum);
-                        __syncwarp();
-                    }
-                }
-                if (f.part) {
-#pragma unroll 1
-                    for (int j = 0; j < BN / 2; j += 16) {
-                        float v[16];
-                        __syncwarp();
-                        tmem_load<16>(from + j, v);
-                        if (j + 16 == BN / 2) {
-                            fence_before();
-                            if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
-                        }
-                        out.store<float>(out.next(), &g.out_map, f.part, f, v, r0, c0 + j, t.split);
-                    }
-                } else {
-                    // two pieces a turn, so that the residuals change places without being moved
-                    constexpr int kTurn = BN / 2 < 2 * N ? 1 : 2;
-#pragma unroll 1
-                    for (int j = 0; j < BN / 2; j += kTurn * N) {
-#pragma unroll
-                        for (int h = 0; h < kTurn; ++h) {
-                            const int at = j + h * N;
-                            float v[N];
-                            __syncwarp();
-                            tmem_load<N>(from + at, v);
-                            if (at + N == BN / 2) {
-                                fence_before();
-                                if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
-                            } else {
-                                next_bias = bias_of(c0 + at + N);
-                                if (f.has_residual) q[(h + 1) % 2].fetch<IO>(f, r0, c0 + at + N);
-                            }
-                            write_out<IO, FULL, N>(g, f, out, r0, c0 + at, bias, q[h], v);
-                            bias = next_bias;
-                        }
-                    }
-                }
-                if (++acc == 2) acc = 0, acc_phase ^= 1;
-            } else {
-                float sum[BN / 2];
-#pragma unroll
-                for (int j = 0; j < BN / 2; ++j) sum[j] = 0.f;
-                for (int kb = 0; kb < t.kbs; kb += kChunk) {
-                    ok = bar_wait(&bars.acc_full[acc], acc_phase, abort);
-                    ok = __all_sync(~0u, ok);
-                    if (!ok) break;
-                    fence_after();
-#pragma unroll
-                    for (int j = 0; j < BN / 2; j += 16) {
-                        float v[16];
-                        tmem_load<16>(tmem + lanes + acc * BN + half * (BN / 2) + j, v);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) sum[j + i] += v[i];
-                    }
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(&bars.acc_empty[acc]);
-                    if (++acc == 2) acc = 0, acc_phase ^= 1;
-                }
-                if (!ok) break;
-                ok = bar_wait(&bars.corr_full[corr], corr_phase, abort);
-                ok = __all_sync(~0u, ok);
-                if (!ok) break;
-                fence_after();
-#pragma unroll
-                for (int j = 0; j < BN / 2; j += 16) {
-                    float v[16];
-                    __syncwarp();
-                    tmem_load<16>(corr_base + lanes + corr * BN + half * (BN / 2) + j, v);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sum[j + i] = isfinite(sum[j + i]) ? sum[j + i] + v[i] : sum[j + i];
-                }
-                fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&bars.corr_empty[corr]);
-                if (++corr == 2) corr = 0, corr_phase ^= 1;
-                // the sums leave sixteen at a time, the others moving up: one copy of the epilogue's code
-#pragma unroll 1
-                for (int j = 0; j < BN / 2; j += 32) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int at = j + h * 16;
-                        float v[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = sum[h * 16 + i];
-                        if (f.part) {
-                            out.store<float>(out.next(), &g.out_map, f.part, f, v, r0, c0 + at, t.split);
-                            continue;
-                        }
-                        if (at + N < BN / 2) {
-                            next_bias = bias_of(c0 + at + N);
-                            if (f.has_residual) q[(h + 1) % 2].fetch<IO>(f, r0, c0 + at + N);
-                        }
-                        write_out<IO, FULL, 16>(g, f, out, r0, c0 + at, bias, q[h], v);
-                        bias = next_bias;
-                    }
-#pragma unroll
-                    for (int i = 0; i + 32 < BN / 2; ++i) sum[i] = sum[i + 32];
-                }
-            }
+            ok = d.unit<IO, KIND, PLANES, BN, BN / 2>(g, f, out, bars, t, t.r0 + quad * 32, half * (BN / 2), tmem, corr_base,
+                                                      lanes);
         }
         // shared memory is given up once every store has read its piece
         if (out.leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
