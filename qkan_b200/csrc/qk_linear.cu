@@ -242,7 +242,7 @@ double cost_of(const Size& s, int bn, int planes, const Cut& c) {
     const long units = s.tiles(bn) * c.splits;
     const double mainloop = c.kper * block_clocks(s, bn, planes), drain = drain_clocks(bn);
     double t = (double)((units + kSms - 1) / kSms) * (mainloop > drain ? mainloop : drain) + drain + 2500;
-    if (c.splits > 1) t += 3500 + 2.0 * c.splits * s.rows * s.cols * 4 / (kSms * 24.0);
+    if (c.splits > 1) t += 4800 + 2.0 * c.splits * s.rows * s.cols * 4 / (kSms * 24.0);
     return t;
 }
 

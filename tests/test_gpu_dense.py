@@ -338,6 +338,32 @@ def test_layer_norm_autograd_views_and_offsets(dtype):
     within(bl.grad, *norm64_grads(x, None, gy)["bias"], "bias alone")
 
 
+# ---------------------------------------------------------------- far offsets
+def test_rows_beyond_32_bit_offsets():
+    """More than 2^31 elements: rows at both ends of the tensors are as the same rows by themselves."""
+    M, D = (1 << 18) + 24, 8192 + 8
+    assert M * D > 1 << 31
+    x = torch.empty(M, D, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1))
+    some = torch.tensor([0, 1, M // 2, M - 2, M - 1], device="cuda")
+    w = _randn(D, seed=2)
+    y, stats = F.layer_norm_forward(x, w)
+    ys, ss = F.layer_norm_forward(x[some], w)
+    assert torch.equal(y[some], ys) and torch.equal(stats[some], ss)
+    g = F.layer_norm_backward(x, w, stats, y, want=("x",))["x"]
+    assert torch.equal(g[some], F.layer_norm_backward(x[some], w, ss, ys, want=("x",))["x"])
+    del g, y
+    # a narrow input and a wide output, an odd output, and the gradients of the former
+    for N in (D, D + 1):
+        xs, wn = x[:, :16].contiguous(), _randn(N, 16, seed=3, dtype=torch.bfloat16)
+        y = F.linear_forward(xs, wn)
+        within(y[some], *linear64(xs[some], wn)[:2], f"y {N}")
+        if N == D:
+            gx = F.linear_backward(xs, wn, x, want=("x",))["x"]
+            v, e = linear64_grads(xs[some], wn, None, x[some])["x"]
+            within(gx[some], v, e, "grad x")
+        del y
+
+
 # ---------------------------------------------------------------- streams, graphs, modules
 def test_operators_on_another_stream_and_two_streams_at_once():
     x, w, b, r, gy = _problem(600, 320, 264, torch.bfloat16)
@@ -357,6 +383,7 @@ def test_operators_on_another_stream_and_two_streams_at_once():
 
 @pytest.mark.parametrize("rows", [1, 5, 300])
 def test_operators_in_a_captured_graph(rows):
+    """Two graphs of the same step, replayed side by side on two streams as well: each has scratch of its own."""
     x, w, b, r, gy = _problem(rows, 264, 520, torch.bfloat16)
     nw = _randn(264, seed=11, dtype=torch.bfloat16)
 
@@ -378,8 +405,11 @@ def test_operators_in_a_captured_graph(rows):
         graphs.append((graph, out))
     for seed in (1, 2):
         x.copy_(_randn(rows, 264, seed=seed, dtype=torch.bfloat16))
+        torch.cuda.synchronize()
         for graph, _ in graphs:
-            graph.replay()
+            with torch.cuda.stream(torch.cuda.Stream()):
+                graph.replay()
+        torch.cuda.synchronize()
         eager = step()
         torch.cuda.synchronize()
         for _, out in graphs:
@@ -441,6 +471,55 @@ def test_modules_in_eval_and_training():
         assert torch.equal(lin(norm(x)), y)
     with pytest.raises(ValueError):
         norm(_randn(5, 63))
+
+
+def test_captured_backward_while_an_eager_graph_of_the_same_leaves_lives():
+    """make_graphed_train_step differentiates aliases of the parameters, so an eager graph that is still alive does not
+    tie the capture to its stream."""
+    from qkan_b200.graph import make_graphed_train_step
+
+    torch.manual_seed(0)
+    model = torch.nn.Sequential(LayerNorm(40, device="cuda"), Linear(40, 72, activation="silu", device="cuda"),
+                                Linear(72, 24, device="cuda"))
+    x, target = _randn(150, 40), _randn(150, 24, seed=1)
+    loss_fn = torch.nn.functional.mse_loss
+    alive = loss_fn(model(x), target)
+    alive.backward(retain_graph=True)
+    eager = [p.grad.clone() for p in model.parameters()]
+    step = make_graphed_train_step(model, x, target, loss_fn, torch.optim.SGD(model.parameters(), lr=0.0))
+    step(x, target)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p.grad, g) for p, g in zip(model.parameters(), eager))
+    assert alive.requires_grad
+
+
+def test_operators_from_two_threads():
+    """Plans and error texts are kept per thread; calls from several at once do not meet."""
+    import threading
+
+    cases = [_problem(30 + 7 * k, 40 + 8 * k, 24 + 5 * k, DTYPES[k % 2], seed=k) for k in range(6)]
+    failures = []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    x, w, b, r, gy = cases[k]
+                    y = F.linear_forward(x, w, b, residual=r)
+                    g = F.linear_backward(x, w, gy)
+                within(y, *linear64(x, w, b, r)[:2], "y")
+                for n, (v, e) in linear64_grads(x, w, b, gy).items():
+                    within(g[n], v, e, n)
+        except Exception as exc:  # seen in the main thread
+            failures.append(exc)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
 
 
 def test_operators_on_a_second_device():
