@@ -923,15 +923,16 @@ def count_kernels(torch, fn):
 
 def run_hqkan_block(run: Run):
     """The launch-bound regime: the hybrid block Linear(768 -> w) -> QKAN[w, w] -> Linear(w -> 768) in bfloat16
-    (qkan_b200.FusedHQKAN, w = 10, one repetition), forward + loss + backward, eager and captured in a CUDA graph."""
+    (qkan_b200.FusedHQKAN, w = 10, one repetition), forward + loss + backward, eager and captured in a CUDA graph. The
+    pre-norm block around it with its residual (qkan_b200.HQKANBlock) is reported beside it and is not in the value."""
     torch, args, dev, rank = run.torch, run.args, run.dev, run.rank
-    from qkan_b200 import FusedHQKAN
+    from qkan_b200 import FusedHQKAN, HQKANBlock
     from qkan_b200.graph import make_graphed_train_step
 
-    table = []
-    for rows in (8192, 1024):
+    table, prenorm = [], []
+    for rows, kind in ((8192, FusedHQKAN), (1024, FusedHQKAN), (8192, HQKANBlock), (1024, HQKANBlock)):
         torch.manual_seed(0)
-        block = FusedHQKAN(768, 10, reps=1, device=dev)
+        block = kind(768, 10, reps=1, device=dev)
         x = torch.randn(rows, 768, device=dev, dtype=torch.bfloat16)
         tgt = torch.randn(rows, 768, device=dev, dtype=torch.bfloat16)
         loss_fn = lambda y, t: torch.nn.functional.mse_loss(y.float(), t.float())  # noqa: E731
@@ -945,8 +946,9 @@ def run_hqkan_block(run: Run):
         eager_ms = run.time_steps(eager, args.steps, args.warmup)[0] / args.steps
         graphed = make_graphed_train_step(block, x, tgt, loss_fn, opt)
         graph_ms = run.time_steps(lambda mark: graphed(x, tgt), args.steps, args.warmup)[0] / args.steps
-        table.append({"rows": rows, "eager_us": 1e3 * eager_ms, "graphed_us": 1e3 * graph_ms,
-                      "library_launches_per_step": lib_k, "all_kernels_per_step": all_k})
+        (table if kind is FusedHQKAN else prenorm).append(
+            {"rows": rows, "eager_us": 1e3 * eager_ms, "graphed_us": 1e3 * graph_ms,
+             "library_launches_per_step": lib_k, "all_kernels_per_step": all_k})
     if rank == 0:
         edges = sum(r["rows"] for r in table) * 100
         ms = sum(r["graphed_us"] for r in table) * 1e-3
@@ -958,7 +960,8 @@ def run_hqkan_block(run: Run):
                                    "forward + MSE + backward at 8192 and 1024 rows, eager and CUDA-graph replay",
                        "l2": "flushed between timed steps (256 MB write)",
                        "library_kernels": "prep, forward, backward, base_backward, finish_grads"},
-            "rows": table, "gpu_launches": sum(r["library_launches_per_step"] for r in table) * args.steps,
+            "rows": table, "prenorm_block": prenorm,
+            "gpu_launches": sum(r["library_launches_per_step"] for r in table) * args.steps,
         }
         print(json.dumps(line))
     run.finish()
