@@ -8,10 +8,15 @@
 // memory: "K-major" when the summed axis is contiguous (forward: x and W), "MN-major" when it is the other axis (W in
 // grad_x, x and gz in grad_weight).
 //
-// A lane of tensor memory is a row of C, so a thread of the epilogue has one row and reads the residual along it. Results
-// go through 64-byte rows in shared memory, from where TMA stores them (rows of whole 16-byte words) or the warp does,
-// row by row. Stored straight from the registers, two bytes per lane and row, a 64 x 128 tile took 1.4 us; that was the
-// whole time of a product with a short depth.
+// A lane of tensor memory is a row of C, so a thread of the epilogue has one row. Results go through 64-byte rows in
+// shared memory, from where TMA stores them (rows of whole 16-byte words) or the warp does, row by row. Lanes along the
+// columns, two bytes stored by each straight from its registers, made the epilogue the whole time of a product with a short
+// depth.
+//
+// Measured (bfloat16): 8192 x 4096 -> 4096 forward 185 us, 1.48 PFLOP/s, bound by the tensor core; 8192 x 768 -> 768 11.6 us;
+// 8192 x 64 -> 768 5.4 us, bound by the epilogue; 64 x 64 -> 64 2.4 us, the latency of one tile. float32: 8192 x 4096 -> 4096
+// 1.26 ms, 218 TFLOP/s of 280 that six bfloat16 products leave, bound by shared memory (the MMAs read 192 KB per block of
+// 1536 clocks, the copies write 96 KB).
 //
 // A product of bfloat16 operands can take P in two parts, h + m, with 16 significant bits: gz of a backward, where
 // rounding it to eight would show beside the rounding of the result. The depth is walked twice, Q being read again.
@@ -189,7 +194,7 @@ __device__ __forceinline__ unsigned long long smem_desc(unsigned addr, bool mn) 
 }
 
 // The fields of the problem that the loops use, in registers. Read from the parameter itself they are fetched again after
-// every asm statement, since its address is taken for the tensor maps: the producer's loop took 320 ns per block that way.
+// every asm statement, since its address is taken for the tensor maps.
 struct Fields {
     int rows, cols, tiles, tiles_c, kper, kblocks, units, act;
     bool has_bias, has_residual, vec, tma_out;

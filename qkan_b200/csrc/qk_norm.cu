@@ -13,6 +13,9 @@
 // A warp takes a whole row where it can: then the sums need no barrier, and their cost is spread over up to 24
 // elements per thread. (With 16 elements per thread and weight and bias read again for every row, bfloat16 rows were bound by
 // instructions, at half of float32's bandwidth.)
+//
+// Measured: 16384 x 4096 float32 forward 87 us (6.2 TB/s), backward 138 us (5.8 TB/s); 65536 x 768 bfloat16 36.8 us (5.5 TB/s)
+// and 63.9 us (4.7 TB/s); 8192 x 768 bfloat16 4.9 us and 11.7 us, of which the second launch is 4; one row 1.4 us.
 #include <type_traits>
 
 #include "qk_dense.cuh"
