@@ -222,9 +222,9 @@ int qk_pz_forward_noalloc(const QkDesc* desc, const void* x, const float* theta,
 /*
  * Dense operators of the hybrid block (Linear -> QKAN -> Linear, src/qkan/solver/cute/cute_ops.py:449-490) and of the
  * Linear-SiLU-Linear head (src/qkan/qkan.py:1170-1211): the linear map with bias, activation and residual in its
- * epilogue, and layer norm, each with its backward pass. All tensors are contiguous and row-major; pointers need the
- * alignment of their element (stats: 8 bytes), and bfloat16 x, weight and grad_y of the linear map whose rows are a
- * multiple of 16 bytes have to start on a 16-byte boundary. Gradients are OVERWRITTEN, summed in a fixed order
+ * epilogue, and layer norm, each with its backward pass. All tensors are contiguous and row-major, and no output overlaps
+ * an input; pointers need the alignment of their element (stats: 8 bytes), and bfloat16 x, weight and grad_y of the linear
+ * map whose rows are a multiple of 16 bytes have to start on a 16-byte boundary (others are refused). Gradients are OVERWRITTEN, summed in a fixed order
  * (run-to-run bitwise reproducible), and written in the type of the tensor that they belong to. A workspace size of 1
  * says that none is needed (its pointer may be NULL), 0 that the descriptor is refused.
  */
@@ -253,7 +253,7 @@ typedef struct QkLinearDesc {
  * qk_linear_backward. It is float32 for QK_F32 and IEEE half for QK_BF16: three more bits than bfloat16 where the
  * activations bend; beyond half's range it is infinite, where every derivative has its limit, and relu's keeps the sign
  * of what is below it. Products and sums: float32, for QK_F32 to float32 accuracy.
- * y may not overlap an input. in_features == 0 gives act(bias) + residual.
+ * in_features == 0 gives act(bias) + residual.
  */
 size_t qk_linear_forward_workspace_bytes(const QkLinearDesc* desc);
 int qk_linear_forward(const QkLinearDesc* desc, const void* x, const void* weight, const void* bias,

@@ -54,6 +54,12 @@ long int_arg(PyObject* o) {
     return v;
 }
 
+bool truth_arg(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw python_error();
+    return v != 0;
+}
+
 int io_code(at::ScalarType t, const char* what) {
     if (t == at::kFloat) return QK_F32;
     if (t == at::kBFloat16) return QK_BF16;
@@ -82,10 +88,11 @@ void require_cuda(const Tensor& x) {
 }
 
 const void* at_or_null(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
-Tensor packed(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
-// contiguous, and on a 16-byte boundary (a view may start anywhere in its storage)
+// contiguous, and the values themselves (the imaginary part of a conjugate is a view whose sign is still to be turned)
+Tensor packed(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+// and on a 16-byte boundary (a view may start anywhere in its storage)
 Tensor aligned(const Tensor& t) {
-    Tensor c = t.contiguous();
+    Tensor c = packed(t);
     return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 ? c.clone() : c;
 }
 
@@ -169,7 +176,7 @@ PyObject* linear_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     bias = packed(bias), residual = packed(residual);
     const Tensor y = at::empty(c.shape, x.options());
     Tensor tape;
-    if (c.desc.activation != QK_ACT_NONE && PyObject_IsTrue(args[5])) tape = at::empty(c.shape, x.options().dtype(c.tape_type()));
+    if (c.desc.activation != QK_ACT_NONE && truth_arg(args[5])) tape = at::empty(c.shape, x.options().dtype(c.tape_type()));
     const Tensor ws = scratch(x, qk_linear_forward_workspace_bytes(&c.desc), "qk_linear_forward_workspace_bytes");
     check(qk_linear_forward(&c.desc, x.const_data_ptr(), w.const_data_ptr(), at_or_null(bias), at_or_null(residual),
                             y.mutable_data_ptr(), const_cast<void*>(at_or_null(tape)), const_cast<void*>(at_or_null(ws)),
@@ -243,7 +250,7 @@ PyObject* norm_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor x = packed(c.x), w = packed(c.w), b = packed(c.b);
     const Tensor y = at::empty(x.sizes(), x.options());
     Tensor stats;
-    if (PyObject_IsTrue(args[4])) stats = at::empty(c.stats_shape, x.options().dtype(at::kFloat));
+    if (truth_arg(args[4])) stats = at::empty(c.stats_shape, x.options().dtype(at::kFloat));
     check(qk_layer_norm_forward(&c.desc, x.const_data_ptr(), at_or_null(w), at_or_null(b), y.mutable_data_ptr(),
                                 static_cast<float*>(const_cast<void*>(at_or_null(stats))), scope.stream),
           "qk_layer_norm_forward");
@@ -267,7 +274,7 @@ PyObject* norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     require_cuda(c.x);
     Scope scope(c.x);
     const Tensor x = packed(c.x), w = packed(c.w);
-    gy = packed(gy), stats = packed(stats);
+    gy = packed(gy), stats = aligned(stats);  // the kernels read a row's two numbers at once
     Tensor gx, gw, gb;
     if (want & 1) gx = at::empty(x.sizes(), x.options());
     if (want & 2) gw = at::empty({c.D}, x.options().dtype(c.param));

@@ -1,4 +1,6 @@
 // C ABI of the dense operators (see include/qkan_b200.h): argument validation and scratch carving.
+#include <initializer_list>
+
 #include "qk_linear.cuh"
 
 namespace {
@@ -8,15 +10,15 @@ using qk::cuda_fail;
 using qk::fail;
 
 bool is_dtype(int t) { return t == QK_F32 || t == QK_BF16; }
+constexpr int kMost = 0x7fffff00;  // of a dimension: indices are rounded up to whole tiles (and steps) in 32 bits
 
 int check_linear(const QkLinearDesc* d) {
     if (!d) return fail(QK_ERR_BAD_ARGUMENT, "desc is NULL");
     if (d->rows < 0 || d->in_features < 0 || d->out_features < 0)
         return fail(QK_ERR_BAD_ARGUMENT, "negative dimension (rows=%d in=%d out=%d)", d->rows, d->in_features,
                     d->out_features);
-    const int most = 0x7fffff00;  // indices are rounded up to whole tiles in 32 bits
-    if (d->rows > most || d->in_features > most || d->out_features > most)
-        return fail(QK_ERR_UNSUPPORTED, "a dimension exceeds %d (rows=%d in=%d out=%d)", most, d->rows, d->in_features,
+    if (d->rows > kMost || d->in_features > kMost || d->out_features > kMost)
+        return fail(QK_ERR_UNSUPPORTED, "a dimension exceeds %d (rows=%d in=%d out=%d)", kMost, d->rows, d->in_features,
                     d->out_features);
     if (!is_dtype(d->io_dtype)) return fail(QK_ERR_BAD_ARGUMENT, "io_dtype %d is neither QK_F32 nor QK_BF16", d->io_dtype);
     if (d->activation < QK_ACT_NONE || d->activation > QK_ACT_SIGMOID)
@@ -28,6 +30,7 @@ int check_linear(const QkLinearDesc* d) {
 int check_norm(const QkNormDesc* d) {
     if (!d) return fail(QK_ERR_BAD_ARGUMENT, "desc is NULL");
     if (d->rows < 0 || d->dim < 1) return fail(QK_ERR_BAD_ARGUMENT, "rows=%d dim=%d: rows >= 0 and dim >= 1 are wanted", d->rows, d->dim);
+    if (d->dim > kMost) return fail(QK_ERR_UNSUPPORTED, "dim=%d exceeds %d", d->dim, kMost);
     if (!is_dtype(d->io_dtype) || !is_dtype(d->param_dtype))
         return fail(QK_ERR_BAD_ARGUMENT, "io_dtype %d / param_dtype %d is neither QK_F32 nor QK_BF16", d->io_dtype, d->param_dtype);
     if (!(d->eps >= 0.f)) return fail(QK_ERR_BAD_ARGUMENT, "eps must be >= 0");
@@ -40,6 +43,13 @@ int check_aligned(const void* p, int width, int io_dtype, const char* what) {
     if (qk::reads_in_place(width, io_dtype) && (uintptr_t)p % 16)
         return fail(QK_ERR_BAD_ARGUMENT, "%s must be 16-byte aligned (its rows are whole 16-byte words)", what);
     return QK_OK;
+}
+
+// every pointer on a boundary of its element; a pointer that is not wanted is NULL, which is one
+int check_elements(std::initializer_list<const void*> all, size_t bytes, const char* what) {
+    uintptr_t bits = 0;
+    for (const void* p : all) bits |= (uintptr_t)p;
+    return bits % bytes ? fail(QK_ERR_BAD_ARGUMENT, "%s must be %zu-byte aligned", what, bytes) : QK_OK;
 }
 
 size_t norm_scratch(const QkNormDesc& d) {
@@ -73,6 +83,8 @@ int qk_linear_forward(const QkLinearDesc* desc, const void* x, const void* weigh
     if (d.rows == 0 || d.out_features == 0) return QK_OK;
     if (!y) return fail(QK_ERR_BAD_ARGUMENT, "y is NULL");
     if (d.in_features && (!x || !weight)) return fail(QK_ERR_BAD_ARGUMENT, "x or weight is NULL");
+    // the tape's half is as wide as bfloat16
+    if ((rc = check_elements({x, weight, bias, residual, y, tape}, qk::dtype_bytes(d.io_dtype), "every tensor"))) return rc;
     if ((rc = check_aligned(x, d.in_features, d.io_dtype, "x"))) return rc;
     if ((rc = check_aligned(weight, d.in_features, d.io_dtype, "weight"))) return rc;
     rc = check_scratch(ws, ws_bytes, qk::linear_forward_scratch(d));
@@ -107,6 +119,7 @@ int qk_linear_backward(const QkLinearDesc* desc, const void* x, const void* weig
     if (!gy) return fail(QK_ERR_BAD_ARGUMENT, "grad_y is NULL");
     if (d.activation != QK_ACT_NONE && !tape) return fail(QK_ERR_BAD_ARGUMENT, "tape is NULL");
     if ((gx && !weight) || (gw && !x)) return fail(QK_ERR_BAD_ARGUMENT, "x or weight is NULL");
+    if ((rc = check_elements({x, weight, tape, gy, gx, gw, gb}, qk::dtype_bytes(d.io_dtype), "every tensor"))) return rc;
     if (gw && (rc = check_aligned(x, d.in_features, d.io_dtype, "x"))) return rc;
     if (gx && (rc = check_aligned(weight, d.in_features, d.io_dtype, "weight"))) return rc;
     if ((gx || gw) && (rc = check_aligned(gy, d.out_features, d.io_dtype, "grad_y"))) return rc;
@@ -129,11 +142,14 @@ int qk_dense_status(void* stream) {
 
 int qk_layer_norm_forward(const QkNormDesc* desc, const void* x, const void* weight, const void* bias, void* y,
                           float* stats, void* stream) {
-    const int rc = check_norm(desc);
+    int rc = check_norm(desc);
     if (rc) return rc;
     const QkNormDesc& d = *desc;
     if (d.rows == 0) return QK_OK;
     if (!x || !y) return fail(QK_ERR_BAD_ARGUMENT, "x or y is NULL");
+    if ((rc = check_elements({x, y}, qk::dtype_bytes(d.io_dtype), "x and y"))) return rc;
+    if ((rc = check_elements({weight, bias}, qk::dtype_bytes(d.param_dtype), "weight and bias"))) return rc;
+    if ((rc = check_elements({stats}, 8, "stats"))) return rc;
     qk::NormArgs a{};
     a.rows = d.rows, a.dim = d.dim, a.io_dtype = d.io_dtype, a.param_dtype = d.param_dtype, a.eps = d.eps;
     a.x = x, a.w = weight, a.b = bias, a.y = y;
@@ -160,6 +176,9 @@ int qk_layer_norm_backward(const QkNormDesc* desc, const void* x, const void* we
     }
     if (!gx && !gw && !gb) return QK_OK;
     if (!x || !stats || !gy) return fail(QK_ERR_BAD_ARGUMENT, "x, stats or grad_y is NULL");
+    if ((rc = check_elements({x, gy, gx}, qk::dtype_bytes(d.io_dtype), "x, grad_y and grad_x"))) return rc;
+    if ((rc = check_elements({weight, gw, gb}, qk::dtype_bytes(d.param_dtype), "weight and its gradients"))) return rc;
+    if ((rc = check_elements({stats}, 8, "stats"))) return rc;
     qk::NormArgs a{};
     a.rows = d.rows, a.dim = d.dim, a.io_dtype = d.io_dtype, a.param_dtype = d.param_dtype, a.eps = d.eps;
     a.x = x, a.w = weight, a.gy = gy, a.gx = gx, a.gw = gw, a.gb = gb;

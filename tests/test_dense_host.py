@@ -100,6 +100,42 @@ def test_norm_pointers_and_workspaces_that_are_refused():
     assert lib.qk_layer_norm_backward(dp, None, None, None, None, None, None, None, None, 0, None) == _abi.QK_OK
 
 
+def test_pointers_off_their_elements_boundary_are_refused():
+    lib = _lib()
+    one, big = ctypes.c_void_p(256), 1 << 40
+    for dtype, off in ((_abi.QK_F32, 258), (_abi.QK_BF16, 257)):
+        odd = ctypes.c_void_p(off)
+        dp = _abi.desc_pointer(_abi.QkLinearDesc(64, 65, 63, dtype, _abi.QK_ACT_SILU, 0))
+        for k in range(6):  # x, weight, bias, residual, y, tape
+            p = [odd if i == k else one for i in range(6)]
+            assert lib.qk_linear_forward(dp, *p, one, big, None) == _abi.QK_ERR_BAD_ARGUMENT
+        for k in range(7):  # x, weight, tape, gy and the gradients
+            p = [odd if i == k else one for i in range(7)]
+            assert lib.qk_linear_backward(dp, *p, one, big, None) == _abi.QK_ERR_BAD_ARGUMENT
+        dp = _abi.desc_pointer(_abi.QkNormDesc(64, 65, dtype, dtype, 1e-5, 0))
+        for k in range(5):  # x, weight, bias, y, stats
+            p = [odd if i == k else one for i in range(5)]
+            assert lib.qk_layer_norm_forward(dp, *p, None) == _abi.QK_ERR_BAD_ARGUMENT
+        for k in range(7):  # x, weight, stats, gy and the gradients
+            p = [odd if i == k else one for i in range(7)]
+            assert lib.qk_layer_norm_backward(dp, *p, one, big, None) == _abi.QK_ERR_BAD_ARGUMENT
+        # a row's two statistics are read at once
+        stats = ctypes.c_void_p(260)
+        assert lib.qk_layer_norm_forward(dp, one, one, one, one, stats, None) == _abi.QK_ERR_BAD_ARGUMENT
+        assert lib.qk_layer_norm_backward(dp, one, one, stats, one, one, one, one, one, big, None) == _abi.QK_ERR_BAD_ARGUMENT
+        assert b"stats must be 8-byte aligned" in lib.qk_last_error()
+
+
+def test_norm_rows_beyond_the_index_range_are_refused():
+    # the loops over a row step past its end in 32 bits
+    lib, one = _lib(), ctypes.c_void_p(256)
+    for dim in (2 ** 31 - 1, 2 ** 31 - 255):
+        dp = _abi.desc_pointer(_abi.QkNormDesc(1, dim, _abi.QK_BF16, _abi.QK_BF16, 1e-5, 0))
+        assert lib.qk_layer_norm_backward_workspace_bytes(dp) == 0
+        assert lib.qk_layer_norm_forward(dp, one, None, None, one, None, None) == _abi.QK_ERR_UNSUPPORTED
+        assert lib.qk_layer_norm_backward(dp, one, None, one, one, one, one, one, one, 1 << 40, None) == _abi.QK_ERR_UNSUPPORTED
+
+
 def test_cpu_tensors_are_refused():
     x, w = torch.zeros(2, 4), torch.zeros(3, 4)
     for call in (lambda: F.fused_linear(x, w), lambda: F.linear_backward(x, w, torch.zeros(2, 3)),

@@ -339,6 +339,33 @@ def test_layer_norm_autograd_views_and_offsets(dtype):
 
 
 # ---------------------------------------------------------------- far offsets
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16"])
+@pytest.mark.parametrize("M,D", [(5, 100), (3, 9001)])
+def test_layer_norm_statistics_of_any_view(dtype, M, D):
+    # the statistics of a row lie on a 4-byte boundary here, or apart
+    x, gy = _randn(M, D, seed=31, dtype=dtype), _randn(M, D, seed=32, dtype=dtype)
+    w = _randn(D, seed=33, dtype=dtype)
+    _, stats = F.layer_norm_forward(x, w)
+    want = F.layer_norm_backward(x, w, stats, gy)
+    shifted = torch.empty(2 * M + 1, device="cuda")[1:].view(M, 2).copy_(stats)
+    apart = torch.empty(2, M, device="cuda").t().copy_(stats)
+    assert shifted.data_ptr() % 8 == 4 and not apart.is_contiguous()
+    for view in (shifted, apart):
+        got = F.layer_norm_backward(x, w, view, gy)
+        for name in want:
+            assert torch.equal(got[name], want[name])
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_views_whose_sign_is_still_to_be_turned(rows):
+    x = torch.view_as_complex(_randn(rows, 24, 2, seed=34)).conj().imag
+    w = torch.view_as_complex(_randn(16, 24, 2, seed=35)).conj().imag
+    assert x.is_neg() and w.is_neg()
+    plain_x, plain_w = x.resolve_neg().contiguous(), w.resolve_neg().contiguous()
+    assert torch.equal(F.fused_linear(x, w), F.fused_linear(plain_x, plain_w))
+    assert torch.equal(F.layer_norm(x), F.layer_norm(plain_x))
+
+
 def test_rows_beyond_32_bit_offsets():
     """More than 2^31 elements: rows at both ends of the tensors are as the same rows by themselves."""
     M, D = (1 << 18) + 24, 8192 + 8
