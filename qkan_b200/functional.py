@@ -496,6 +496,8 @@ def _activation_code(activation) -> int:
 
 
 def _want_bits(want) -> int:
+    if want == _GRADS:
+        return 7
     bits = 0
     for name in want:
         if name not in _GRAD_BITS:
@@ -505,6 +507,8 @@ def _want_bits(want) -> int:
 
 
 def _named(grads, want) -> dict:
+    if want == _GRADS:
+        return dict(zip(_GRADS, grads))
     return {name: grads[_GRADS.index(name)] for name in want}
 
 
