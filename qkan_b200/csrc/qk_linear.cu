@@ -4,8 +4,9 @@
 //   prepare   operands that the products cannot read where they lie: float32 is split into three bfloat16 parts, rows
 //             that are no multiple of 16 bytes are padded, and in the backward gz = gy * act'(tape) is formed, with
 //             its column sums for grad_bias on the way
-//   products  forward: one (a few rows: qk_gemv.cu, as in the backward); backward: grad_weight and grad_x, in one launch where
-//             both fit the GPU side by side
+//   products  forward: one; backward: grad_weight and grad_x, in one launch where both fit the GPU side by side. A few rows
+//             take the kernels of qk_gemv.cu in both directions, few outputs in float32 the one of qk_narrow.cu forward;
+//             neither needs anything prepared.
 //   reduce    adds the slices of a depth that was cut for want of tiles, then the epilogue; adds grad_bias' slabs
 #include "qk_linear.cuh"
 
@@ -314,10 +315,16 @@ Slabs slabs_of(long rows, long cols) {
 
 struct ForwardScratch {
     Plan plan;
+    NarrowPlan narrow;  // few outputs in float32
     size_t x, w, part, total;
 };
 ForwardScratch plan_forward(const QkLinearDesc& d) {
     ForwardScratch s{};
+    if (few_outputs(d.out_features, d.io_dtype)) {
+        s.narrow = narrow_plan(d.rows, d.in_features);
+        if (s.narrow.splits > 1) s.total = align256((size_t)s.narrow.splits * d.rows * d.out_features * 4);
+        return s;
+    }
     const int planes = planes_of(d.io_dtype);
     const bool pack = !reads_in_place(d.in_features, d.io_dtype);
     s.plan = plan_for({d.rows, d.out_features, blocks_of(d.in_features)}, planes);
@@ -495,6 +502,13 @@ cudaError_t launch_linear_forward(const LinearArgs& a, cudaStream_t st) {
     const QkLinearDesc d{M, K, N, a.io_dtype, a.act, 0};
     const ForwardScratch& s = forward_scratch(d);
     char* ws = static_cast<char*>(a.scratch);
+    if (few_outputs(N, a.io_dtype)) {
+        float* part = s.narrow.splits > 1 ? reinterpret_cast<float*>(ws) : nullptr;
+        const cudaError_t e = launch_narrow({s.narrow, M, N, K, a.x, a.w, part, epi}, st);
+        if (e != cudaSuccess || !part) return e;
+        add_reduce(red, part, s.narrow.splits, M, N, epi);
+        return launch_reduce(red, st);
+    }
     const bool pack = !reads_in_place(K, a.io_dtype);
     const void *x = a.x, *w = a.w;
     cudaError_t e = cudaSuccess;

@@ -83,6 +83,22 @@ struct FewPlan {
 FewPlan few_plan(int in, int out);
 cudaError_t launch_few_backward(const FewArgs& a, cudaStream_t st);
 
+// ---- few outputs in float32 (qk_narrow.cu) ----------------------------------------
+inline bool few_outputs(int cols, int io_dtype) { return io_dtype == QK_F32 && cols <= 32; }
+struct NarrowPlan {
+    int tm;                   // rows of a thread
+    int chunks, per, splits;  // chunks of the depth in all, per slice, slices
+};
+NarrowPlan narrow_plan(int rows, int depth);
+struct NarrowArgs : NarrowPlan {
+    int rows, cols, depth;
+    const void* x;
+    const void* w;
+    float* part;  // splits > 1: [splits][rows][cols] sums, no epilogue; nullptr otherwise
+    Epilogue epi;
+};
+cudaError_t launch_narrow(const NarrowArgs& a, cudaStream_t st);
+
 // ---- the map (qk_linear.cu) ----------------------------------------------------
 struct LinearArgs {
     int rows, in, out, act, io_dtype;

@@ -61,6 +61,31 @@ def test_linear_forward_and_backward(size, dtype):
         within(g[k], v, e, f"plain grad {k}")
 
 
+# one to four rows per thread, 16 and 32 columns, a depth that ends inside a chunk, cut or not, rows of whole words and others
+@pytest.mark.parametrize("size", [(17, 1, 1), (24, 100, 32), (100, 3445, 10), (400, 4100, 17), (2000, 768, 31), (5000, 1030, 20),
+                                  (700, 5, 3), (40000, 36, 32), (20001, 33, 16), (513, 32, 16), (129, 4096, 32)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_linear_few_outputs_in_float32(size, act):
+    M, K, N = size
+    x, w, b, r, _ = _problem(M, K, N, torch.float32, seed=40)
+    want, bound, z, zb = linear64(x, w, b, r, act)
+    y, tape = F.linear_forward(x, w, b, activation=act, residual=r, return_tape=True)
+    within(y, want, bound, "y")
+    if tape is not None:
+        within(tape, z, zb, "tape")
+    # rows that do not start on a 16-byte boundary, and the same bits again
+    odd = torch.empty(M * K + 1, device="cuda")[1:].view(M, K).copy_(x)
+    within(F.linear_forward(odd, w), *linear64(x, w)[:2], "odd start")
+    assert torch.equal(F.linear_forward(x, w, b, activation=act, residual=r), y)
+    # what is not finite stays in its row and column
+    x[M // 2, K // 2], w[N // 2, K // 3] = float("inf"), float("nan")
+    got = F.linear_forward(x, w)
+    there = torch.zeros(M, N, dtype=torch.bool, device="cuda")
+    there[M // 2], there[:, N // 2] = True, True
+    assert torch.equal(~torch.isfinite(got), there)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16"])
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("rows", [1, 6, 150])
