@@ -5,8 +5,8 @@
 //             that are no multiple of 16 bytes are padded, and in the backward gz = gy * act'(tape) is formed, with
 //             its column sums for grad_bias on the way
 //   products  forward: one; backward: grad_weight and grad_x, in one launch where both fit the GPU side by side. A few rows
-//             take the kernels of qk_gemv.cu in both directions, few outputs in float32 the one of qk_narrow.cu forward;
-//             neither needs anything prepared.
+//             take the kernels of qk_gemv.cu in both directions, few outputs or little of everything in float32 the one of
+//             qk_narrow.cu forward; neither needs anything prepared.
 //   reduce    adds the slices of a depth that was cut for want of tiles, then the epilogue; adds grad_bias' slabs
 #include "qk_linear.cuh"
 
@@ -315,13 +315,13 @@ Slabs slabs_of(long rows, long cols) {
 
 struct ForwardScratch {
     Plan plan;
-    NarrowPlan narrow;  // few outputs in float32
+    NarrowPlan narrow;  // few outputs or little of everything in float32
     size_t x, w, part, total;
 };
 ForwardScratch plan_forward(const QkLinearDesc& d) {
     ForwardScratch s{};
-    if (few_outputs(d.out_features, d.io_dtype)) {
-        s.narrow = narrow_plan(d.rows, d.in_features);
+    if (is_narrow(d.rows, d.out_features, d.in_features, d.io_dtype)) {
+        s.narrow = narrow_plan(d.rows, d.out_features, d.in_features);
         if (s.narrow.splits > 1) s.total = align256((size_t)s.narrow.splits * d.rows * d.out_features * 4);
         return s;
     }
@@ -502,7 +502,7 @@ cudaError_t launch_linear_forward(const LinearArgs& a, cudaStream_t st) {
     const QkLinearDesc d{M, K, N, a.io_dtype, a.act, 0};
     const ForwardScratch& s = forward_scratch(d);
     char* ws = static_cast<char*>(a.scratch);
-    if (few_outputs(N, a.io_dtype)) {
+    if (is_narrow(M, N, K, a.io_dtype)) {
         float* part = s.narrow.splits > 1 ? reinterpret_cast<float*>(ws) : nullptr;
         const cudaError_t e = launch_narrow({s.narrow, M, N, K, a.x, a.w, part, epi}, st);
         if (e != cudaSuccess || !part) return e;

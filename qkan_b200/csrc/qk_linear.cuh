@@ -83,13 +83,19 @@ struct FewPlan {
 FewPlan few_plan(int in, int out);
 cudaError_t launch_few_backward(const FewArgs& a, cudaStream_t st);
 
-// ---- few outputs in float32 (qk_narrow.cu) ----------------------------------------
-inline bool few_outputs(int cols, int io_dtype) { return io_dtype == QK_F32 && cols <= 32; }
+// ---- few outputs, or few of everything, in float32 (qk_narrow.cu) ------------------
+// Few of them: up to 32 (48: 8192 x 768 39 us here, 20 on the tensor cores). And small products, where the launch that
+// prepares the operands counts: up to 2^24 multiplications (us here and there: 64 x 64 -> 64 4.6 and 7.5, 256 x 256 -> 256
+// 7.9 and 11.3, 333 x 517 -> 333 18.3 and 16.6) for up to 2^18 results (344 x 18 -> 3416 15.4 and 13.7).
+inline bool is_narrow(long rows, long cols, long depth, int io_dtype) {
+    if (io_dtype != QK_F32) return false;
+    return cols <= 32 || (rows * cols <= 1 << 18 && rows * cols * depth <= 1 << 24);
+}
 struct NarrowPlan {
     int tm;                   // rows of a thread
     int chunks, per, splits;  // chunks of the depth in all, per slice, slices
 };
-NarrowPlan narrow_plan(int rows, int depth);
+NarrowPlan narrow_plan(int rows, int cols, int depth);
 struct NarrowArgs : NarrowPlan {
     int rows, cols, depth;
     const void* x;

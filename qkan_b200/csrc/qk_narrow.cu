@@ -1,12 +1,12 @@
-// The linear map in float32 for few outputs (the hybrid block's down projection): y[m,n] = act(sum_k x[m,k] W[n,k] + b[n])
-// + r[m,n] with at most 32 columns n.
+// The linear map in float32 for few outputs (the hybrid block's down projection), or little of everything:
+// y[m,n] = act(sum_k x[m,k] W[n,k] + b[n]) + r[m,n], 16 or 32 columns n at a time.
 //
 // Bound by reading x once, from some 16 columns on by the float32 units. On the tensor cores x would be split into its three
 // parts first, 6 bytes written and read again for each 4: with so few columns that costs more than the products. Measured,
 // in us, against the tensor cores: 55447 x 1032 -> 16 69 (3.3 TB/s) and 201, -> 32 114 and 203; 8192 x 768 -> 10 12.7 and 19.6;
-// 24 x 100 -> 10 3.4 and 7.5, there for want of a second launch. With 48 columns it lost, 8192 x 768 39 and 20.
+// 24 x 100 -> 10 3.4 and 7.5, there for want of a second launch.
 //
-// A CTA has a tile of rows and all columns, and walks the depth in chunks of 32 through a ring in shared memory
+// A CTA has a tile of rows by 16 or 32 columns, and walks the depth in chunks of 32 through a ring in shared memory
 // (cp.async). A warp's lanes are 8 rows by 4 columns, TM x TN sums each, rows (columns) 8 (4) apart: with 36 floats from row
 // to row the lanes meet no bank twice. Two neighbouring products of the depth go through one packed operation, which needs
 // no value twice in a pair. Where there are too few tiles, the depth is cut and the slices added by the reduction.
@@ -45,6 +45,7 @@ __global__ void __launch_bounds__(kThreads, 3) narrow_kernel(const NarrowArgs a)
     after_previous();
     const int tile = blockIdx.x / a.splits, split = blockIdx.x - tile * a.splits;
     const long r0 = (long)tile * T::kRows;
+    const int c0 = blockIdx.y * NP, width = min(NP, a.cols - c0);
     const int chunk0 = split * a.per, chunks = min(a.per, a.chunks - chunk0);
     const float* x = static_cast<const float*>(a.x);
     const float* w = static_cast<const float*>(a.w);
@@ -57,7 +58,7 @@ __global__ void __launch_bounds__(kThreads, 3) narrow_kernel(const NarrowArgs a)
     for (int i = 0; i < kPieces; ++i) {
         const int row = row0 + i * kApart;
         from[i] = (row < T::kRows ? x + (size_t)min(r0 + row, a.rows - 1L) * a.depth
-                                  : w + (size_t)min(row - T::kRows, a.cols - 1) * a.depth) + part0;
+                                  : w + (size_t)(c0 + min(row - T::kRows, width - 1)) * a.depth) + part0;
     }
     auto fetch = [&](int c) {
         if (c < chunks) {
@@ -113,15 +114,16 @@ __global__ void __launch_bounds__(kThreads, 3) narrow_kernel(const NarrowArgs a)
     for (int i = 0; i < T::TM; ++i)
 #pragma unroll
         for (int j = 0; j < T::TN; ++j)
-            if (n + 4 * j < a.cols) ring[(m + 8 * i) * a.cols + n + 4 * j] = acc[i][j].x + acc[i][j].y;
+            if (n + 4 * j < width) ring[(m + 8 * i) * width + n + 4 * j] = acc[i][j].x + acc[i][j].y;
     __syncthreads();
-    const int count = (int)min((long)T::kRows, a.rows - r0) * a.cols;
-    const size_t first = (size_t)r0 * a.cols;
+    const int count = (int)min((long)T::kRows, a.rows - r0) * width;
     float* part = a.part ? a.part + (size_t)split * a.rows * a.cols : nullptr;
 #pragma unroll 1
     for (int t = threadIdx.x; t < count; t += kThreads) {
-        if (part) part[first + t] = ring[t];
-        else finish_element(a.epi, first + t, t % a.cols, ring[t]);
+        const int row = t / width, col = c0 + t - row * width;
+        const size_t at = (size_t)(r0 + row) * a.cols + col;
+        if (part) part[at] = ring[t];
+        else finish_element(a.epi, at, col, ring[t]);
     }
 }
 
@@ -133,7 +135,7 @@ cudaError_t run(const NarrowArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     const long tiles = ((long)a.rows + T::kRows - 1) / T::kRows;
     if (tiles * a.splits > 0x7fffffffl) return cudaErrorInvalidConfiguration;
-    return launch_after(narrow_kernel<NP, TM, VEC>, (unsigned)(tiles * a.splits), kThreads, T::kSmem, st, a);
+    return launch_after(narrow_kernel<NP, TM, VEC>, dim3((unsigned)(tiles * a.splits), (a.cols + NP - 1) / NP), kThreads, T::kSmem, st, a);
 }
 
 template <int NP, int TM>
@@ -154,11 +156,12 @@ cudaError_t run_np(const NarrowArgs& a, cudaStream_t st) {
 // much, since W is read from shared memory for all of them. (us with 1, 2, 4: 100 x 768 -> 10 5.5, 5.8, 6.7; 8192 x 100 -> 10
 // 8.8, 5.9, 6.2; 2000 x 4096 -> 10 27, 17, 15; 55447 x 1032 -> 32 238, 136, 114.) The depth is cut until there are four CTAs per
 // SM, of four chunks at least (2000 x 4096 -> 10: two per SM 17, one 23).
-NarrowPlan narrow_plan(int rows, int depth) {
+NarrowPlan narrow_plan(int rows, int cols, int depth) {
     NarrowPlan p;
-    auto tiles_of = [&](int tm) { return ((long)rows + kThreads / 4 * tm - 1) / (kThreads / 4 * tm); };
+    const long across = (cols + 31L) / 32;
+    auto tiles_of = [&](int tm) { return ((long)rows + kThreads / 4 * tm - 1) / (kThreads / 4 * tm) * across; };
     p.tm = 1;
-    while (p.tm < 4 && (tiles_of(p.tm) > kSms || (rows >= 256 * p.tm && (long)rows * depth >= 1 << 20))) p.tm *= 2;
+    while (p.tm < 4 && (tiles_of(p.tm) > kSms || (rows >= 256 * p.tm && across * rows * depth >= 1 << 20))) p.tm *= 2;
     p.chunks = (int)((depth + kDepth - 1L) / kDepth);
     const long tiles = tiles_of(p.tm), want = (4 * kSms + tiles - 1) / tiles, most = p.chunks < 4 ? 1 : p.chunks / 4;
     const int splits = (int)(want < most ? want : most);

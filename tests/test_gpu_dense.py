@@ -63,7 +63,9 @@ def test_linear_forward_and_backward(size, dtype):
 
 # one to four rows per thread, 16 and 32 columns, a depth that ends inside a chunk, cut or not, rows of whole words and others
 @pytest.mark.parametrize("size", [(17, 1, 1), (24, 100, 32), (100, 3445, 10), (400, 4100, 17), (2000, 768, 31), (5000, 1030, 20),
-                                  (700, 5, 3), (40000, 36, 32), (20001, 33, 16), (513, 32, 16), (129, 4096, 32)],
+                                  (700, 5, 3), (40000, 36, 32), (20001, 33, 16), (513, 32, 16), (129, 4096, 32),
+                                  # little of everything
+                                  (19, 184, 186), (64, 64, 64), (100, 1000, 33), (24, 600, 1001), (512, 64, 512)],
                          ids=lambda s: "x".join(map(str, s)))
 @pytest.mark.parametrize("act", ["none", "gelu"])
 def test_linear_few_outputs_in_float32(size, act):
