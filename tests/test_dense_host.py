@@ -47,7 +47,7 @@ def test_dimensions_beyond_the_index_range_are_refused():
 
 def test_linear_pointers_and_workspaces_that_are_refused():
     lib = _lib()
-    dp = _abi.desc_pointer(_abi.QkLinearDesc(64, 64, 64, _abi.QK_F32, _abi.QK_ACT_SILU, 0))
+    dp = _abi.desc_pointer(_abi.QkLinearDesc(640, 640, 640, _abi.QK_F32, _abi.QK_ACT_SILU, 0))
     one = ctypes.c_void_p(256)
     big = 1 << 40
     for x, w, y in ((None, one, one), (one, None, one), (one, one, None)):
