@@ -41,6 +41,16 @@ __device__ __forceinline__ void split3(float x, float y, unsigned& h, unsigned& 
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(l) : "f"(y), "f"(x));
 }
 
+// x = h + m to within 2^-15 of x, for products that add both parts' to one sum. An infinity in the other operand has to give
+// an infinity there and not inf - inf or 0 * inf: so h is cut off, which leaves m the sign of x, and m is not zero beside an h
+// that is not (2^-24 of it, for |h| from 2^-109 on). Beside an infinite h m is infinite too.
+__device__ __forceinline__ void split2(float x, float y, unsigned& h, unsigned& m) {
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(y), "f"(x));
+    auto rest = [](float v, float cut) { return copysignf(fmaxf(fabsf(v - cut), fabsf(cut) * 0x1p-24f), v); };
+    x = rest(x, __uint_as_float(h << 16)), y = rest(y, __uint_as_float(h & 0xffff0000u));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(m) : "f"(y), "f"(x));
+}
+
 template <typename IO>
 __device__ __forceinline__ void load8(const void* p, size_t at, bool vec, int n, float (&v)[8]) {
     const IO* s = static_cast<const IO*>(p) + at;
@@ -112,17 +122,14 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const PrepArgsL a) {
                 out[plane / 8] = make_uint4(m[0], m[1], m[2], m[3]);
                 out[plane / 4] = make_uint4(l[0], l[1], l[2], l[3]);
             } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(h[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
                 if (j.two) {
                     unsigned m[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        // of an infinity or a NaN nothing is left
-                        const float x = v[2 * i] - __uint_as_float(h[i] << 16), y = v[2 * i + 1] - __uint_as_float(h[i] & 0xffff0000u);
-                        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(m[i]) : "f"(isfinite(y) ? y : 0.f), "f"(isfinite(x) ? x : 0.f));
-                    }
+                    for (int i = 0; i < 4; ++i) split2(v[2 * i], v[2 * i + 1], h[i], m[i]);
                     out[plane / 8] = make_uint4(m[0], m[1], m[2], m[3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(h[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
                 }
             }
             out[0] = make_uint4(h[0], h[1], h[2], h[3]);
