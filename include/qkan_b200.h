@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define QK_ABI_VERSION 5
+#define QK_ABI_VERSION 6
 
 enum QkDtype { QK_F32 = 0, QK_BF16 = 1 };
 
@@ -238,13 +238,19 @@ enum QkActivation {
     QK_ACT_SIGMOID = 6
 };
 
+enum QkLinearFlags {
+    /* bfloat16 backward with an activation: gz rounded to bfloat16 before its two products, as in a framework that stores
+     * it. Half the products' time, and sqrt 2 of the rounding error of grad_x and grad_weight. */
+    QK_LINEAR_ROUND_GRADS = 2
+};
+
 typedef struct QkLinearDesc {
     int32_t rows;         /* M */
     int32_t in_features;  /* K */
     int32_t out_features; /* N */
     int32_t io_dtype;     /* QkDtype of every tensor but the tape */
     int32_t activation;   /* QkActivation */
-    uint32_t flags;       /* 0 */
+    uint32_t flags;       /* QkLinearFlags */
 } QkLinearDesc;
 
 /*
@@ -262,7 +268,7 @@ int qk_linear_forward(const QkLinearDesc* desc, const void* x, const void* weigh
 
 /*
  * With gz = grad_y * act'(tape): grad_x (M,K) = gz weight, grad_weight (N,K) = gz^T x, grad_bias (N) = column sums of
- * gz. Any of the three may be NULL; x and weight are read only by the gradient that needs them. The gradient of the
+ * gz, which has 16 significant bits at least unless QK_LINEAR_ROUND_GRADS says otherwise. Any of the three may be NULL; x and weight are read only by the gradient that needs them. The gradient of the
  * residual is grad_y itself.
  */
 size_t qk_linear_backward_workspace_bytes(const QkLinearDesc* desc);

@@ -10,7 +10,7 @@ import importlib.util
 import os
 from ctypes import Structure, c_char_p, c_float, c_int, c_int32, c_size_t, c_uint32, c_void_p
 
-QK_ABI_VERSION = 5
+QK_ABI_VERSION = 6
 
 QK_F32 = 0
 QK_BF16 = 1
@@ -22,6 +22,7 @@ ANSATZ_CODES = {"pz_encoding": QK_ANSATZ_PZ, "pz": QK_ANSATZ_PZ, "rpz_encoding":
                 "rpz": QK_ANSATZ_RPZ, "real": QK_ANSATZ_REAL}
 
 (QK_ACT_NONE, QK_ACT_SILU, QK_ACT_GELU, QK_ACT_GELU_TANH, QK_ACT_RELU, QK_ACT_TANH, QK_ACT_SIGMOID) = range(7)
+QK_LINEAR_ROUND_GRADS = 2
 # the names of layer.make_base_activation, and "none"
 ACTIVATION_CODES = {"none": QK_ACT_NONE, "silu": QK_ACT_SILU, "swish": QK_ACT_SILU, "gelu": QK_ACT_GELU,
                     "gelu_exact": QK_ACT_GELU, "gelu_tanh": QK_ACT_GELU_TANH, "relu": QK_ACT_RELU,

@@ -6,7 +6,7 @@
 //
 // Functions of the module (positional arguments only; functional.py has the public ones):
 //   linear_forward(x, weight, bias, residual, activation, want_tape) -> (y, tape)
-//   linear_backward(x, weight, gy, tape, activation, want) -> (gx, gw, gb)
+//   linear_backward(x, weight, gy, tape, activation, want, round_grads) -> (gx, gw, gb)
 //   norm_forward(x, weight, bias, eps, want_stats) -> (y, stats)
 //   norm_backward(x, weight, stats, gy, want, param_dtype) -> (gx, gw, gb)
 // `want` has bit 0 for x, 1 for the weight, 2 for the bias; what is not wanted comes back as None.
@@ -199,8 +199,9 @@ PyObject* linear_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 PyObject* linear_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    argument_count(n, 6, "linear_backward");
+    argument_count(n, 7, "linear_backward");
     LinearCall c(args[0], args[1], args[4]);
+    if (truth_arg(args[6])) c.desc.flags |= QK_LINEAR_ROUND_GRADS;
     Tensor gy = tensor_arg(args[2], "gy"), tape = optional_arg(args[3], "tape");
     const long want = int_arg(args[5]);
     check_like(gy, "gy", c.shape, c.dtype, c.x.device());

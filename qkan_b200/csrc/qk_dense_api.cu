@@ -23,7 +23,7 @@ int check_linear(const QkLinearDesc* d) {
     if (!is_dtype(d->io_dtype)) return fail(QK_ERR_BAD_ARGUMENT, "io_dtype %d is neither QK_F32 nor QK_BF16", d->io_dtype);
     if (d->activation < QK_ACT_NONE || d->activation > QK_ACT_SIGMOID)
         return fail(QK_ERR_BAD_ARGUMENT, "activation %d is not a QkActivation value", d->activation);
-    if (d->flags) return fail(QK_ERR_BAD_ARGUMENT, "unknown flag bits 0x%x", d->flags);
+    if (d->flags & ~(uint32_t)QK_LINEAR_ROUND_GRADS) return fail(QK_ERR_BAD_ARGUMENT, "unknown flag bits 0x%x", d->flags);
     return QK_OK;
 }
 
@@ -127,6 +127,7 @@ int qk_linear_backward(const QkLinearDesc* desc, const void* x, const void* weig
     if (rc) return rc;
     qk::LinearArgs a{};
     a.rows = d.rows, a.in = d.in_features, a.out = d.out_features, a.act = d.activation, a.io_dtype = d.io_dtype;
+    a.flags = d.flags;
     a.x = x, a.w = weight, a.tape = const_cast<void*>(tape), a.gy = gy;
     a.gx = gx, a.gw = gw, a.gb = gb, a.scratch = ws;
     const cudaError_t e = qk::launch_linear_backward(a, st);

@@ -346,11 +346,12 @@ ForwardScratch plan_forward(const QkLinearDesc& d) {
 // The layout is that of all gradients, whatever is asked for. grad_bias: the sums of gz's columns come from the products
 // (the tensor core sums gz as it makes grad_weight) where nothing else needs to go over gz, else from prepare.
 //
-// gz in bfloat16: where it is not gy itself it has to be rounded. To bfloat16 where there is much of it, as a framework
-// that stores gz has it: over many values that error is as large as the one of rounding the gradients, so theirs is sqrt 2
-// of what it would be. Over few values it can be up to twice: those are taken in two parts, products of twice the depth
-// (1501 x 517 -> 333: 40 against 33 us for the training step). Few rows have gz in float32.
-constexpr long kTwoPartsMost = 1 << 18;  // values of gz
+// gz in bfloat16: where it is not gy itself it is taken in two parts, products of twice the depth, so that the gradients
+// carry the rounding of their own type alone. Rounded to bfloat16 once, as a framework that stores gz has it, its error is as
+// large as that of rounding the gradients, whatever the depth: theirs is 1.41 times as large then (measured at 800 x 72 ->
+// 400 and 8192 x 4096 -> 4096), or up to twice where one term makes the sum. The caller can ask for that
+// (QK_LINEAR_ROUND_GRADS); all gradients with SiLU then take, in us, 500 for 856 at 8192 x 4096 -> 4096, 68 for 85 at
+// 65536 x 256 -> 256, 16.6 for 18.7 at 1501 x 517 -> 333. Few rows have gz in float32.
 struct BackwardScratch {
     Plan plan_w, plan_x;
     bool two;       // gz in two parts
@@ -371,7 +372,7 @@ BackwardScratch plan_backward(const QkLinearDesc& d) {
         s.total = align256((size_t)s.few.slabs * M * K * 4);  // partial sums of grad_x
         return s;
     }
-    s.two = d.activation != QK_ACT_NONE && planes == 1 && M * N <= kTwoPartsMost;
+    s.two = d.activation != QK_ACT_NONE && planes == 1 && !(d.flags & QK_LINEAR_ROUND_GRADS);
     const int times = s.two ? 2 : 1;
     s.together = K > 0 && plan_pair({N, K, times * blocks_of(M)}, {M, K, times * blocks_of(N)}, planes, &s.plan_w, &s.plan_x);
     if (!pack_gz && s.plan_w.bn > 128) {
@@ -407,7 +408,8 @@ const S& remembered(const QkLinearDesc& d) {
     static thread_local int next = 0;
     for (auto& k : kept)
         if (k.set && k.desc.rows == d.rows && k.desc.in_features == d.in_features &&
-            k.desc.out_features == d.out_features && k.desc.io_dtype == d.io_dtype && k.desc.activation == d.activation)
+            k.desc.out_features == d.out_features && k.desc.io_dtype == d.io_dtype && k.desc.activation == d.activation &&
+            k.desc.flags == d.flags)
             return k.s;
     auto& k = kept[next];
     next = (next + 1) % kKept;
@@ -536,7 +538,7 @@ cudaError_t launch_linear_forward(const LinearArgs& a, cudaStream_t st) {
 
 cudaError_t launch_linear_backward(const LinearArgs& a, cudaStream_t st) {
     const int M = a.rows, K = a.in, N = a.out;
-    const QkLinearDesc d{M, K, N, a.io_dtype, a.act, 0};
+    const QkLinearDesc d{M, K, N, a.io_dtype, a.act, a.flags};
     const BackwardScratch& s = backward_scratch(d);
     char* ws = static_cast<char*>(a.scratch);
     ReduceArgs red{};

@@ -108,6 +108,7 @@ cudaError_t launch_narrow(const NarrowArgs& a, cudaStream_t st);
 // ---- the map (qk_linear.cu) ----------------------------------------------------
 struct LinearArgs {
     int rows, in, out, act, io_dtype;
+    uint32_t flags;
     const void* x;
     const void* w;
     const void* bias;

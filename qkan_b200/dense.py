@@ -14,16 +14,18 @@ from . import functional as qf
 
 
 class Linear(nn.Linear):
-    """``act(x weight^T + bias) + residual`` as one kernel."""
+    """``act(x weight^T + bias) + residual`` as one kernel. ``round_grads``: as in ``functional.linear_backward``."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None,
-                 activation: str = "none"):
+                 activation: str = "none", round_grads: bool = False):
         super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
         qf._activation_code(activation)
         self.activation = activation
+        self.round_grads = bool(round_grads)
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-        return qf.fused_linear(x, self.weight, self.bias, activation=self.activation, residual=residual)
+        return qf.fused_linear(x, self.weight, self.bias, activation=self.activation, residual=residual,
+                               round_grads=self.round_grads)
 
     def extra_repr(self) -> str:
         return super().extra_repr() + ("" if self.activation == "none" else f", activation={self.activation}")

@@ -535,20 +535,23 @@ def linear_forward(x, weight, bias=None, *, activation="none", residual=None, re
     return out if return_tape else out[0]
 
 
-def linear_backward(x, weight, gy, *, tape=None, activation="none", want=_GRADS) -> dict:
+def linear_backward(x, weight, gy, *, tape=None, activation="none", want=_GRADS, round_grads: bool = False) -> dict:
     """Gradients of ``sum(linear_forward(x, weight, bias, ...) * gy)`` by name; the residual's is ``gy`` itself.
 
-    ``tape`` is what the forward returned with the same ``activation``.
+    ``tape`` is what the forward returned with the same ``activation``. ``round_grads=True`` (bfloat16 with an activation;
+    no effect otherwise) rounds ``gy * act'(z)`` to bfloat16 before the two products: half their time, 1.4 times the
+    gradients' rounding error.
     """
-    return _named(_abi.dense().linear_backward(x, weight, gy, tape, _activation_code(activation), _want_bits(want)), want)
+    grads = _abi.dense().linear_backward(x, weight, gy, tape, _activation_code(activation), _want_bits(want), round_grads)
+    return _named(grads, want)
 
 
 class _LinearFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, code):
+    def forward(ctx, x, weight, bias, residual, code, round_grads):
         y, tape = _abi.dense().linear_forward(x, weight, bias, residual, code, True)
         ctx.save_for_backward(x, weight, tape)
-        ctx.code = code
+        ctx.code, ctx.round_grads = code, round_grads
         return y
 
     @staticmethod
@@ -557,20 +560,21 @@ class _LinearFunction(torch.autograd.Function):
         x, weight, tape = ctx.saved_tensors
         need = ctx.needs_input_grad
         want = need[0] + 2 * need[1] + 4 * need[2]
-        grads = _abi.dense().linear_backward(x, weight, gy, tape, ctx.code, want) if want else (None, None, None)
-        return (*grads, gy if need[3] else None, None)
+        grads = (_abi.dense().linear_backward(x, weight, gy, tape, ctx.code, want, ctx.round_grads) if want
+                 else (None, None, None))
+        return (*grads, gy if need[3] else None, None, None)
 
 
-def fused_linear(x, weight, bias=None, *, activation="none", residual=None) -> torch.Tensor:
+def fused_linear(x, weight, bias=None, *, activation="none", residual=None, round_grads: bool = False) -> torch.Tensor:
     """Differentiable ``act(x weight^T + bias) + residual`` as one kernel (``linear_forward`` / ``linear_backward``).
 
     ``activation``: the names of ``layer.make_base_activation``, or "none". With a residual this is the closing
     projection of a pre-norm block, without one the projections of the reference's ``FusedHQKAN``
-    (``src/qkan/solver/cute/cute_ops.py:449-490``).
+    (``src/qkan/solver/cute/cute_ops.py:449-490``). ``round_grads``: as in ``linear_backward``.
     """
     code = _activation_code(activation)
     if _wants_grad(x, weight, bias, residual):
-        return _LinearFunction.apply(x, weight, bias, residual, code)
+        return _LinearFunction.apply(x, weight, bias, residual, code, round_grads)
     return _abi.dense().linear_forward(x, weight, bias, residual, code, False)[0]
 
 
