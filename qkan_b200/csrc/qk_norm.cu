@@ -5,7 +5,8 @@
 //   grad_w = sum over rows of gy * xh                  grad_b = sum over rows of gy
 //
 // Bound by memory: 2 M D elements forward, 3 M D backward. So each row is read once: T threads hold it in registers, E
-// elements each, take the mean, then the squares about the mean (no cancellation, whatever the row's offset), and write.
+// elements each, take the mean, then the squares about the mean, and write. Both directions take x - mean first, which for
+// values near the mean is exact (x * rstd - mean * rstd would round mean * rstd, an error that grows with the row's offset).
 // A fixed set of CTAs walks the rows, so that weight and bias, and in the backward the threads' own columns of grad_w and
 // grad_b, stay in registers; one partial row per CTA goes to scratch, and a second launch adds those in order (no
 // atomics: the same bits every run). The next row is fetched before the current one is worked on.
@@ -120,6 +121,12 @@ __device__ __forceinline__ void load_params(const void* p, int dtype, int c, flo
     }
 }
 
+// sum / dim, correctly rounded but for rare last bits, so that the mean of a constant row is that constant; `inv` is 1 / dim
+__device__ __forceinline__ float mean_of(float sum, float dim, float inv) {
+    const float m = sum * inv;
+    return fmaf(fmaf(-m, dim, sum), inv, m);
+}
+
 // Sums over the T threads of a group. Two buffers used in turn make one barrier per sum enough: who writes a buffer
 // again has passed the barrier of the sum between, behind which nobody reads it any more.
 template <int T>
@@ -184,7 +191,7 @@ __global__ void __launch_bounds__(block_of(T), 512 / block_of(T)) norm_forward_k
         if (row + step < a.rows) p.load(xs + (row + step) * a.dim, a.dim, lane);
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) s = add2(s, x[i]);  // columns past the end hold zeros
-        const float mean = sum(make_float2(s.x + s.y, 0.f)).x * inv;
+        const float mean = mean_of(sum(make_float2(s.x + s.y, 0.f)).x, (float)a.dim, inv);
         f2 q = pk(0.f);
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) {
@@ -231,15 +238,17 @@ __global__ void __launch_bounds__(block_of(T), 512 / block_of(T)) norm_backward_
         f2 xh[E / 2], g[E / 2], s1 = pk(0.f), s2 = pk(0.f);
         px.unpack(xh);
         pg.unpack(g);
-        const f2 rstd = pk(st.y), shift = pk(-st.x * st.y);
+        const f2 rstd = pk(st.y);
+        const float mean = st.x;
         if (row + step < a.rows) {
             px.load(xs + (row + step) * a.dim, a.dim, lane);
             pg.load(gys + (row + step) * a.dim, a.dim, lane);
             st = a.stats[row + step];
         }
-        // past the end gy is zero, and so is all that it is a factor of
+        // past the end gy is zero, and so is all that it is a factor of, as long as xh there is finite: so x stays zero there
+        auto shift_of = [&](int e) { return (e / VEC * T + lane) * VEC < a.dim ? -mean : 0.f; };
         auto pair = [&](int i, f2 weight) {
-            xh[i] = fma2(xh[i], rstd, shift);
+            xh[i] = mul2(add2(xh[i], make_float2(shift_of(2 * i), shift_of(2 * i + 1))), rstd);
             dw[i] = fma2(g[i], xh[i], dw[i]);
             db[i] = add2(db[i], g[i]);
             g[i] = mul2(g[i], weight);

@@ -119,3 +119,85 @@ def test_rounding_of_the_gradients_is_the_callers_choice():
         _, tape = F.linear_forward(a, b, activation=act, return_tape=True)
         plain, fast = (F.linear_backward(a, b, g, tape=tape, activation=act, round_grads=r) for r in (False, True))
         assert all(torch.equal(plain[k], fast[k]) for k in plain)
+
+
+# ---------------------------------------------------------------- layer norm of rows far from zero
+DTYPES = [torch.float32, torch.bfloat16]
+STEP = 2.0 ** -24
+HALF = 2.0 ** -8  # of a bfloat16 result
+
+
+def _norm_gradients64(xh, rstd, w, gy):
+    """Gradients and the sizes of what they are made of, from the exact normalised rows."""
+    gw = gy if w is None else gy * w
+    m1, m2 = gw.mean(-1, keepdim=True), (gw * xh).mean(-1, keepdim=True)
+    size = rstd * (gw.abs() + gw.abs().mean(-1, keepdim=True) + xh.abs() * (gw * xh).abs().mean(-1, keepdim=True))
+    return rstd * (gw - m1 - xh * m2), size
+
+
+def _close(got, want, bound, what):
+    d = (got.double() - want).abs() - bound
+    assert torch.isfinite(got).all() and float(d.max()) <= 0, f"{what}: {float(d.max()):.3e} beyond its bound"
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16"])
+@pytest.mark.parametrize("D", [2, 96, 768, 1000, 1024, 2052, 5000, 8191, 9000])
+@pytest.mark.parametrize("value", [3.0, -1000.0, 3300.0, 1e4, 2.0 ** 120])
+def test_layer_norm_of_constant_rows_is_its_bias(value, D, dtype):
+    """The sum of a constant row is exact here (few bits), so its mean is the constant, and nothing is left of x - mean."""
+    if value > 1e30 and D > 128:
+        pytest.skip("the sum is beyond float32")
+    M = 6
+    x = torch.full((M, D), value, dtype=dtype, device="cuda")
+    w, b, gy = (_randn(*s, seed=k, dtype=dtype) for k, s in enumerate(((D,), (D,), (M, D))))
+    y, stats = F.layer_norm_forward(x, w, b)
+    assert torch.equal(y, b.expand(M, D))
+    assert torch.equal(stats[:, 0], x[:, 0].float())
+    g = F.layer_norm_backward(x, w, stats, gy)
+    assert not g["weight"].any()
+    want, size = _norm_gradients64(torch.zeros(M, D, device="cuda").double(), 1e-5 ** -0.5, w.double(), gy.double())
+    # sums of up to 64 additions in a row, a few operations around them
+    _close(g["x"], want, 72 * STEP * size + (HALF * want.abs() if dtype == torch.bfloat16 else 0), "grad x")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16"])
+@pytest.mark.parametrize("D", [2, 96, 768, 1000, 1024, 2052, 5000, 8190, 9000])
+def test_layer_norm_far_from_zero_is_as_exact_as_near(D, dtype):
+    """Whole numbers on both sides of a mean that is one: sums, mean and variance's sum are exact, so that what is left
+    are the roundings of rstd (4 steps) and of two products. A variance as E[x^2] - mean^2, or x * rstd - mean * rstd, would be off
+    by the mean's square or the mean itself instead."""
+    M = 40
+    mean = 192 if dtype == torch.bfloat16 else 1500  # bfloat16 holds whole numbers up to 256
+    g = torch.Generator().manual_seed(D)
+    k = torch.randint(1, 8, (M, D // 2), generator=g)
+    x = torch.stack((mean + k, mean - k), -1).view(M, D).to(dtype).cuda()
+    w, b, gy = (_randn(*s, seed=j, dtype=dtype) for j, s in enumerate(((D,), (D,), (M, D))))
+    dev = x.double() - mean
+    rstd = 1 / torch.sqrt((dev * dev).mean(-1, keepdim=True) + 1e-5)
+    xh = dev * rstd
+    half = dtype == torch.bfloat16
+    y, stats = F.layer_norm_forward(x, w, b)
+    want = xh * w.double() + b.double()
+    _close(y, want, 8 * STEP * (xh * w.double()).abs() + 2 * STEP * want.abs() + (HALF * want.abs() if half else 0), "y")
+    assert bool((stats[:, 0] == mean).all())
+    got = F.layer_norm_backward(x, w, stats, gy)
+    want, size = _norm_gradients64(xh, rstd, w.double(), gy.double())
+    _close(got["x"], want, 80 * STEP * size + (HALF * want.abs() if half else 0), "grad x")
+    want = (gy.double() * xh).sum(0)
+    _close(got["weight"], want, (M + 8) * STEP * (gy.double() * xh).abs().sum(0) + (HALF * want.abs() if half else 0), "grad weight")
+
+
+def test_bounds_of_the_far_rows_tell_a_naive_variance_and_zeros():
+    """The rows above, computed the ways that they are to tell apart, in float32 by torch."""
+    mean, D = 1500.0, 768
+    k = torch.randint(1, 8, (40, D // 2), generator=torch.Generator().manual_seed(D))
+    x = torch.stack((mean + k, mean - k), -1).view(40, D).float().cuda()
+    dev = x.double() - mean
+    rstd = 1 / torch.sqrt((dev * dev).mean(-1, keepdim=True) + 1e-5)
+    xh = dev * rstd
+    bound = 10 * STEP * xh.abs()
+    naive = (x - mean) * torch.rsqrt((x * x).mean(-1, keepdim=True) - mean * mean + 1e-5)
+    spread = x * rstd.float() - mean * rstd.float()
+    for wrong in (naive, spread, torch.zeros_like(x)):
+        assert float(((wrong.double() - xh).abs() - bound).max()) > 0
+    _close((x - mean) * rstd.float(), xh, bound, "as the kernels take it")
