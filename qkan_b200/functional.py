@@ -10,6 +10,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _abi
 
@@ -512,8 +513,21 @@ def _named(grads, want) -> dict:
     return {name: grads[_GRADS.index(name)] for name in want}
 
 
+def _has_tangent(*tensors) -> bool:
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a call has to go through its autograd function: for a gradient, or for a forward-mode tangent, which the
+    function refuses (the binding works below autograd and would drop it)."""
+    recorded = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    return recorded or _has_tangent(*tensors)
+
+
+def _refuse_tangent(gy) -> None:
+    if _has_tangent(gy):
+        raise RuntimeError("the dense operators have no forward-mode AD: grad_y has a tangent")
 
 
 def dense_status() -> None:
@@ -557,6 +571,7 @@ class _LinearFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
+        _refuse_tangent(gy)
         x, weight, tape = ctx.saved_tensors
         need = ctx.needs_input_grad
         want = need[0] + 2 * need[1] + 4 * need[2]
@@ -607,6 +622,7 @@ class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
+        _refuse_tangent(gy)
         x, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
         return (*_abi.dense().norm_backward(x, weight, stats, gy, need[0] + 2 * need[1] + 4 * need[2], ctx.bias_dtype), None)
