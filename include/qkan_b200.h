@@ -277,6 +277,28 @@ int qk_linear_backward(const QkLinearDesc* desc, const void* x, const void* weig
                        size_t workspace_bytes, void* cuda_stream);
 
 /*
+ * How a product of the linear map would be run, for tests and tuning: a function of the descriptor alone, nothing is
+ * launched. product: 0 the forward's, 1 grad_weight's, 2 grad_x's, both gradients being wanted.
+ */
+enum QkLinearPath {
+    QK_LINEAR_NOTHING = 0,  /* an axis is empty */
+    QK_LINEAR_FEW_ROWS = 1, /* one pass over the weight */
+    QK_LINEAR_SMALL = 2,    /* float32 as it is: few outputs, or little of everything */
+    QK_LINEAR_TENSOR = 3    /* tiles of 128 rows on the tensor cores; the other fields are about those */
+};
+typedef struct QkLinearPlan {
+    int32_t path;
+    int32_t tile_cols; /* 64, 128 or 256 */
+    int32_t slices;    /* of the depth */
+    int32_t blocks;    /* of 64 of the depth, per slice */
+    int32_t units;     /* tiles x slices, shared by 148 SMs */
+    int32_t paired;    /* one launch for both gradients */
+    int32_t gz_parts;  /* 1 or 2 (bfloat16), 3 (float32) */
+    int32_t sums_bias; /* grad_bias comes with grad_weight's product */
+} QkLinearPlan;
+int qk_linear_plan(const QkLinearDesc* desc, int product, QkLinearPlan* plan);
+
+/*
  * The linear map's kernels bound every wait inside them. QK_OK if none ran out on the current device since the last
  * call, QK_ERR_LAUNCH otherwise (results since then are not valid). Synchronises `cuda_stream`; not for captures.
  */

@@ -23,6 +23,7 @@ ANSATZ_CODES = {"pz_encoding": QK_ANSATZ_PZ, "pz": QK_ANSATZ_PZ, "rpz_encoding":
 
 (QK_ACT_NONE, QK_ACT_SILU, QK_ACT_GELU, QK_ACT_GELU_TANH, QK_ACT_RELU, QK_ACT_TANH, QK_ACT_SIGMOID) = range(7)
 QK_LINEAR_ROUND_GRADS = 2
+QK_LINEAR_NOTHING, QK_LINEAR_FEW_ROWS, QK_LINEAR_SMALL, QK_LINEAR_TENSOR = range(4)
 # the names of layer.make_base_activation, and "none"
 ACTIVATION_CODES = {"none": QK_ACT_NONE, "silu": QK_ACT_SILU, "swish": QK_ACT_SILU, "gelu": QK_ACT_GELU,
                     "gelu_exact": QK_ACT_GELU, "gelu_tanh": QK_ACT_GELU_TANH, "relu": QK_ACT_RELU,
@@ -67,6 +68,7 @@ SYMBOLS = {
     "qk_linear_forward": (c_int, [_P] * 7 + [_P, c_size_t, _P]),
     "qk_linear_backward_workspace_bytes": (c_size_t, [_P]),
     "qk_linear_backward": (c_int, [_P] * 8 + [_P, c_size_t, _P]),
+    "qk_linear_plan": (c_int, [_P, c_int, _P]),
     "qk_dense_status": (c_int, [_P]),
     "qk_layer_norm_forward": (c_int, [_P] * 7),
     "qk_layer_norm_backward_workspace_bytes": (c_size_t, [_P]),
@@ -101,6 +103,11 @@ class QkLinearDesc(Structure):
         ("activation", c_int32),
         ("flags", c_uint32),
     ]
+
+
+class QkLinearPlan(Structure):
+    _fields_ = [(name, c_int32) for name in ("path", "tile_cols", "slices", "blocks", "units", "paired", "gz_parts",
+                                             "sums_bias")]
 
 
 class QkNormDesc(Structure):
@@ -189,4 +196,4 @@ def desc_pointer(desc: Structure):
 
 
 __all__ = [name for name in dir() if name.startswith("QK") or name in (
-    "QkDesc", "QkLinearDesc", "QkNormDesc", "QkanLibraryError", "ANSATZ_CODES", "ACTIVATION_CODES", "load", "dense", "last_error", "check", "desc_pointer", "SYMBOLS", "LIB_PATH")]
+    "QkDesc", "QkLinearDesc", "QkLinearPlan", "QkNormDesc", "QkanLibraryError", "ANSATZ_CODES", "ACTIVATION_CODES", "load", "dense", "last_error", "check", "desc_pointer", "SYMBOLS", "LIB_PATH")]

@@ -134,6 +134,14 @@ int qk_linear_backward(const QkLinearDesc* desc, const void* x, const void* weig
     return e == cudaSuccess ? QK_OK : cuda_fail(e, "linear backward launch");
 }
 
+int qk_linear_plan(const QkLinearDesc* desc, int product, QkLinearPlan* plan) {
+    const int rc = check_linear(desc);
+    if (rc) return rc;
+    if (product < 0 || product > 2 || !plan) return fail(QK_ERR_BAD_ARGUMENT, "product %d is none of 0, 1, 2, or plan is NULL", product);
+    *plan = qk::linear_plan(*desc, product);
+    return QK_OK;
+}
+
 int qk_dense_status(void* stream) {
     unsigned n = 0;
     const cudaError_t e = qk::gemm_gave_up(&n, static_cast<cudaStream_t>(stream));

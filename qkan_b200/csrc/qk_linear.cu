@@ -275,20 +275,21 @@ Plan plan_for(const Size& s, int planes, double* cost = nullptr, long most_units
 }
 
 // Two products in one launch: where both fit the SMs side by side, that costs the longer of the two, not the sum.
-// False: one after the other is cheaper.
-bool plan_pair(const Size& a, const Size& b, int planes, Plan* pa, Plan* pb) {
+// False: one after the other is cheaper. Tiles have at most `most_bn` columns.
+bool plan_pair(const Size& a, const Size& b, int planes, Plan* pa, Plan* pb, double* cost, int most_bn = 256) {
     double ca, cb;
-    *pa = plan_for(a, planes, &ca);
-    *pb = plan_for(b, planes, &cb);
+    *pa = plan_for(a, planes, &ca, 0, 0, most_bn);
+    *pb = plan_for(b, planes, &cb, 0, 0, most_bn);
     double least = ca + cb;
     bool together = false;
-    for (int bn = planes == 3 ? 128 : 256; bn >= 64; bn /= 2)
+    for (int bn = planes == 3 || most_bn < 256 ? 128 : 256; bn >= 64; bn /= 2)
         for (int first = kSms / 8; first < kSms; first += kSms / 8) {
             double ta, tb;
             const Plan qa = plan_for(a, planes, &ta, first, bn), qb = plan_for(b, planes, &tb, kSms - first, bn);
             const double t = ta > tb ? ta : tb;
             if (t < least) least = t, *pa = qa, *pb = qb, together = true;
         }
+    *cost = least;
     return together;
 }
 
@@ -374,13 +375,18 @@ BackwardScratch plan_backward(const QkLinearDesc& d) {
     }
     s.two = d.activation != QK_ACT_NONE && planes == 1 && !(d.flags & QK_LINEAR_ROUND_GRADS);
     const int times = s.two ? 2 : 1;
-    s.together = K > 0 && plan_pair({N, K, times * blocks_of(M)}, {M, K, times * blocks_of(N)}, planes, &s.plan_w, &s.plan_x);
+    const Size size_w{N, K, times * blocks_of(M)}, size_x{M, K, times * blocks_of(N)};
+    double least = 0;
+    s.together = K > 0 && plan_pair(size_w, size_x, planes, &s.plan_w, &s.plan_x, &least);
     if (!pack_gz && s.plan_w.bn > 128) {
-        // narrower tiles, whose product can sum gz, against another pass over gz
-        double wide, narrow;
-        plan_for({N, K, blocks_of(M)}, planes, &wide);
-        const Plan p = plan_for({N, K, blocks_of(M)}, planes, &narrow, 0, 0, 128);
-        if (narrow < wide + 5000 + 2.0 * M * N / (kSms * 16)) s.plan_w = p, s.together = false;
+        // Narrower tiles, whose product can sum gz, save the pass over gz: both products in one launch with such tiles, or
+        // grad_weight's alone with them and grad_x's as is best for it.
+        least += 5000 + 2.0 * M * N / (kSms * 16);
+        Plan w, x;
+        double cost, cost_x;
+        if (plan_pair(size_w, size_x, planes, &w, &x, &cost, 128) && cost < least) least = cost, s.plan_w = w, s.plan_x = x, s.together = true;
+        w = plan_for(size_w, planes, &cost, 0, 0, 128), x = plan_for(size_x, planes, &cost_x);
+        if (cost + cost_x < least) s.plan_w = w, s.plan_x = x, s.together = false;
     }
     s.slabs = slabs_of(M, N);
     s.sums = K > 0 && !pack_gz && s.plan_w.bn <= 128;
@@ -488,6 +494,36 @@ cudaError_t run_alone(GemmArgs& a, int which, int planes, int bn, cudaStream_t s
 }
 
 }  // namespace
+
+QkLinearPlan linear_plan(const QkLinearDesc& d, int product) {
+    QkLinearPlan p{};
+    const long M = d.rows, K = d.in_features, N = d.out_features;
+    p.gz_parts = planes_of(d.io_dtype);
+    if (M == 0 || K == 0 || N == 0) return p;
+    if (product == 0 ? few_rows(d.rows, d.io_dtype) : few_rows_backward(d.rows, d.io_dtype)) {
+        p.path = QK_LINEAR_FEW_ROWS;
+        return p;
+    }
+    if (product == 0 && is_narrow(M, N, K, d.io_dtype)) {
+        p.path = QK_LINEAR_SMALL;
+        return p;
+    }
+    p.path = QK_LINEAR_TENSOR;
+    Plan plan = {};
+    long rows = M;
+    if (product == 0) {
+        plan = forward_scratch(d).plan;
+    } else {
+        const BackwardScratch& s = backward_scratch(d);
+        plan = product == 1 ? s.plan_w : s.plan_x;
+        if (product == 1) rows = N;
+        p.paired = s.together, p.sums_bias = s.sums;
+        if (s.two) p.gz_parts = 2;
+    }
+    p.tile_cols = plan.bn, p.slices = plan.cut.splits, p.blocks = plan.cut.kper;
+    p.units = (int)(Size{rows, product == 0 ? N : K, 0}.tiles(plan.bn) * plan.cut.splits);
+    return p;
+}
 
 size_t linear_forward_scratch(const QkLinearDesc& d) {
     if (few_rows(d.rows, d.io_dtype) || d.out_features == 0 || d.in_features == 0) return 0;

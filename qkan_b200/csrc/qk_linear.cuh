@@ -122,6 +122,8 @@ struct LinearArgs {
     void* scratch;
 };
 
+// of product 0 (forward), 1 (grad_weight), 2 (grad_x)
+QkLinearPlan linear_plan(const QkLinearDesc& d, int product);
 // bytes of scratch
 size_t linear_forward_scratch(const QkLinearDesc& d);
 size_t linear_backward_scratch(const QkLinearDesc& d);

@@ -1,5 +1,9 @@
 """The dense operators' descriptors and plans without a GPU."""
 
+import ctypes
+import math
+import random
+
 from qkan_b200 import Linear, _abi
 
 
@@ -32,3 +36,47 @@ def test_flags_of_the_linear_map():
 
 def test_rounding_of_the_gradients_is_off_unless_asked_for():
     assert Linear(4, 3).round_grads is False and Linear(4, 3, round_grads=True).round_grads is True
+
+
+def _plan(product, M, K, N, dtype=_abi.QK_BF16, act=_abi.QK_ACT_NONE, flags=0):
+    plan = _abi.QkLinearPlan()
+    assert _lib().qk_linear_plan(_linear(M, K, N, dtype, act, flags), product, ctypes.byref(plan)) == _abi.QK_OK
+    return plan
+
+
+def test_plans_that_are_refused():
+    lib, plan = _lib(), _abi.QkLinearPlan()
+    for product in (-1, 3):
+        assert lib.qk_linear_plan(_linear(64, 64, 64), product, ctypes.byref(plan)) == _abi.QK_ERR_BAD_ARGUMENT
+    assert lib.qk_linear_plan(_linear(64, 64, 64), 0, None) == _abi.QK_ERR_BAD_ARGUMENT
+    assert lib.qk_linear_plan(None, 0, ctypes.byref(plan)) == _abi.QK_ERR_BAD_ARGUMENT
+    assert lib.qk_linear_plan(_linear(-1, 64, 64), 0, ctypes.byref(plan)) == _abi.QK_ERR_BAD_ARGUMENT
+    for size in ((0, 8, 8), (8, 0, 8), (8, 8, 0)):
+        for product in range(3):
+            assert _plan(product, *size).path == _abi.QK_LINEAR_NOTHING
+
+
+def _cut(plan):
+    return plan.tile_cols, plan.slices, plan.blocks
+
+
+def test_gradients_run_one_by_one_take_the_plans_that_are_best_alone():
+    """grad_x over the whole GPU has the sizes of a forward product; it is not left with the plan of a share of the SMs."""
+    rng = random.Random(5)
+    sizes = [(73, 3648, 648), (1816, 480, 888)]
+    for _ in range(600):
+        sizes.append([max(8, int(math.exp(rng.uniform(math.log(8), math.log(4096)))) // 8 * 8) for _ in range(3)])
+    alone = 0
+    for M, K, N in sizes:
+        weight, x = (_plan(p, M, K, N) for p in (1, 2))
+        assert weight.paired == x.paired and weight.sums_bias == (weight.tile_cols <= 128)
+        if x.paired:
+            assert weight.units + x.units <= 148 and weight.tile_cols == x.tile_cols, (M, K, N)
+            continue
+        alone += 1
+        assert _cut(x) == _cut(_plan(0, M, N, K)), (M, K, N)
+        if weight.tile_cols > 128:
+            assert _cut(weight) == _cut(_plan(0, N, M, K)), (M, K, N)
+    assert alone > 20
+    # a pair is not given up for narrower tiles where it is the cheaper of the two
+    assert _plan(2, 1816, 480, 888).paired
