@@ -262,7 +262,8 @@ template <typename IO>
 cudaError_t launch_few_typed(const FewArgs& a, cudaStream_t st) {
     if (a.rows <= 2) return launch_few_rows<IO, 2>(a, st);
     if (a.rows <= 4) return launch_few_rows<IO, 4>(a, st);
-    return a.rows <= 8 ? launch_few_rows<IO, 8>(a, st) : launch_few_rows<IO, 16>(a, st);
+    if constexpr (sizeof(IO) == 4) return a.rows <= 8 ? launch_few_rows<IO, 8>(a, st) : launch_few_rows<IO, 16>(a, st);
+    return cudaErrorInvalidValue;  // few_rows_backward() lets none through
 }
 
 }  // namespace

@@ -447,7 +447,7 @@ template <typename IO, int VEC, int T>
 cudaError_t run_t(const NormArgs& a, bool backward, cudaStream_t st) {
     const int need = (a.dim + T - 1) / T;  // elements per thread
     if (need <= 8) return run_e<IO, VEC, T, 8>(a, backward, st);
-    if constexpr (sizeof(IO) == 2)  // rows of whole 16-byte words that do not start on one: by element, as many of them
+    if constexpr (sizeof(IO) == 2 && T * 16 < kMaxDim)  // rows of whole 16-byte words that do not start on one: by element, as many of them
         if (need > 16 && !backward) return run_e<IO, VEC, T, 24>(a, backward, st);
     return run_e<IO, VEC, T, 16>(a, backward, st);
 }
