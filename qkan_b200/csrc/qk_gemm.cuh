@@ -42,7 +42,10 @@ constexpr int kChunk = 2;           // stages between two drains of hh (float32)
 constexpr int kGemmThreads = 352;   // copies of P, MMAs, 8 epilogue warps, copies of Q
 constexpr int kDrainWarps = 8;
 constexpr int kQWarp = 10;
-constexpr unsigned long long kGiveUpNs = 10ull * 1000 * 1000 * 1000;  // the longest that a wait may take
+// The longest that a wait may take: this time, and this many rounds of 64 tries (a try that fails takes 1.36 us, so 1.4 s).
+// The clock runs on while another process has the GPU, the tries do not.
+constexpr unsigned long long kGiveUpNs = 10ull * 1000 * 1000 * 1000;
+constexpr int kGiveUpRounds = 1 << 14;
 
 constexpr int kStoreBytes = 2048;   // 32 rows of 64 bytes: what a warp stages for one store; two of them per warp
 
@@ -116,11 +119,11 @@ __device__ __forceinline__ unsigned long long now_ns() {
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
 }
-// Waits for the phase of `parity` to end. Every wait ends: after kGiveUpNs, or once another warp has given up, the
+// Waits for the phase of `parity` to end. Every wait ends: after kGiveUpNs and kGiveUpRounds, or once another warp has given up, the
 // answer is false, and the caller leaves its loop.
 __device__ __noinline__ bool bar_wait_long(unsigned long long* b, unsigned parity, volatile int* abort) {
     const unsigned long long start = now_ns();
-    while (now_ns() - start < kGiveUpNs) {
+    for (int round = 0; round < kGiveUpRounds || now_ns() - start < kGiveUpNs; ++round) {
         for (int i = 0; i < 64; ++i)
             if (bar_try(b, parity)) return true;
         if (*abort) return false;
