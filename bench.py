@@ -927,6 +927,7 @@ def run_hqkan_block(run: Run):
     pre-norm block around it with its residual (qkan_b200.HQKANBlock) is reported beside it and is not in the value."""
     torch, args, dev, rank = run.torch, run.args, run.dev, run.rank
     from qkan_b200 import FusedHQKAN, HQKANBlock
+    from qkan_b200.functional import dense_status
     from qkan_b200.graph import make_graphed_train_step
 
     table, prenorm = [], []
@@ -949,6 +950,7 @@ def run_hqkan_block(run: Run):
         (table if kind is FusedHQKAN else prenorm).append(
             {"rows": rows, "eager_us": 1e3 * eager_ms, "graphed_us": 1e3 * graph_ms,
              "library_launches_per_step": lib_k, "all_kernels_per_step": all_k})
+    dense_status(dev)
     if rank == 0:
         edges = sum(r["rows"] for r in table) * 100
         ms = sum(r["graphed_us"] for r in table) * 1e-3

@@ -530,12 +530,14 @@ def _refuse_tangent(gy) -> None:
         raise RuntimeError("the dense operators have no forward-mode AD: grad_y has a tangent")
 
 
-def dense_status() -> None:
-    """Raise if a wait inside the linear map's kernels ran out on the current device since the last call.
+def dense_status(device=None) -> None:
+    """Raise if a wait inside the linear map's kernels ran out on ``device`` (default: the current one) since the last call.
 
-    Synchronises the current stream; results computed since then are not valid in that case.
+    Synchronises that device's current stream; results computed since then are not valid in that case. ``QKAN.train_`` asks
+    at every log step where the model has the package's ``Linear``; loops of one's own and replayed graphs should.
     """
-    _abi.check(_abi.load().qk_dense_status(torch.cuda.current_stream().cuda_stream), "qk_dense_status")
+    with torch.cuda.device(device):
+        _abi.check(_abi.load().qk_dense_status(torch.cuda.current_stream().cuda_stream), "qk_dense_status")
 
 
 def linear_forward(x, weight, bias=None, *, activation="none", residual=None, return_tape: bool = False):

@@ -20,6 +20,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from . import functional as qf
 from .dense import Linear
 from .layer import SOLVER_NAME, QKANLayer, make_base_activation
 from .parallel import get_dist_info, print0
@@ -306,6 +307,9 @@ class QKAN(nn.Module):
         if closure is None and is_lbfgs:
             closure = default_closure
 
+        # the linear map's kernels bound their waits: one that ran out raises here, not later
+        asks = any(isinstance(m, Linear) for m in self.modules())
+
         pbar = tqdm(range(steps), ncols=100, disable=not verbose)
         for step in pbar:
             self.train()
@@ -339,6 +343,8 @@ class QKAN(nn.Module):
             results["train_loss"].append(train_loss.detach().cpu().numpy())
             results["test_loss"].append(test_loss.detach().cpu().numpy())
             results["reg"].append(state["reg"].detach().cpu().numpy())
+            if asks and (step % max(log, 1) == 0 or step == steps - 1):
+                qf.dense_status(next(self.parameters()).device)
         return results
 
     # ------------------------------------------------------------------ checkpoints (rank 0 writes)

@@ -201,3 +201,15 @@ def test_bounds_of_the_far_rows_tell_a_naive_variance_and_zeros():
     for wrong in (naive, spread, torch.zeros_like(x)):
         assert float(((wrong.double() - xh).abs() - bound).max()) > 0
     _close((x - mean) * rstd.float(), xh, bound, "as the kernels take it")
+
+
+def test_status_of_a_device_and_in_training():
+    from qkan_b200 import QKAN
+
+    for device in (None, "cuda", "cuda:0", torch.device("cuda"), 0):
+        F.dense_status(device)
+    model = QKAN([6, 5, 3], is_map=True, hidden=8, fused_head=True, seed=1).to("cuda")
+    data = {k: _randn(40, 6 if k.endswith("input") else 3, seed=j) for j, k in
+            enumerate(("train_input", "train_label", "test_input", "test_label"))}
+    out = model.train_(data, steps=3, log=2, verbose=False)
+    assert len(out["train_loss"]) == 3
