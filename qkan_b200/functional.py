@@ -558,6 +558,7 @@ def linear_backward(x, weight, gy, *, tape=None, activation="none", want=_GRADS,
     no effect otherwise) rounds ``gy * act'(z)`` to bfloat16 before the two products: half their time, 1.4 times the
     gradients' rounding error.
     """
+    want = tuple(want)  # read twice
     grads = _abi.dense().linear_backward(x, weight, gy, tape, _activation_code(activation), _want_bits(want), round_grads)
     return _named(grads, want)
 
@@ -610,6 +611,7 @@ def layer_norm_backward(x, weight, stats, gy, *, want=_GRADS, param_dtype=None) 
     ``weight`` None stands for ones; the parameters' gradients have the weight's dtype, or ``param_dtype`` where there is
     no weight (default: that of ``x``).
     """
+    want = tuple(want)
     return _named(_abi.dense().norm_backward(x, weight, stats, gy, _want_bits(want), param_dtype), want)
 
 

@@ -17,7 +17,7 @@ class PlainBinding:
         return gy.detach() @ w.detach() if want & 1 else None, None, None
 
     def norm_backward(self, x, w, stats, gy, want, param_dtype):
-        return gy.detach() * 2, None, None
+        return gy.detach() * 2, *[gy.detach().sum(0) if want & bit else None for bit in (2, 4)]
 
     def norm_forward(self, x, w, b, eps, want_stats):
         return x.detach() * 2, (torch.zeros(*x.shape[:-1], 2) if want_stats else None)
@@ -74,3 +74,11 @@ def test_a_tangent_of_the_outputs_gradient_is_refused(f):
         with pytest.raises(RuntimeError, match="forward-mode AD"):
             torch.autograd.grad(y, leaf, gy, retain_graph=True)
         assert torch.autograd.grad(y, leaf, torch.ones_like(y))[0].shape == x.shape
+
+
+@pytest.mark.parametrize("want", [(), ("x",), ("weight", "x"), ("x", "weight", "bias")])
+def test_gradients_asked_for_by_any_iterable(want):
+    gy, stats = torch.randn(3, 4), torch.zeros(3, 2)
+    for form in (tuple, list, iter, lambda names: (name for name in names), dict.fromkeys):
+        assert list(F.layer_norm_backward(x, None, stats, gy, want=form(want))) == list(want)
+        assert list(F.linear_backward(x, w, torch.randn(3, 5), want=form(want))) == list(want)
