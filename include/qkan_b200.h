@@ -309,7 +309,7 @@ typedef struct QkNormDesc {
     int32_t dim;         /* D >= 1, the normalised axis */
     int32_t io_dtype;    /* QkDtype of x, y, grad_y, grad_x */
     int32_t param_dtype; /* QkDtype of weight, bias and their gradients */
-    float eps;           /* added to the variance; >= 0 */
+    float eps;           /* added to the variance; >= 0 and finite */
     uint32_t flags;      /* 0 */
 } QkNormDesc;
 

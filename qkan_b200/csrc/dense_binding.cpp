@@ -21,7 +21,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <cmath>
+#include <limits>
 #include <string>
 
 #include "../../include/qkan_b200.h"
@@ -255,7 +255,8 @@ PyObject* norm_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     NormCall c(args[0], args[1], args[2], at::kFloat, false);
     const double eps = PyFloat_AsDouble(args[3]);
     if (eps == -1.0 && PyErr_Occurred()) throw python_error();
-    TORCH_CHECK_VALUE(eps >= 0.0 && std::isfinite(eps), "eps must be finite and >= 0, got ", std::to_string(eps));
+    TORCH_CHECK_VALUE(eps >= 0.0 && eps <= std::numeric_limits<float>::max(),
+                      "eps must be >= 0 and finite in float32, got ", std::to_string(eps));
     c.desc.eps = (float)eps;
     require_cuda(c.x);
     Scope scope(c.x);

@@ -1,4 +1,5 @@
 // C ABI of the dense operators (see include/qkan_b200.h): argument validation and scratch carving.
+#include <cmath>
 #include <initializer_list>
 
 #include "qk_linear.cuh"
@@ -33,7 +34,7 @@ int check_norm(const QkNormDesc* d) {
     if (d->dim > kMost) return fail(QK_ERR_UNSUPPORTED, "dim=%d exceeds %d", d->dim, kMost);
     if (!is_dtype(d->io_dtype) || !is_dtype(d->param_dtype))
         return fail(QK_ERR_BAD_ARGUMENT, "io_dtype %d / param_dtype %d is neither QK_F32 nor QK_BF16", d->io_dtype, d->param_dtype);
-    if (!(d->eps >= 0.f)) return fail(QK_ERR_BAD_ARGUMENT, "eps must be >= 0");
+    if (!(d->eps >= 0.f) || std::isinf(d->eps)) return fail(QK_ERR_BAD_ARGUMENT, "eps must be >= 0 and finite");
     if (d->flags) return fail(QK_ERR_BAD_ARGUMENT, "unknown flag bits 0x%x", d->flags);
     return QK_OK;
 }

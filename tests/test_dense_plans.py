@@ -4,7 +4,11 @@ import ctypes
 import math
 import random
 
+import pytest
+import torch
+
 from qkan_b200 import Linear, _abi
+from qkan_b200 import functional as F
 
 
 def _lib():
@@ -80,3 +84,16 @@ def test_gradients_run_one_by_one_take_the_plans_that_are_best_alone():
     assert alone > 20
     # a pair is not given up for narrower tiles where it is the cheaper of the two
     assert _plan(2, 1816, 480, 888).paired
+
+
+def test_eps_beyond_float32_is_refused():
+    """Where eps is infinite every row would come out as the bias."""
+    for eps in (1e39, 1e300, float("inf"), float("nan"), -1e-5):
+        with pytest.raises(ValueError, match="eps"):
+            F.layer_norm(torch.zeros(2, 4), eps=eps)
+    lib, one = _lib(), ctypes.c_void_p(256)
+    desc = _abi.desc_pointer(_abi.QkNormDesc(4, 4, 0, 0, float("inf"), 0))
+    assert lib.qk_layer_norm_forward(desc, one, None, None, one, None, None) == _abi.QK_ERR_BAD_ARGUMENT
+    assert b"eps" in lib.qk_last_error()
+    with pytest.raises(RuntimeError, match="no CPU fallback"):  # the last of the checks
+        F.layer_norm(torch.zeros(2, 4), eps=3e38)
