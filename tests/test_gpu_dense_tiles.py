@@ -330,3 +330,48 @@ def test_layer_norm_by_the_depth_of_its_sums(size, offset, dtype):
             continue
         e = (M + 2) * STEP * gyd.abs().sum(0) if name == "bias" else (gyd.abs() * off).sum(0) + (M + 2) * STEP * (gyd * xh).abs().sum(0)
         within(g[name], v, e + (2.0 ** -8 * (v.abs() + e) if half else 0), f"grad {name}")
+
+
+@pytest.mark.parametrize("size", [(7, 31), (33, 768), (20, 1036), (20, 1037), (9, 4096), (4, 9000)], ids=lambda s: "x".join(map(str, s)))
+def test_layer_norm_of_float32_rows_with_bfloat16_parameters(size):
+    M, D = size
+    x, gy = _randn(M, D), _randn(M, D, seed=3)
+    w, b = _randn(D, seed=1, dtype=BF16), _randn(D, seed=2, dtype=BF16)
+    y, stats = F.layer_norm_forward(x, w, b)
+    within(y, *norm64(x, w, b)[:2], "y")
+    g = F.layer_norm_backward(x, w, stats, gy)
+    assert g["weight"].dtype == g["bias"].dtype == BF16 and g["x"].dtype == F32
+    for k, (v, e) in norm64_grads(x, w, gy, half_params=True).items():
+        within(g[k], v, e, k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 3, 200])
+def test_a_vocabulary_projection(rows, dtype):
+    """An odd number of outputs, far more of them than anything else."""
+    x, w, b, _, gy = _problem(rows, 768, 50257, dtype, seed=12)
+    within(F.linear_forward(x, w, b), *linear64(x, w, b)[:2], "y")
+    g = F.linear_backward(x, w, gy)
+    for k, (v, e) in linear64_grads(x, w, b, gy).items():
+        within(g[k], v, e, k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+def test_gradients_of_more_than_32_bits_of_values(dtype):
+    """gz of 2^31 values and more, behind an activation: the gradients of rows at both ends as those rows by themselves."""
+    M, N, K = (1 << 18) + 24, 8192 + 8, 16
+    if dtype == F32:
+        M, N = (1 << 17) + 24, 16384 + 8
+    assert M * N > 1 << 31
+    x, w = _randn(M, K, dtype=dtype), _randn(N, K, seed=1, dtype=dtype)
+    gy = torch.empty(M, N, dtype=dtype, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(2))
+    _, tape = F.linear_forward(x, w, activation="silu", return_tape=True)
+    some = torch.tensor([0, 1, M // 2, M - 2, M - 1], device="cuda")
+    got = F.linear_backward(x, w, gy, tape=tape, activation="silu", want=("x", "bias"))
+    v, e = linear64_grads(x[some], w, None, gy[some], "silu")["x"]
+    within(got["x"][some], v, e, "grad x")
+    gy[:-2] = 0
+    got = F.linear_backward(x, w, gy, tape=tape, activation="silu", want=("weight", "bias"))
+    for k, (v, e) in linear64_grads(x[-2:], w, None, gy[-2:], "silu").items():
+        if k != "x":  # zeros add nothing to a sum, but the slices are cut otherwise
+            within(got[k], v, e * 4, k)
