@@ -83,9 +83,9 @@ def test_bfloat16_gradients_carry_one_rounding(size, act):
     the second derivative, some 2^-12 of gy in the mean. Beside the gradient's own rounding, 2^-9 and 2^-10 in the mean
     square, they add a few hundredths; gz rounded to bfloat16 would make it 1.41."""
     x, w, gy, _ = _tape_problem(*size, seed=40)
+    w = (w * size[1] ** -0.5).bfloat16()  # arguments of order one, where the slope is no constant
     _, tape = F.linear_forward(x, w, activation=act, return_tape=True)
-    tape = torch.randn_like(tape)  # arguments of order one, where the slope is no constant
-    want = _gradients64(x, w, gy, tape, act)
+    want = _gradients64(x, w, gy, x.double() @ w.double().t(), act)
     got = F.linear_backward(x, w, gy, tape=tape, activation=act)
     for k, v in want.items():
         assert _rounding_ratio(got[k], v) <= 1.05, k
