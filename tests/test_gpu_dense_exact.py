@@ -213,3 +213,20 @@ def test_status_of_a_device_and_in_training():
             enumerate(("train_input", "train_label", "test_input", "test_label"))}
     out = model.train_(data, steps=3, log=2, verbose=False)
     assert len(out["train_loss"]) == 3
+
+
+@pytest.mark.parametrize("D", [100, 768, 1037, 4096])
+def test_layer_norm_parameter_gradients_are_added_without_further_rounding(D):
+    """Some 300 partial sums of a few rows each. Added in order, K numbers carry sqrt(K / 6) steps of the root of their
+    squares' sum: eight rows or groups at most make 1.2, the last rounding 0.3, and for the weight the roundings in xhat 1.5 at
+    most; adding 300 of them in float32, 32 by 32, would bring 2.5 more."""
+    M = 600
+    x, w, gy = _randn(M, D), _randn(D, seed=1), _randn(M, D, seed=2)
+    _, stats = F.layer_norm_forward(x, w)
+    got = F.layer_norm_backward(x, w, stats, gy)
+    xd, gyd = x.double(), gy.double()
+    xc = xd - xd.mean(-1, keepdim=True)
+    xh = xc / torch.sqrt((xc * xc).mean(-1, keepdim=True) + 1e-5)
+    for name, terms, steps in (("bias", gyd, 1.3), ("weight", gyd * xh, 2.4)):
+        off = (got[name].double() - terms.sum(0)) / terms.square().sum(0).sqrt()
+        assert float(off.square().mean().sqrt()) <= steps * STEP, (name, float(off.square().mean().sqrt()) / STEP)
