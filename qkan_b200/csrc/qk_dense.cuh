@@ -107,7 +107,7 @@ __device__ __forceinline__ float activate(float z, int act) {
     }
 }
 // Beyond +-10^4 every derivative has reached its limit, which is what an infinite z (and one that the tape holds as such)
-// gets; a NaN passes.
+// gets; a NaN passes, but for relu, whose derivative is 1 above 0 and 0 elsewhere (torch's lets the gradient through at NaN).
 template <bool FAST>
 __device__ __forceinline__ float act_slope(float z, int act) {
     asm("{max.NaN.f32 %0, %0, %1;\n min.NaN.f32 %0, %0, %2;}" : "+f"(z) : "f"(-1e4f), "f"(1e4f));

@@ -73,10 +73,10 @@ __device__ __forceinline__ void load8(const void* p, size_t at, bool vec, int n,
     }
 }
 
-// Bound by memory: reads the source once, writes 2 (bfloat16) or 6 (float32) bytes per element. A thread owns eight
+// Bound by memory: reads the source once, writes 2 (bfloat16; gz in two parts 4) or 6 (float32) bytes per element. A thread owns eight
 // columns and walks the rows of a slab, so that column sums stay in its registers. Measured, x and gy of 65536 x 256 and a
-// small W in float32: 54 us for 336 MB, 6.2 TB/s; gz and its sums of 65536 x 256 in bfloat16 with SiLU: 29 us for 101 MB,
-// bound by the slope's instructions.
+// small W in float32: 54 us for 336 MB, 6.2 TB/s; gz in two parts and its sums, 16384 x 2048 in bfloat16 with SiLU: 59 us for
+// 268 MB (in one part 50 for 201), bound by the slope's instructions.
 template <typename IO>
 __global__ void __launch_bounds__(kThreads) prepare_kernel(const PrepArgsL a) {
     __shared__ float sums[kThreads * 8];

@@ -15,8 +15,8 @@
 // elements per thread. (With 16 elements per thread and weight and bias read again for every row, bfloat16 rows were bound by
 // instructions, at half of float32's bandwidth.)
 //
-// Measured: 16384 x 4096 float32 forward 87 us (6.2 TB/s), backward 138 us (5.8 TB/s); 65536 x 768 bfloat16 36.8 us (5.5 TB/s)
-// and 63.9 us (4.7 TB/s); 8192 x 768 bfloat16 4.9 us and 11.7 us, of which the second launch is 4; one row 1.4 us.
+// Measured: 16384 x 4096 float32 forward 87 us (6.2 TB/s), backward 139 us (5.8 TB/s); 65536 x 768 bfloat16 36.9 us (5.5 TB/s)
+// and 64.1 us (4.7 TB/s); 8192 x 768 bfloat16 5.2 us and 12.8 us, of which the second launch is 4; one row 1.7 us.
 #include <type_traits>
 
 #include "qk_dense.cuh"
@@ -315,7 +315,8 @@ __global__ void __launch_bounds__(block_of(T), 512 / block_of(T)) norm_backward_
 }
 
 // Rows wider than the registers of a group hold: one CTA per row, which reads the row once per pass (from L2 after the
-// first).
+// first), an element at a time, and is bound by those loads: 8192 x 16384 float32 forward 291 us (3.7 TB/s), backward 698
+// (2.3 TB/s), bfloat16 184 and 476. Kept simple: no model of the framework has such rows.
 template <typename IO>
 __global__ void __launch_bounds__(kWideThreads) norm_wide_forward_kernel(const NormArgs a) {
     after_previous();
