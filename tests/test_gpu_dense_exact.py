@@ -215,12 +215,11 @@ def test_status_of_a_device_and_in_training():
     assert len(out["train_loss"]) == 3
 
 
-@pytest.mark.parametrize("D", [100, 768, 1037, 4096])
-def test_layer_norm_parameter_gradients_are_added_without_further_rounding(D):
+@pytest.mark.parametrize("M,D", [(600, 100), (600, 768), (600, 1037), (600, 4096), (600, 9000), (8192, 9000)])
+def test_layer_norm_parameter_gradients_are_added_without_further_rounding(M, D):
     """Some 300 partial sums of a few rows each. Added in order, K numbers carry sqrt(K / 6) steps of the root of their
     squares' sum: eight rows or groups at most make 1.2, the last rounding 0.3, and for the weight the roundings in xhat 1.5 at
-    most; adding 300 of them in float32, 32 by 32, would bring 2.5 more."""
-    M = 600
+    most; adding 300 of them in float32, 32 by 32, would bring 2.5 more. Above 8192 columns a thread adds rows / 64, in double."""
     x, w, gy = _randn(M, D), _randn(D, seed=1), _randn(M, D, seed=2)
     _, stats = F.layer_norm_forward(x, w)
     got = F.layer_norm_backward(x, w, stats, gy)
@@ -230,3 +229,39 @@ def test_layer_norm_parameter_gradients_are_added_without_further_rounding(D):
     for name, terms, steps in (("bias", gyd, 1.3), ("weight", gyd * xh, 2.4)):
         off = (got[name].double() - terms.sum(0)) / terms.square().sum(0).sqrt()
         assert float(off.square().mean().sqrt()) <= steps * STEP, (name, float(off.square().mean().sqrt()) / STEP)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16"])
+def test_captures_that_fork_and_join(dtype):
+    """The operators on two streams of one capture, whose kernels each wait for what is before them on their own stream, and
+    for the other stream where it was told to."""
+    sizes = ((1, 64, 72), (8, 100, 30), (300, 256, 256), (700, 264, 520), (2100, 1032, 2056))
+    problems = [(_randn(M, K, dtype=dtype), _randn(N, K, dtype=dtype, scale=K ** -0.5), _randn(K, dtype=dtype)) for M, K, N in sizes]
+    side = torch.cuda.Stream()
+
+    def step(fork):
+        out = []
+        for x, w, n in problems:
+            here = torch.cuda.current_stream()
+            other = side if fork else here
+            other.wait_stream(here)
+            with torch.cuda.stream(other):
+                a, stats = F.layer_norm_forward(x, n)
+                g = F.layer_norm_backward(x, n, stats, x)["x"]
+            z, tape = F.linear_forward(x, w, activation="silu", return_tape=True)
+            here.wait_stream(other)
+            y = F.linear_forward(a, w, residual=z)
+            out += [y, *F.linear_backward(g, w, y, tape=tape, activation="silu").values()]
+        return out
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        replayed = step(True)
+    for seed in (1, 2):
+        for x, *_ in problems:
+            x.copy_(_randn(*x.shape, seed=seed, dtype=dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(replayed, step(False)):
+            assert torch.equal(a, b)
+        torch.cuda.synchronize()
