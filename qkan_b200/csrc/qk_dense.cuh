@@ -66,7 +66,7 @@ struct NormArgs {
     float* part;           // [2][slices][dim] partial sums of gw, gb
 };
 // slices of the backward's partial sums for this problem
-int norm_slices(int rows, int dim, int io_dtype);
+int norm_slices(int rows, int dim, int io_dtype, int param_dtype);
 cudaError_t launch_norm_forward(const NormArgs& a, cudaStream_t st);
 cudaError_t launch_norm_backward(const NormArgs& a, cudaStream_t st);
 

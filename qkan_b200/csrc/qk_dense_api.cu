@@ -54,7 +54,7 @@ int check_elements(std::initializer_list<const void*> all, size_t bytes, const c
 }
 
 size_t norm_scratch(const QkNormDesc& d) {
-    return qk::align256((size_t)2 * qk::norm_slices(d.rows, d.dim, d.io_dtype) * d.dim * sizeof(float));
+    return qk::align256((size_t)2 * qk::norm_slices(d.rows, d.dim, d.io_dtype, d.param_dtype) * d.dim * sizeof(float));
 }
 
 // a size of 0 says that the descriptor was refused, so "none" is 1
