@@ -158,10 +158,10 @@ __global__ void __launch_bounds__(kFewThreads) few_backward_kernel(const FewArgs
     __syncthreads();
     if (a.gb && block == 0)
         for (int n = threadIdx.x; n < count; n += kFewThreads) {
-            float s = 0.f;
+            double s = 0.;
 #pragma unroll
             for (int r = 0; r < R; ++r) s += gz[n][r];
-            store_dt(a.gb, n0 + n, a.io_dtype, s);
+            store_dt(a.gb, n0 + n, a.io_dtype, (float)s);
         }
     const long first = (long)block * kFewThreads * kFewCols + threadIdx.x * VEC;
     long col[kFewCols];

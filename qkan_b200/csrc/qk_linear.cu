@@ -143,9 +143,9 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const PrepArgsL a) {
     for (int t = threadIdx.x; t < width; t += kThreads) {
         const int col = (b - slab * j.cblocks) * width + t;
         if (col >= j.cols) break;
-        float s = 0.f;
+        double s = 0.;  // up to 256 of them in order
         for (int y = 0; y < ny; ++y) s += sums[y * width + t];
-        j.colpart[(size_t)slab * j.cols + col] = s;
+        j.colpart[(size_t)slab * j.cols + col] = (float)s;
     }
 }
 
@@ -164,10 +164,11 @@ struct ReduceArgs {
     int slabs, cols, io_dtype;
 };
 
-// The sum over `count` slices, n apart, of 32 neighbouring elements, by 256 threads; valid in the first 32 of them.
-__device__ __forceinline__ float tall_sum(const float* part, size_t n, size_t at, int count, float (&tile)[8][33]) {
+// The sum over `count` slices, n apart, of 32 neighbouring elements, by 256 threads; valid in the first 32 of them. In double:
+// some hundred float32 additions in order were most of grad_bias' error (1000 x 4096 -> 16 1.8e-7, torch's sums 8e-8).
+__device__ __forceinline__ float tall_sum(const float* part, size_t n, size_t at, int count, double (&tile)[8][33]) {
     const int x = threadIdx.x % 32, y = threadIdx.x / 32;
-    float s = 0.f;
+    double s = 0.;
     if (at < n) {
 #pragma unroll 8
         for (int k = y; k < count; k += 8) s += part[(size_t)k * n + at];
@@ -178,14 +179,14 @@ __device__ __forceinline__ float tall_sum(const float* part, size_t n, size_t at
 #pragma unroll
         for (int k = 1; k < 8; ++k) s += tile[k][x];
     }
-    return s;
+    return (float)s;
 }
 
 // The slices of each sum in a fixed order, then the epilogue: an element per thread, or (tall) 32 per CTA. The blocks
 // behind those add grad_bias' slabs, 32 columns each.
 __global__ void __launch_bounds__(kThreads) reduce_kernel(const ReduceArgs a) {
     after_previous();
-    __shared__ float tile[8][33];
+    __shared__ double tile[8][33];
     int b = blockIdx.x;
     ReduceJob j = a.job[0];
     bool sums = a.count > 0 && b < j.blocks;

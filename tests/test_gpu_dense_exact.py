@@ -1,5 +1,7 @@
 """What the dense operators' float64 comparisons with element bounds cannot see: values that are not finite, roundings that
 show in the mean square only, and which kernel a problem takes."""
+import math
+
 import pytest
 import torch
 
@@ -267,3 +269,20 @@ def test_captures_that_fork_and_join(dtype):
         for a, b in zip(replayed, step(False)):
             assert torch.equal(a, b)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("size", [(5, 64, 512), (16, 264, 4096), (40, 72, 520), (1000, 264, 16), (1000, 264, 520), (20000, 24, 16),
+                                  (20000, 24, 1001), (200000, 16, 16)], ids=lambda s: "x".join(map(str, s)))
+def test_float32_grad_bias_adds_few_numbers_in_order(size):
+    """A thread adds rows / (592 slabs x the threads beside it) values in float32, 16 in flight at most; all sums of those are in
+    double, each rounded once: sqrt(K / 6) steps for K of them, and 0.5."""
+    M, K, N = size
+    x, w, gy = _randn(M, K), _randn(N, K), _randn(M, N)
+    got = F.linear_backward(x, w, gy, want=("bias",))["bias"]
+    assert torch.equal(F.linear_backward(x, w, gy)["bias"], got)
+    groups = max(N, 64) / 8
+    beside = 256 / min(32, 2 ** math.ceil(math.log2(groups)))
+    rows = M / beside / max(1, min(592 / math.ceil(groups / 32), M / (4 * beside)))
+    off = (got.double() - gy.double().sum(0)) / gy.double().square().sum(0).sqrt()
+    steps = math.sqrt(max(rows, 4) / 6) + 0.5
+    assert float(off.square().mean().sqrt()) <= steps * STEP, (float(off.square().mean().sqrt()) / STEP, steps)
