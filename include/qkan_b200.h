@@ -291,7 +291,7 @@ typedef struct QkLinearPlan {
     int32_t tile_cols; /* 64, 128 or 256 */
     int32_t slices;    /* of the depth */
     int32_t blocks;    /* of 64 of the depth, per slice */
-    int32_t units;     /* tiles x slices, shared by 148 SMs */
+    int32_t units;     /* tiles x slices, shared by 148 SMs; INT32_MAX for that many and more */
     int32_t paired;    /* one launch for both gradients */
     int32_t gz_parts;  /* 1 or 2 (bfloat16), 3 (float32) */
     int32_t sums_bias; /* grad_bias comes with grad_weight's product */

@@ -522,7 +522,8 @@ QkLinearPlan linear_plan(const QkLinearDesc& d, int product) {
         if (s.two) p.gz_parts = 2;
     }
     p.tile_cols = plan.bn, p.slices = plan.cut.splits, p.blocks = plan.cut.kper;
-    p.units = (int)(Size{rows, product == 0 ? N : K, 0}.tiles(plan.bn) * plan.cut.splits);
+    const long units = Size{rows, product == 0 ? N : K, 0}.tiles(plan.bn) * plan.cut.splits;
+    p.units = units < INT32_MAX ? (int)units : INT32_MAX;
     return p;
 }
 

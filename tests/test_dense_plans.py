@@ -97,3 +97,13 @@ def test_eps_beyond_float32_is_refused():
     assert b"eps" in lib.qk_last_error()
     with pytest.raises(RuntimeError, match="no CPU fallback"):  # the last of the checks
         F.layer_norm(torch.zeros(2, 4), eps=3e38)
+
+
+def test_plans_of_the_largest_sizes():
+    most = 0x7fffff00
+    for dtype in (_abi.QK_F32, _abi.QK_BF16):
+        for size in ((most, 64, most), (most, most, 64), (64, most, most), (most, most, most)):
+            for product in range(3):
+                plan = _plan(product, *size, dtype=dtype)
+                assert plan.path == _abi.QK_LINEAR_TENSOR and plan.units >= 1 and plan.slices >= 1 and plan.blocks >= 1
+    assert _plan(0, most, 64, most).units == 2 ** 31 - 1
