@@ -41,7 +41,7 @@ __device__ __forceinline__ void split3(float x, float y, unsigned& h, unsigned& 
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(l) : "f"(y), "f"(x));
 }
 
-// x = h + m to within 2^-15 of x, for products that add both parts' to one sum. An infinity in the other operand has to give
+// x = h + m to within 2^-16 of x, for products that add both parts' to one sum. An infinity in the other operand has to give
 // an infinity there and not inf - inf or 0 * inf: so h is cut off, which leaves m the sign of x, and m is not zero beside an h
 // that is not (2^-24 of it, for |h| from 2^-109 on). Beside an infinite h m is infinite too.
 __device__ __forceinline__ void split2(float x, float y, unsigned& h, unsigned& m) {

@@ -81,7 +81,7 @@ def _rounding_ratio(got, want):
                                   (2100, 1032, 2056)], ids=lambda s: "x".join(map(str, s)))
 @pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
 def test_bfloat16_gradients_carry_one_rounding(size, act):
-    """gz in 15 bits or more and a tape in half: the first is off by 2^-15 at most, the second moves gz by 2^-11 |z| times
+    """gz in 16 bits or more and a tape in half: the first is off by 2^-16 at most, the second moves gz by 2^-11 |z| times
     the second derivative, some 2^-12 of gy in the mean. Beside the gradient's own rounding, 2^-9 and 2^-10 in the mean
     square, they add a few hundredths; gz rounded to bfloat16 would make it 1.41."""
     x, w, gy, _ = _tape_problem(*size, seed=40)
