@@ -258,7 +258,8 @@ typedef struct QkLinearDesc {
  * tape (M,N), NULL when no backward follows or the activation is QK_ACT_NONE: the argument of the activation, for
  * qk_linear_backward. It is float32 for QK_F32 and IEEE half for QK_BF16: three more bits than bfloat16 where the
  * activations bend; beyond half's range it is infinite, where every derivative has its limit, and relu's keeps the sign
- * of what is below it (its derivative is 1 above 0 and 0 elsewhere, at NaN too). Products and sums: float32, for QK_F32 to float32 accuracy.
+ * of what is below it (its derivative is 1 above 0 and 0 elsewhere, at NaN too). Products and sums: float32, for QK_F32
+ * to float32 accuracy.
  * in_features == 0 gives act(bias) + residual.
  */
 size_t qk_linear_forward_workspace_bytes(const QkLinearDesc* desc);

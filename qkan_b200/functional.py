@@ -563,6 +563,22 @@ def linear_backward(x, weight, gy, *, tape=None, activation="none", want=_GRADS,
     return _named(grads, want)
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, grads, *inputs):
+        return tuple(None if g is None else g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("the dense operators have no second derivatives: a gradient of theirs was differentiated")
+
+
+def _first_derivatives(grads, *inputs):
+    """Gradients as they leave a backward pass. With ``create_graph=True`` (calls are recorded there) differentiating them
+    again, with respect to any of the inputs that they depend on, has to raise."""
+    return _NoSecondDerivative.apply(grads, *inputs) if torch.is_grad_enabled() else grads
+
+
 class _LinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, code, round_grads):
@@ -572,7 +588,6 @@ class _LinearFunction(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
         _refuse_tangent(gy)
         x, weight, tape = ctx.saved_tensors
@@ -580,7 +595,7 @@ class _LinearFunction(torch.autograd.Function):
         want = need[0] + 2 * need[1] + 4 * need[2]
         grads = (_abi.dense().linear_backward(x, weight, gy, tape, ctx.code, want, ctx.round_grads) if want
                  else (None, None, None))
-        return (*grads, gy if need[3] else None, None, None)
+        return (*_first_derivatives(grads, x, weight, gy), gy if need[3] else None, None, None)
 
 
 def fused_linear(x, weight, bias=None, *, activation="none", residual=None, round_grads: bool = False) -> torch.Tensor:
@@ -624,12 +639,12 @@ class _LayerNormFunction(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
         _refuse_tangent(gy)
         x, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        return (*_abi.dense().norm_backward(x, weight, stats, gy, need[0] + 2 * need[1] + 4 * need[2], ctx.bias_dtype), None)
+        grads = _abi.dense().norm_backward(x, weight, stats, gy, need[0] + 2 * need[1] + 4 * need[2], ctx.bias_dtype)
+        return (*_first_derivatives(grads, x, weight, gy), None)
 
 
 def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5) -> torch.Tensor:

@@ -82,3 +82,32 @@ def test_gradients_asked_for_by_any_iterable(want):
     for form in (tuple, list, iter, lambda names: (name for name in names), dict.fromkeys):
         assert list(F.layer_norm_backward(x, None, stats, gy, want=form(want))) == list(want)
         assert list(F.linear_backward(x, w, torch.randn(3, 5), want=form(want))) == list(want)
+
+
+@pytest.mark.parametrize("f", [lambda t: F.fused_linear(t, w), F.layer_norm])
+def test_second_derivatives_are_refused_and_not_zero(f):
+    """With create_graph=True, also where the output's gradient is a constant."""
+    leaf = x.clone().requires_grad_(True)
+    plain, = torch.autograd.grad(f(leaf).sum(), leaf)
+    assert not plain.requires_grad
+    for loss in (f(leaf).sum(), f(leaf).square().sum()):
+        g, = torch.autograd.grad(loss, leaf, create_graph=True)
+        assert g.requires_grad and torch.isfinite(g).all()
+        with pytest.raises(RuntimeError, match="no second derivatives"):
+            (g.square().sum() + leaf.sum()).backward()
+    g, = torch.autograd.grad(f(leaf).sum(), leaf, create_graph=True)
+    assert torch.equal(g, plain)
+    leaf.grad = None
+    f(leaf).sum().backward(create_graph=True)  # asked for and not used
+    assert torch.equal(leaf.grad.detach(), plain)
+    with pytest.raises(RuntimeError, match="no second derivatives"):
+        torch.autograd.functional.hessian(lambda t: f(t).sum(), x)
+
+
+def test_the_residuals_gradient_is_differentiable_as_it_is():
+    leaf, r = x.clone().requires_grad_(True), torch.randn(3, 5, requires_grad=True)
+    y = F.fused_linear(leaf, w, residual=r) + r
+    gr, = torch.autograd.grad((y * r.detach().clone().requires_grad_(True)).sum(), r, create_graph=True)
+    assert gr.requires_grad
+    again, = torch.autograd.grad(y.square().sum(), r, create_graph=True)
+    assert torch.autograd.grad(again.sum(), r)[0].shape == r.shape
