@@ -31,6 +31,8 @@
 // rounding. Where hh's sum is not finite the small products are left out: float32's own infinities come out.
 #pragma once
 
+#include <atomic>
+
 #include "qk_linear.cuh"
 
 namespace qk {
@@ -733,15 +735,20 @@ cudaError_t launch_tile(const GemmArgs& a, cudaStream_t st) {
     return g.row_sums ? cudaErrorInvalidValue : launch_shape<BN, PLANES, kPlain>(a, st);
 }
 
-// adds this unit's count of waits that ran out, and clears it; synchronises the stream
+// Adds this unit's waits that ran out since the last call; synchronises the stream. The count on the device only grows, and
+// what was reported of it is kept here: clearing it would lose a wait of another stream between the read and the write.
 inline cudaError_t take_gave_up(unsigned* total, cudaStream_t st) {
+    static std::atomic<unsigned> reported[64];
+    int dev = 0;
     unsigned n = 0;
-    const unsigned zero = 0;
-    cudaError_t e = cudaMemcpyFromSymbolAsync(&n, g_gave_up, sizeof n, 0, cudaMemcpyDeviceToHost, st);
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(&n, g_gave_up, sizeof n, 0, cudaMemcpyDeviceToHost, st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-    if (e == cudaSuccess && n) e = cudaMemcpyToSymbolAsync(g_gave_up, &zero, sizeof n, 0, cudaMemcpyHostToDevice, st);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-    *total += n;
+    if (e != cudaSuccess) return e;
+    unsigned before = reported[dev & 63].load();
+    while (n > before && !reported[dev & 63].compare_exchange_weak(before, n)) {
+    }
+    if (n > before) *total += n - before;
     return e;
 }
 
